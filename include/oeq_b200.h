@@ -39,7 +39,7 @@ enum {
 };
 
 enum { OEQ_MODE_UVU = 0, OEQ_MODE_UVW = 1 };
-enum { OEQ_F32 = 0, OEQ_F64 = 1 };
+enum { OEQ_F32 = 0, OEQ_F64 = 1, OEQ_BF16 = 2, OEQ_F16 = 3 }; /* 16-bit types: linear maps of row groups only */
 
 /* One entry of an Irreps: mul copies of (l, parity).
  * Reference: openequivariance/implementations/e3nn_lite.py:157-188. */
@@ -208,6 +208,50 @@ int oeq_conv_double_backward(oeq_conv* h, int64_t nodes, int64_t edges, const vo
                              const void* dZ, const void* EX, const void* EY, const void* EW, const int64_t* rows,
                              const int64_t* cols, const int64_t* sender_perm, void* GX, void* GY, void* GW, void* GdZ,
                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- row groups --------------------------------------------------------------------
+ * A batch whose rows belong to groups (chemical elements, the systems of a batch, experts) is described by
+ *   order  [rows]       int64: the rows in the order of their groups, equal groups in the order of the rows; rows whose group
+ *                       is not in 0 .. groups - 1 belong to none and come last
+ *   slots  [rows]       int64: the position of each row in `order`
+ *   offsets[groups + 1] int64: position of the first row of each group; offsets[groups] = rows that have a group
+ *   blocks [oeq_row_groups_blocks][3] int32: (group, first position, number of rows) of each run of 64 sorted rows of a
+ *                       group, its last run being shorter; unused entries, all behind the others, are (-1, 0, 0)
+ * Everything is computed on the GPU; sizes depend on rows and groups alone.  At most 2^31 - 1 rows and OEQ_MOST_GROUPS groups.
+ * The reference has no counterpart. */
+#define OEQ_MOST_GROUPS 8191
+int64_t oeq_row_groups_blocks(int64_t rows, int64_t groups);
+size_t oeq_row_groups_workspace_bytes(int64_t rows, int64_t groups);
+/* From the group of each row (index [rows], int64). */
+int oeq_row_groups(int64_t rows, int64_t groups, const int64_t* index, int64_t* order, int64_t* slots, int64_t* offsets,
+                   int32_t* blocks, void* workspace, size_t workspace_bytes, void* stream);
+/* From the number of rows of each group (counts [groups], int64; below zero counts as zero) when the rows lie in the order
+ * of their groups: index [rows] is the group of each row, -1 behind the last group's rows.  Groups are cut off at the last
+ * row. */
+int oeq_row_groups_from_counts(int64_t rows, int64_t groups, const int64_t* counts, int64_t* index, int64_t* offsets,
+                               int32_t* blocks, void* stream);
+
+/* ---- linear maps of irreps with the weights of a row's group -------------------------
+ * Z[r,o,w,k] = c sum over input blocks i with the irrep of o and channels u of W[group of r][i,o][u,w] X[r,i,u,k], where
+ * 1 / c^2 is the number of channels summed.  W is [groups][weight_numel]: the paths (i, o) with i outermost, each
+ * [channels of i][channels of o].  Rows without a group get zeros.  dtype: OEQ_F32, OEQ_BF16, OEQ_F16
+ * (FP32 sums, rounded once), OEQ_F64.  `order` may be NULL when the rows lie in the order of their groups.
+ * A handle holds no device memory: calls on one may run on any streams and threads at once. */
+typedef struct oeq_grouped oeq_grouped;
+int oeq_grouped_create(const oeq_irrep* in, int n_in, const oeq_irrep* out, int n_out, oeq_grouped** handle);
+int oeq_grouped_destroy(oeq_grouped* h);
+int64_t oeq_grouped_weight_numel(const oeq_grouped* h);
+int oeq_grouped_forward(oeq_grouped* h, int dtype, int64_t rows, int64_t groups, const void* X, const void* W,
+                        const int64_t* order, const int64_t* offsets, const int32_t* blocks, void* Z, void* stream);
+/* dX from dZ and W; every row of dX is written. */
+int oeq_grouped_backward_input(oeq_grouped* h, int dtype, int64_t rows, int64_t groups, const void* dZ, const void* W,
+                               const int64_t* order, const int64_t* offsets, const int32_t* blocks, void* dX, void* stream);
+/* dW from X and dZ, every weight of every group (zeros for groups without rows), summed in a fixed order.  The workspace
+ * (oeq_grouped_workspace_bytes, of the current device) is free again after the call's launches. */
+size_t oeq_grouped_workspace_bytes(const oeq_grouped* h, int dtype, int64_t rows, int64_t groups);
+int oeq_grouped_backward_weights(oeq_grouped* h, int dtype, int64_t rows, int64_t groups, const void* X, const void* dZ,
+                                 const int64_t* order, const int64_t* offsets, void* dW, void* workspace,
+                                 size_t workspace_bytes, void* stream);
 
 /* Exercises the error path of the kernels' bounded waits without harming the device: one thread polls a barrier
  * that nothing completes `polls` times (at most 2^20), gives up, and the call reports what oeq_*_check would report,

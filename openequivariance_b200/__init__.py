@@ -14,7 +14,8 @@ from .wigner import wigner_3j
 
 __all__ = ["Irrep", "Irreps", "TPProblem", "Instruction", "FullyConnectedTPProblem",
            "ChannelwiseTPP", "SingleInstruction", "wigner_3j", "TensorProduct",
-           "TensorProductConv", "LoopUnrollTP", "LoopUnrollConv", "CoordGraph"]
+           "TensorProductConv", "LoopUnrollTP", "LoopUnrollConv", "CoordGraph",
+           "RowGroups", "GroupedLinear"]
 
 
 def __getattr__(name):
@@ -27,4 +28,7 @@ def __getattr__(name):
         from . import conv
         return {"TensorProductConv": conv.TensorProductConv, "LoopUnrollConv": conv.TensorProductConv,
                 "CoordGraph": conv.CoordGraph}[name]
+    if name in ("RowGroups", "GroupedLinear"):
+        from . import grouped
+        return getattr(grouped, name)
     raise AttributeError(name)

@@ -80,6 +80,17 @@ SYMBOLS = {
     "oeq_conv_last_backward_launches": (_INT, [_P]),
     "oeq_conv_has_double_backward": (_INT, [_P]),
     "oeq_conv_double_backward": (_INT, [_P, _I64, _I64] + [_P] * 14 + [_P, _SZ, _P]),
+    "oeq_row_groups_blocks": (_I64, [_I64, _I64]),
+    "oeq_row_groups_workspace_bytes": (_SZ, [_I64, _I64]),
+    "oeq_row_groups": (_INT, [_I64, _I64, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "oeq_row_groups_from_counts": (_INT, [_I64, _I64, _P, _P, _P, _P, _P]),
+    "oeq_grouped_create": (_INT, [C.POINTER(_Irrep), _INT, C.POINTER(_Irrep), _INT, C.POINTER(_P)]),
+    "oeq_grouped_destroy": (_INT, [_P]),
+    "oeq_grouped_weight_numel": (_I64, [_P]),
+    "oeq_grouped_forward": (_INT, [_P, _INT, _I64, _I64, _P, _P, _P, _P, _P, _P, _P]),
+    "oeq_grouped_backward_input": (_INT, [_P, _INT, _I64, _I64, _P, _P, _P, _P, _P, _P, _P]),
+    "oeq_grouped_workspace_bytes": (_SZ, [_P, _INT, _I64, _I64]),
+    "oeq_grouped_backward_weights": (_INT, [_P, _INT, _I64, _I64, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "oeq_selftest_bounded_wait": (_INT, [_INT, _P]),
     "oeq_tp_launch_info": (_INT, [_P, _INT, _PI, _PI, _PI, _PI, _PI, _PI]),
     "oeq_conv_launch_info": (_INT, [_P, _INT, _PI, _PI, _PI, _PI, _PI, _PI]),
@@ -112,13 +123,9 @@ _torch_lib = None
 _registered = []    # handles of the registered ops: an op can be called as long as the process lives
 
 
-def register_ops(forward, gradient, handle, *, deterministic=False, shared=False, has_weights=True, f64=False, dims=(),
-                 second=None):
-    """Register the torch ops ``openequivariance_b200::<forward>`` and ``::<gradient>`` of one operator (native kernels
-    and autograd, ``csrc/oeq_torch.cpp``) and return their overloads.  ``dims``: x, y, z row lengths and the number of
-    weights; ``second``: an op already registered that may replace the second derivatives (``call_second``)."""
+def torch_lib():
+    """Load (building first if needed) the library of the torch ops."""
     global _torch_lib
-    import torch
     lib()
     with _lock:
         if _torch_lib is None:
@@ -128,7 +135,19 @@ def register_ops(forward, gradient, handle, *, deterministic=False, shared=False
             t.oeq_torch_register.argtypes = [C.c_char_p] * 3 + [_P, _P] + [_INT] * 4 + [_I64] * 4
             t.oeq_torch_call_second.argtypes = [C.c_char_p, _INT]
             t.oeq_torch_conv_gradients.argtypes = [C.c_char_p] + [_I64] * 2 + [_P] * 14 + [C.POINTER(_I64), C.POINTER(_P)]
+            t.oeq_torch_grouped_error.restype = C.c_char_p
+            t.oeq_torch_grouped_register.restype, t.oeq_torch_grouped_register.argtypes = _I64, [_P, _I64, _I64]
             _torch_lib = t
+    return _torch_lib
+
+
+def register_ops(forward, gradient, handle, *, deterministic=False, shared=False, has_weights=True, f64=False, dims=(),
+                 second=None):
+    """Register the torch ops ``openequivariance_b200::<forward>`` and ``::<gradient>`` of one operator (native kernels
+    and autograd, ``csrc/oeq_torch.cpp``) and return their overloads.  ``dims``: x, y, z row lengths and the number of
+    weights; ``second``: an op already registered that may replace the second derivatives (``call_second``)."""
+    import torch
+    torch_lib()
     is_conv = isinstance(handle, ConvHandle)
     code = _torch_lib.oeq_torch_register(forward.encode(), gradient.encode(), second.encode() if second else None,
                                          None if is_conv else handle.ptr, handle.ptr if is_conv else None,

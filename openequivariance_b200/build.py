@@ -15,7 +15,10 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liboeq_b200.so")
-SOURCES = ["oeq_runtime.cu"]
+SOURCES = ["oeq_runtime.cu", "oeq_grouped.cu"]
+TORCH_SOURCES = ["oeq_torch.cpp", "oeq_torch_grouped.cpp"]
+# headers of the kernels that are compiled with the library (those of the others are read at run time)
+INCLUDED = ["oeq_internal.h", "oeq_common.cuh", "tc_common.cuh", "grouped_kernels.cuh", "row_groups_kernels.cuh"]
 
 
 def _nvcc() -> str:
@@ -68,7 +71,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     sources = [os.path.join(CSRC, s) for s in SOURCES]
 
     def command(out):
-        cmd = [_nvcc(), "-O2", "-std=c++17", "-shared", "-Xcompiler", "-fPIC", "-lineinfo",
+        cmd = [_nvcc(), "-O2", "-std=c++17", "--threads", "0", "-shared", "-Xcompiler", "-fPIC", "-lineinfo",
                "-gencode", "arch=compute_100a,code=sm_100a", "-cudart", "static", "-o", out] + sources + ["-ldl"]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
@@ -76,7 +79,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
             cmd.insert(1, "-DOEQ_DEV_PROFILE")      # development build: cycle accounting inside the kernels
         return cmd
 
-    return _build(LIB, sources + [HEADER], command, verbose, force)
+    return _build(LIB, sources + [os.path.join(CSRC, h) for h in INCLUDED] + [HEADER], command, verbose, force)
 
 
 def torch_library_path() -> str:
@@ -92,18 +95,19 @@ def build_torch_library(force: bool = False, verbose: bool = False) -> str:
     root = os.path.dirname(torch.__file__)
     include = os.path.join(root, "include")
     cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
-    source = os.path.join(CSRC, "oeq_torch.cpp")
+    sources = [os.path.join(CSRC, s) for s in TORCH_SOURCES]
 
     # The host compiler that nvcc uses, not $CXX: the library hands C++ objects to and from torch and has to share its
     # libstdc++.  With a second copy linked in, the first number written to a stream (an error message) ends the process.
     def command(out):
         return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
                 f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + include,
-                "-I" + os.path.join(include, "torch", "csrc", "api", "include"), "-I" + cuda, source, "-o", out,
+                "-I" + os.path.join(include, "torch", "csrc", "api", "include"), "-I" + cuda] + sources + ["-o", out,
                 "-L" + os.path.join(root, "lib"), "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
                 "-L" + HERE, "-l:" + os.path.basename(lib), "-Wl,-rpath,$ORIGIN"]
 
-    return _build(torch_library_path(), [source, HEADER, os.path.abspath(__file__)], command, verbose, force)
+    deps = sources + [os.path.join(CSRC, "oeq_torch_common.h"), HEADER, os.path.abspath(__file__)]
+    return _build(torch_library_path(), deps, command, verbose, force)
 
 
 if __name__ == "__main__":

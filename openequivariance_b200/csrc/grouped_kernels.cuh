@@ -1,0 +1,277 @@
+// Linear maps of irreps with one set of weights for each group of rows, on the FMA units: every type, every degree.
+//
+//   Z[r,o,w,k] = c_o sum_{i,u} W_g[i,o][u,w] X[r,i,u,k],  g = group of row r          (product; dX with W transposed)
+//   dW_g[i,o][u,w] = c_o sum_{r in g, k} X[r,i,u,k] dZ[r,o,w,k]                        (weight gradient)
+//
+// Both kernels are 64 x 64 register-tiled products with 4 x 4 values
+// per thread; 16 steps of the sum are staged in shared memory while the next 16 are on their way in registers.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "oeq_common.cuh"
+
+namespace oeq {
+
+constexpr int GP_BLOCKS = 32, GP_PATHS = 64;    // blocks of an Irreps and paths that fit the kernels' parameters
+
+struct GpPath {
+    int src, src_mul, src_off;  // source block, its multiplicity and first column
+    int w_off, w_ld;            // first weight; weights between neighbouring input channels
+    int dst;                    // target block
+};
+struct GpTarget {
+    int off, mul, d;            // first column, multiplicity, components
+    int path_begin, path_end;
+    double scale;
+};
+// A linear map from a source row to a target row.
+struct GpProblem {
+    int n_targets, n_paths, src_dim, dst_dim, w_numel;
+    bool transposed;            // the sum runs over the weights' output channels
+    GpTarget target[GP_BLOCKS];
+    GpPath path[GP_PATHS];
+};
+
+// ---- types: sums are held in FP32, those of FP64 values in FP64
+template <class T> struct GpAcc { typedef float type; };
+template <> struct GpAcc<double> { typedef double type; };
+__device__ __forceinline__ float gp_load(const float* p) { return __ldg(p); }
+__device__ __forceinline__ double gp_load(const double* p) { return __ldg(p); }
+__device__ __forceinline__ float gp_load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float gp_load(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ void gp_store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void gp_store(double* p, double v) { *p = v; }
+__device__ __forceinline__ void gp_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void gp_store(__half* p, float v) { *p = __float2half_rn(v); }
+
+// The last group g in [0, groups) with offsets[g] <= p; p < offsets[groups].
+__device__ __forceinline__ int gp_group(const long long* __restrict__ offsets, int groups, long long p) {
+    int lo = 0, hi = groups - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (__ldg(offsets + mid) <= p) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+__device__ __forceinline__ long long gp_row(const long long* __restrict__ order, long long p) { return order ? __ldg(order + p) : p; }
+
+// The grouped rows are cut into `parts` equal ranges of sorted positions.
+__device__ __forceinline__ long long gp_cut(long long n, int part, int parts) { return (long long)((unsigned long long)n * part / parts); }
+// The range that position p of n is in.
+__device__ __forceinline__ int gp_part(long long n, long long p, int parts) { return (int)(((unsigned long long)(p + 1) * parts - 1) / (unsigned long long)n); }
+
+constexpr int GP_TILE = 64, GP_STEP = 16, GP_SIMT_THREADS = 256;
+
+// acc[4][4] += a[k][row] b[k][col] over GP_STEP staged steps
+template <class A>
+__device__ __forceinline__ void gp_multiply(const A (*a)[GP_TILE], const A (*b)[GP_TILE], int r0, int c0, A (&acc)[4][4]) {
+#pragma unroll
+    for (int k = 0; k < GP_STEP; ++k) {
+        A x[4], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = a[k][r0 + i];
+            y[i] = b[k][c0 + i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] += x[i] * y[j];
+    }
+}
+
+// ---------------------------------------------------------------------------- product
+// CTA (x, y): entry x of the block table and column y; a column is a target block, 64 of its channels and 64 of the block's up
+// to 64 d (row, component) pairs.  Row y of the grid behind the table writes the zeros of the rows without a group.
+template <class T>
+__global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt(const __grid_constant__ GpProblem gp, const T* __restrict__ X, const T* __restrict__ W,
+                                                                    const long long* __restrict__ order, const long long* __restrict__ offsets,
+                                                                    const int* __restrict__ table, int blocks, long long rows, int groups,
+                                                                    T* __restrict__ Z) {
+    typedef typename GpAcc<T>::type A;
+    __shared__ __align__(16) A sa[GP_STEP][GP_TILE], sb[GP_STEP][GP_TILE];
+    const int tid = threadIdx.x;
+    if ((int)blockIdx.x >= blocks) {            // rows without a group: zeros
+        const long long n = min(__ldg(offsets + groups), rows), part = (long long)(blockIdx.x - blocks) * gridDim.y + blockIdx.y;
+        const long long parts = (long long)(gridDim.x - blocks) * gridDim.y;
+        for (long long i = part * blockDim.x + tid; i < (rows - n) * gp.dst_dim; i += parts * blockDim.x)
+            gp_store(Z + gp_row(order, n + i / gp.dst_dim) * gp.dst_dim + i % gp.dst_dim, A(0));
+        return;
+    }
+    const int g = table[3 * blockIdx.x], n_rows = table[3 * blockIdx.x + 2];
+    const long long first = table[3 * blockIdx.x + 1];
+    if (g < 0) return;
+    int t = 0, column = blockIdx.y;
+    for (; t < gp.n_targets; ++t) {
+        const int n = (gp.target[t].mul + GP_TILE - 1) / GP_TILE * gp.target[t].d;
+        if (column < n) break;
+        column -= n;
+    }
+    const GpTarget& to = gp.target[t];
+    const int d = to.d, pair0 = column % d * GP_TILE, pairs = n_rows * d, c_tile = column / d * GP_TILE;
+    if (pair0 >= pairs) return;
+    // staging: thread -> (step, 4 rows apart) of A and of B
+    const int k_a = tid % GP_STEP, r_a = tid / GP_STEP;
+    const T* x_row[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int pair = pair0 + r_a + 16 * i;
+        x_row[i] = pair < pairs ? X + gp_row(order, first + pair / d) * gp.src_dim + pair % d : nullptr;
+    }
+    const T* w_group = W + (long long)g * gp.w_numel;
+    const int kb = gp.transposed ? tid % GP_STEP : tid / 16 % GP_STEP, cb = gp.transposed ? tid / GP_STEP : tid % 16;
+    A acc[4][4] = {}, a[4], b[4];
+    const int r0 = tid / 16 * 4, c0 = tid % 16 * 4;
+    int p = to.path_begin, u0 = 0;
+    auto fetch = [&] {
+        const GpPath& path = gp.path[p];
+        const T* w = w_group + path.w_off;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int u = u0 + k_a;
+            a[i] = x_row[i] && u < path.src_mul ? (A)gp_load(x_row[i] + path.src_off + u * d) : A(0);
+            const int v = u0 + kb, c = c_tile + cb + 16 * i;
+            b[i] = v < path.src_mul && c < to.mul ? (A)gp_load(w + (gp.transposed ? (long long)c * path.w_ld + v : (long long)v * path.w_ld + c)) : A(0);
+        }
+        u0 += GP_STEP;
+        if (u0 >= path.src_mul) {
+            ++p;
+            u0 = 0;
+        }
+    };
+    if (p < to.path_end) fetch();
+    for (bool more = to.path_begin < to.path_end; more;) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sa[k_a][r_a + 16 * i] = a[i];
+            sb[kb][cb + 16 * i] = b[i];
+        }
+        __syncthreads();
+        more = p < to.path_end;
+        if (more) fetch();
+        gp_multiply(sa, sb, r0, c0, acc);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int pair = pair0 + r0 + i;
+        if (pair >= pairs) break;
+        T* z = Z + gp_row(order, first + pair / d) * gp.dst_dim + to.off + pair % d;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c_tile + c0 + j < to.mul) gp_store(z + (c_tile + c0 + j) * d, (A)(acc[i][j] * (A)to.scale));
+    }
+}
+
+// ---------------------------------------------------------------------------- weight gradient
+// A CTA has a path, a tile of its weights and a range of the sorted rows.  A group that lies within the range is complete; the part of
+// one that began before it goes to slot 0 of the CTA's two partial tiles, the part of one that goes on behind it to slot 1.
+// oeq_grouped_join adds the parts in the order of the ranges: no atomics, the same sums in every run.
+struct GpSplit {
+    int parts[GP_PATHS];        // ranges of each path
+    int first[GP_PATHS + 1];    // its first CTA
+};
+template <class T>
+__global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __grid_constant__ GpProblem gp, const __grid_constant__ GpSplit split,
+                                                                       const T* __restrict__ X, const T* __restrict__ dZ,
+                                                                       const long long* __restrict__ order, const long long* __restrict__ offsets,
+                                                                       long long rows, int groups, T* __restrict__ dW,
+                                                                       typename GpAcc<T>::type* __restrict__ partial) {
+    typedef typename GpAcc<T>::type A;
+    __shared__ __align__(16) A sa[GP_STEP][GP_TILE], sb[GP_STEP][GP_TILE];
+    const int tid = threadIdx.x;
+    int p = 0;
+    while ((int)blockIdx.x >= split.first[p + 1]) ++p;
+    const GpPath& path = gp.path[p];
+    const GpTarget& to = gp.target[path.dst];
+    const int parts = split.parts[p], part = ((int)blockIdx.x - split.first[p]) % parts, tile_of = ((int)blockIdx.x - split.first[p]) / parts;
+    const int w_tiles = (to.mul + GP_TILE - 1) / GP_TILE, u_tile = tile_of / w_tiles * GP_TILE, w_tile = tile_of % w_tiles * GP_TILE, d = to.d;
+    const long long n = min(__ldg(offsets + groups), rows);
+    if (n == 0) return;
+    const long long lo = gp_cut(n, part, parts), hi = gp_cut(n, part + 1, parts);
+    if (lo >= hi) return;
+    const int k_s = tid / 16, c_s = tid % 16, r0 = tid / 16 * 4, c0 = tid % 16 * 4;
+    int g = gp_group(offsets, groups, lo);
+    for (long long at = lo; at < hi;) {
+        long long begin = __ldg(offsets + g), end = __ldg(offsets + g + 1);
+        if (end <= at) {                        // (a group without rows)
+            ++g;
+            continue;
+        }
+        const long long stop = min(end, hi);
+        const long long pairs = (stop - at) * d;
+        A acc[4][4] = {}, a[4], b[4];
+        auto fetch = [&](long long k0) {
+            const long long k = k0 + k_s;
+            const bool in = k < pairs;
+            const long long row = in ? gp_row(order, at + k / d) : 0;
+            const T *x = X + row * gp.src_dim + path.src_off + k % d, *z = dZ + row * gp.dst_dim + to.off + k % d;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int u = u_tile + c_s + 16 * i, w = w_tile + c_s + 16 * i;
+                a[i] = in && u < path.src_mul ? (A)gp_load(x + u * d) : A(0);
+                b[i] = in && w < to.mul ? (A)gp_load(z + w * d) : A(0);
+            }
+        };
+        fetch(0);
+        for (long long k0 = 0; k0 < pairs; k0 += GP_STEP) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sa[k_s][c_s + 16 * i] = a[i];
+                sb[k_s][c_s + 16 * i] = b[i];
+            }
+            __syncthreads();
+            if (k0 + GP_STEP < pairs) fetch(k0 + GP_STEP);
+            gp_multiply(sa, sb, r0, c0, acc);
+        }
+        const bool whole = begin >= lo && end <= hi;
+        A* tile = whole ? nullptr : partial + ((long long)blockIdx.x * 2 + (begin < lo ? 0 : 1)) * (GP_TILE * GP_TILE);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int u = u_tile + r0 + i, w = w_tile + c0 + j;
+                if (!whole) tile[(r0 + i) * GP_TILE + c0 + j] = acc[i][j];
+                else if (u < path.src_mul && w < to.mul)
+                    gp_store(dW + (long long)g * gp.w_numel + path.w_off + (long long)u * path.w_ld + w, (A)(acc[i][j] * (A)to.scale));
+            }
+        at = stop;
+        ++g;
+    }
+}
+
+// Gradients of the groups that no single range has: the sum of their parts, and zeros where there are no rows.
+// Blocks x over the weights, y over the groups.
+template <class T>
+__global__ void __launch_bounds__(256) oeq_grouped_join(const __grid_constant__ GpProblem gp, const __grid_constant__ GpSplit split,
+                                                        const long long* __restrict__ offsets, long long rows, int groups, int tile_u, int tile_w,
+                                                        const typename GpAcc<T>::type* __restrict__ partial, T* __restrict__ dW) {
+    typedef typename GpAcc<T>::type A;
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= gp.w_numel) return;
+    int p = 0;
+    while (p + 1 < gp.n_paths && i >= gp.path[p + 1].w_off) ++p;           // (the paths lie in the order of their weights)
+    const GpPath& path = gp.path[p];
+    const int parts = split.parts[p], u = (i - path.w_off) / path.w_ld, w = (i - path.w_off) % path.w_ld;
+    const long long tile = (long long)tile_u * tile_w, n = min(__ldg(offsets + groups), rows);
+    const A* at = partial + (split.first[p] + (long long)(u / tile_u * ((path.w_ld + tile_w - 1) / tile_w) + w / tile_w) * parts) * 2 * tile +
+                  (long long)(u % tile_u) * tile_w + w % tile_w;
+    for (int g = blockIdx.y; g < groups; g += gridDim.y) {
+        const long long begin = min(__ldg(offsets + g), n), end = min(__ldg(offsets + g + 1), n);
+        A s = A(0);
+        if (begin < end) {
+            const int j0 = gp_part(n, begin, parts), j1 = gp_part(n, end - 1, parts);
+            if (j0 == j1) continue;
+            s = at[(j0 * 2 + 1) * tile];
+            for (int j = j0 + 1; j <= j1; ++j)
+                if (n >= parts || gp_cut(n, j, parts) < gp_cut(n, j + 1, parts)) s += at[j * 2 * tile];    // (a range without rows has no part)
+            s *= (A)gp.target[path.dst].scale;
+        }
+        gp_store(dW + (long long)g * gp.w_numel + i, s);
+    }
+}
+
+}  // namespace oeq

@@ -1,0 +1,320 @@
+// Row groups and linear maps with the weights of a row's group: the host side behind include/oeq_b200.h.
+//
+// The kernels are compiled with the library (their shapes are run-time values); nothing here allocates device memory, synchronises or
+// keeps anything of a call.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+#include <vector>
+
+#include "../../include/oeq_b200.h"
+#include "oeq_internal.h"
+#include "grouped_kernels.cuh"
+#include "row_groups_kernels.cuh"
+
+using namespace oeq;
+
+namespace {
+
+#define OEQ_CUDA(expr)                                                                                                  \
+    do {                                                                                                                \
+        cudaError_t e_ = (expr);                                                                                        \
+        if (e_ != cudaSuccess) return oeq_fail(OEQ_ERR_CUDA, std::string(#expr) + ": " + cudaGetErrorString(e_));       \
+    } while (0)
+
+constexpr int64_t MOST_ROWS = (int64_t(1) << 31) - 1;
+constexpr size_t SMEM_MOST = 227 * 1024;
+
+size_t elem_bytes(int dtype) { return dtype == OEQ_F64 ? 8 : (dtype == OEQ_F32 ? 4 : 2); }
+bool known_dtype(int dtype) { return dtype == OEQ_F32 || dtype == OEQ_F64 || dtype == OEQ_BF16 || dtype == OEQ_F16; }
+
+int sm_count(int& n) {
+    static int counts[64] = {};         // of the devices; a race writes the same value twice
+    int dev = 0;
+    OEQ_CUDA(cudaGetDevice(&dev));
+    if (dev < 64 && counts[dev]) {
+        n = counts[dev];
+        return OEQ_OK;
+    }
+    OEQ_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < 64) counts[dev] = n;
+    return OEQ_OK;
+}
+
+// Shared memory beyond 48 KB has to be allowed once for a kernel and device; asked for in every call that needs it.
+template <class K>
+int allow_smem(K kernel, size_t bytes) {
+    if (bytes > 48 * 1024) OEQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    return OEQ_OK;
+}
+
+int check_groups(int64_t rows, int64_t groups) {
+    if (rows < 0 || rows > MOST_ROWS) return oeq_fail(OEQ_ERR_INVALID, "rows must be in 0 .. 2^31 - 1");
+    if (groups < 1 || groups > OEQ_MOST_GROUPS) return oeq_fail(OEQ_ERR_INVALID, "groups must be in 1 .. " + std::to_string(OEQ_MOST_GROUPS));
+    return OEQ_OK;
+}
+
+// ---------------------------------------------------------------------------- row groups
+size_t small_smem(int64_t groups) { return (RG_SMALL_WARPS * (groups + 1) + 2 * (groups + 2) + 33) * sizeof(int); }
+// One CTA walks 32 rows a step in each of its warps; beyond these many rows the runs of many CTAs are faster.
+bool small_groups(int64_t rows, int64_t groups) { return rows <= 8192 && small_smem(groups) <= SMEM_MOST; }
+struct Runs {
+    int64_t run;        // rows of a run
+    int runs;
+};
+Runs runs_of(int64_t rows) {
+    const int64_t run = std::max<int64_t>(256, ((rows + 1183) / 1184 + 31) / 32 * 32);
+    return {run, (int)std::max<int64_t>(1, (rows + run - 1) / run)};
+}
+
+// ---------------------------------------------------------------------------- linear maps
+
+}  // namespace
+
+struct oeq_grouped {
+    GpProblem forward, backward, weights;       // X -> Z, dZ -> dX, and X -> Z with the paths in the order of their weights
+    int d_max = 0;
+};
+
+namespace {
+
+int column_count(const GpProblem& gp) {
+    int n = 0;
+    for (int t = 0; t < gp.n_targets; ++t) n += (gp.target[t].mul + GP_TILE - 1) / GP_TILE * gp.target[t].d;
+    return n;
+}
+
+template <class T>
+int simt_product(const GpProblem& gp, int64_t rows, int64_t groups, const void* X, const void* W, const int64_t* order, const int64_t* offsets,
+                 const int32_t* blocks, void* Z, cudaStream_t st) {
+    const int n = (int)oeq_row_groups_blocks(rows, groups), columns = column_count(gp);
+    if (columns == 0) return OEQ_OK;
+    int sms = 0;
+    if (int rc = sm_count(sms)) return rc;
+    const dim3 grid((unsigned)(n + (sms + columns - 1) / columns), (unsigned)columns);
+    oeq_grouped_simt<T><<<grid, GP_SIMT_THREADS, 0, st>>>(gp, (const T*)X, (const T*)W, (const long long*)order, (const long long*)offsets, blocks, n, rows,
+                                                          (int)groups, (T*)Z);
+    OEQ_CUDA(cudaGetLastError());
+    return OEQ_OK;
+}
+
+// Ranges of rows: about four CTAs an SM, 64 rows and more each.
+GpSplit simt_split(const GpProblem& gp, int64_t rows, int sms) {
+    GpSplit s{};
+    int columns = 0;
+    auto tiles = [&](int p) { return (gp.path[p].src_mul + GP_TILE - 1) / GP_TILE * ((gp.target[gp.path[p].dst].mul + GP_TILE - 1) / GP_TILE); };
+    for (int p = 0; p < gp.n_paths; ++p) columns += tiles(p);
+    const int parts = (int)std::max<int64_t>(1, std::min<int64_t>((4 * sms + columns - 1) / std::max(1, columns), rows / 64));
+    for (int p = 0; p < gp.n_paths; ++p) {
+        s.parts[p] = parts;
+        s.first[p + 1] = s.first[p] + tiles(p) * parts;
+    }
+    return s;
+}
+
+template <class T>
+int join(const GpProblem& gp, const GpSplit& split, int tile_u, int tile_w, int64_t rows, int64_t groups, const int64_t* offsets, void* dW, const void* ws,
+         cudaStream_t st) {
+    const dim3 grid((unsigned)((gp.w_numel + 255) / 256), (unsigned)std::min<int64_t>(groups, 1024));
+    oeq_grouped_join<T><<<grid, 256, 0, st>>>(gp, split, (const long long*)offsets, rows, (int)groups, tile_u, tile_w, (const typename GpAcc<T>::type*)ws, (T*)dW);
+    OEQ_CUDA(cudaGetLastError());
+    return OEQ_OK;
+}
+
+template <class T>
+int simt_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* X, const void* dZ, const int64_t* order, const int64_t* offsets, void* dW,
+                 void* ws, cudaStream_t st) {
+    int sms = 0;
+    if (int rc = sm_count(sms)) return rc;
+    const GpSplit split = simt_split(gp, rows, sms);
+    if (rows > 0) {
+        oeq_grouped_simt_dw<T><<<split.first[gp.n_paths], GP_SIMT_THREADS, 0, st>>>(gp, split, (const T*)X, (const T*)dZ, (const long long*)order,
+                                                                                    (const long long*)offsets, rows, (int)groups, (T*)dW,
+                                                                                    (typename GpAcc<T>::type*)ws);
+        OEQ_CUDA(cudaGetLastError());
+    }
+    return join<T>(gp, split, GP_TILE, GP_TILE, rows, groups, offsets, dW, ws, st);
+}
+
+int check_call(const oeq_grouped* h, int dtype, int64_t rows, int64_t groups) {
+    if (!h) return oeq_fail(OEQ_ERR_INVALID, "null handle");
+    if (!known_dtype(dtype)) return oeq_fail(OEQ_ERR_INVALID, "unknown dtype");
+    return check_groups(rows, groups);
+}
+
+int product(const GpProblem& gp, int dtype, int64_t rows, int64_t groups, const void* X, const void* W, const int64_t* order, const int64_t* offsets,
+            const int32_t* blocks, void* Z, void* stream) {
+    if (rows == 0 || gp.dst_dim == 0) return OEQ_OK;
+    if (!offsets || !blocks || !Z || (gp.src_dim && !X) || (gp.w_numel && !W)) return oeq_fail(OEQ_ERR_INVALID, "null pointer");
+    const cudaStream_t st = (cudaStream_t)stream;
+    switch (dtype) {
+        case OEQ_F64: return simt_product<double>(gp, rows, groups, X, W, order, offsets, blocks, Z, st);
+        case OEQ_F32: return simt_product<float>(gp, rows, groups, X, W, order, offsets, blocks, Z, st);
+        case OEQ_BF16: return simt_product<__nv_bfloat16>(gp, rows, groups, X, W, order, offsets, blocks, Z, st);
+        default: return simt_product<__half>(gp, rows, groups, X, W, order, offsets, blocks, Z, st);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t oeq_row_groups_blocks(int64_t rows, int64_t groups) { return rows / RG_BLOCK + std::min(rows, groups); }
+
+size_t oeq_row_groups_workspace_bytes(int64_t rows, int64_t groups) {
+    if (rows < 0 || groups < 1 || small_groups(rows, groups)) return 0;
+    return ((size_t)runs_of(rows).runs + 1) * (size_t)(groups + 1) * sizeof(int);
+}
+
+int oeq_row_groups(int64_t rows, int64_t groups, const int64_t* index, int64_t* order, int64_t* slots, int64_t* offsets, int32_t* blocks, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+    if (int rc = check_groups(rows, groups)) return rc;
+    if (!offsets || (rows > 0 && (!index || !order || !slots || !blocks))) return oeq_fail(OEQ_ERR_INVALID, "null pointer");
+    if (oeq_row_groups_workspace_bytes(rows, groups) > workspace_bytes || (oeq_row_groups_workspace_bytes(rows, groups) && !workspace))
+        return oeq_fail(OEQ_ERR_INVALID, "workspace too small");
+    const cudaStream_t st = (cudaStream_t)stream;
+    const int n = (int)oeq_row_groups_blocks(rows, groups), keys = (int)groups + 1;
+    const long long* in = (const long long*)index;
+    long long *ord = (long long*)order, *slt = (long long*)slots, *off = (long long*)offsets;
+    if (small_groups(rows, groups)) {
+        const size_t smem = small_smem(groups);
+        if (int rc = allow_smem(oeq_row_groups_small, smem)) return rc;
+        oeq_row_groups_small<<<1, 32 * RG_SMALL_WARPS, smem, st>>>(in, (int)rows, (int)groups, n, ord, slt, off, blocks);
+    } else {
+        const Runs r = runs_of(rows);
+        int *counts = (int*)workspace, *totals = counts + (size_t)r.runs * keys;
+        const unsigned ctas = (unsigned)((r.runs + RG_WARPS - 1) / RG_WARPS);
+        const size_t smem = (size_t)RG_WARPS * keys * sizeof(int), smem_place = smem + (2 * (groups + 2) + 33) * sizeof(int);
+        if (int rc = allow_smem(oeq_row_groups_count, smem)) return rc;
+        if (int rc = allow_smem(oeq_row_groups_place, smem_place)) return rc;
+        oeq_row_groups_count<<<ctas, 32 * RG_WARPS, smem, st>>>(in, rows, r.run, r.runs, (int)groups, counts);
+        OEQ_CUDA(cudaGetLastError());
+        oeq_row_groups_scan<<<(unsigned)((keys + 31) / 32), 1024, 0, st>>>(counts, totals, r.runs, keys);
+        OEQ_CUDA(cudaGetLastError());
+        oeq_row_groups_place<<<ctas, 32 * RG_WARPS, smem_place, st>>>(in, rows, r.run, r.runs, (int)groups, n, counts, totals, ord, slt, off, blocks);
+    }
+    OEQ_CUDA(cudaGetLastError());
+    return OEQ_OK;
+}
+
+int oeq_row_groups_from_counts(int64_t rows, int64_t groups, const int64_t* counts, int64_t* index, int64_t* offsets, int32_t* blocks, void* stream) {
+    if (int rc = check_groups(rows, groups)) return rc;
+    if (!counts || !offsets || (rows > 0 && (!index || !blocks))) return oeq_fail(OEQ_ERR_INVALID, "null pointer");
+    const int n = (int)oeq_row_groups_blocks(rows, groups);
+    const size_t smem = (2 * (groups + 2) + 33) * sizeof(int);
+    if (int rc = allow_smem(oeq_row_groups_counts, smem)) return rc;
+    const unsigned ctas = (unsigned)std::min<int64_t>(296, std::max<int64_t>(1, (rows + 511) / 512));
+    oeq_row_groups_counts<<<ctas, 512, smem, (cudaStream_t)stream>>>((const long long*)counts, rows, (int)groups, n, (long long*)index, (long long*)offsets, blocks);
+    OEQ_CUDA(cudaGetLastError());
+    return OEQ_OK;
+}
+
+int oeq_grouped_create(const oeq_irrep* in, int n_in, const oeq_irrep* out, int n_out, oeq_grouped** handle) {
+    if (!handle || n_in < 0 || n_out < 0 || (n_in && !in) || (n_out && !out)) return oeq_fail(OEQ_ERR_INVALID, "null or negative argument");
+    *handle = nullptr;
+    if (n_in > GP_BLOCKS || n_out > GP_BLOCKS)
+        return oeq_fail(OEQ_ERR_UNSUPPORTED, "at most " + std::to_string(GP_BLOCKS) + " blocks of irreps on each side (join blocks of one irrep)");
+    struct Block { int64_t off; int mul, l, parity; };
+    std::vector<Block> a, b;
+    auto lay_out = [](const oeq_irrep* src, int n, std::vector<Block>& to, int64_t& dim) {
+        dim = 0;
+        for (int i = 0; i < n; ++i) {
+            if (src[i].mul < 0 || src[i].l < 0 || src[i].l > 64 || (src[i].parity != 1 && src[i].parity != -1)) return false;
+            to.push_back({dim, src[i].mul, src[i].l, src[i].parity});
+            dim += (int64_t)src[i].mul * (2 * src[i].l + 1);
+        }
+        return dim < (int64_t(1) << 24);
+    };
+    int64_t a_dim = 0, b_dim = 0, numel = 0;
+    if (!lay_out(in, n_in, a, a_dim) || !lay_out(out, n_out, b, b_dim)) return oeq_fail(OEQ_ERR_INVALID, "malformed irreps");
+    struct Path { int i, o; int64_t w; };
+    std::vector<Path> paths;
+    for (int i = 0; i < n_in; ++i)
+        for (int o = 0; o < n_out; ++o)
+            if (a[i].l == b[o].l && a[i].parity == b[o].parity && a[i].mul && b[o].mul) {
+                paths.push_back({i, o, numel});
+                numel += (int64_t)a[i].mul * b[o].mul;
+            }
+    if (paths.size() > (size_t)GP_PATHS) return oeq_fail(OEQ_ERR_UNSUPPORTED, "at most " + std::to_string(GP_PATHS) + " paths (join blocks of one irrep)");
+    if (numel >= (int64_t(1) << 30)) return oeq_fail(OEQ_ERR_UNSUPPORTED, "2^30 weights of a group or more");
+    // 1 / sqrt(channels that are summed): the same for every path of an irrep, so that the gradients have it too
+    auto scale = [&](const Block& x) {
+        int64_t n = 0;
+        for (const Block& y : a) n += y.l == x.l && y.parity == x.parity ? y.mul : 0;
+        return n ? 1.0 / std::sqrt((double)n) : 0.0;
+    };
+    oeq_grouped* h = new oeq_grouped();
+    auto fill = [&](GpProblem& gp, const std::vector<Block>& dst, int64_t src_dim, int64_t dst_dim, bool transposed) {
+        gp.n_targets = (int)dst.size();
+        gp.src_dim = (int)src_dim;
+        gp.dst_dim = (int)dst_dim;
+        gp.w_numel = (int)numel;
+        gp.transposed = transposed;
+        int n = 0;
+        for (int t = 0; t < gp.n_targets; ++t) {
+            GpTarget& to = gp.target[t];
+            to = {(int)dst[t].off, dst[t].mul, 2 * dst[t].l + 1, n, n, scale(dst[t])};
+            for (const Path& p : paths)
+                if ((transposed ? p.i : p.o) == t) {
+                    const Block& src = transposed ? b[p.o] : a[p.i];
+                    gp.path[n++] = {transposed ? p.o : p.i, src.mul, (int)src.off, (int)p.w, b[p.o].mul, t};
+                }
+            to.path_end = n;
+        }
+        gp.n_paths = n;
+    };
+    fill(h->forward, b, a_dim, b_dim, false);
+    fill(h->backward, a, b_dim, a_dim, true);
+    h->weights = h->forward;
+    std::sort(h->weights.path, h->weights.path + h->weights.n_paths, [](const GpPath& x, const GpPath& y) { return x.w_off < y.w_off; });
+    for (const Path& p : paths) h->d_max = std::max(h->d_max, 2 * a[p.i].l + 1);
+    *handle = h;
+    return OEQ_OK;
+}
+
+int oeq_grouped_destroy(oeq_grouped* h) {
+    delete h;
+    return OEQ_OK;
+}
+
+int64_t oeq_grouped_weight_numel(const oeq_grouped* h) { return h ? h->forward.w_numel : 0; }
+
+int oeq_grouped_forward(oeq_grouped* h, int dtype, int64_t rows, int64_t groups, const void* X, const void* W, const int64_t* order, const int64_t* offsets,
+                        const int32_t* blocks, void* Z, void* stream) {
+    if (int rc = check_call(h, dtype, rows, groups)) return rc;
+    return product(h->forward, dtype, rows, groups, X, W, order, offsets, blocks, Z, stream);
+}
+
+int oeq_grouped_backward_input(oeq_grouped* h, int dtype, int64_t rows, int64_t groups, const void* dZ, const void* W, const int64_t* order,
+                               const int64_t* offsets, const int32_t* blocks, void* dX, void* stream) {
+    if (int rc = check_call(h, dtype, rows, groups)) return rc;
+    return product(h->backward, dtype, rows, groups, dZ, W, order, offsets, blocks, dX, stream);
+}
+
+size_t oeq_grouped_workspace_bytes(const oeq_grouped* h, int dtype, int64_t rows, int64_t groups) {
+    int sms = 0;
+    if (!h || rows <= 0 || !known_dtype(dtype) || h->forward.n_paths == 0 || sm_count(sms)) return 0;
+    const GpSplit s = simt_split(h->weights, rows, sms);
+    return (size_t)s.first[h->weights.n_paths] * 2 * GP_TILE * GP_TILE * std::max<size_t>(4, elem_bytes(dtype));
+}
+
+int oeq_grouped_backward_weights(oeq_grouped* h, int dtype, int64_t rows, int64_t groups, const void* X, const void* dZ, const int64_t* order,
+                                 const int64_t* offsets, void* dW, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = check_call(h, dtype, rows, groups)) return rc;
+    const GpProblem& gp = h->weights;
+    if (gp.w_numel == 0) return OEQ_OK;
+    if (!offsets || !dW || (rows > 0 && (!X || !dZ))) return oeq_fail(OEQ_ERR_INVALID, "null pointer");
+    const size_t want = oeq_grouped_workspace_bytes(h, dtype, rows, groups);
+    if (workspace_bytes < want || (want && !workspace)) return oeq_fail(OEQ_ERR_INVALID, "workspace too small");
+    const cudaStream_t st = (cudaStream_t)stream;
+    switch (dtype) {
+        case OEQ_F64: return simt_weights<double>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st);
+        case OEQ_F32: return simt_weights<float>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st);
+        case OEQ_BF16: return simt_weights<__nv_bfloat16>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st);
+        default: return simt_weights<__half>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st);
+    }
+}
+
+}  // extern "C"

@@ -34,6 +34,7 @@
 
 #include "../../include/oeq_b200.h"
 #include "oeq_common.cuh"
+#include "oeq_internal.h"
 
 namespace {
 
@@ -2191,6 +2192,8 @@ struct oeq_conv {
     int* d_status = nullptr;
     cudaStream_t last_stream = nullptr;
 };
+
+int oeq_fail(int code, const std::string& message) { return fail(code, message); }
 
 extern "C" {
 

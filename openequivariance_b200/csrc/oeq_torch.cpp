@@ -23,11 +23,15 @@
 #include <string>
 #include <vector>
 
-#include "../../include/oeq_b200.h"
+#include "oeq_torch_common.h"
 
 namespace {
 
 using at::Tensor;
+using oeq_torch::Args;
+using oeq_torch::check;
+using oeq_torch::direct;
+using oeq_torch::index_ptr;
 using c10::OperatorHandle;
 using c10::Stack;
 using torch::autograd::variable_list;
@@ -50,10 +54,6 @@ struct Op {
     std::mutex mutex;
     std::map<c10::DeviceIndex, Kept> kept;  // large backward scratch
 };
-
-void check(int rc) { TORCH_CHECK(rc == OEQ_OK, "oeq_b200: ", oeq_last_error()); }
-
-typedef at::ArrayRef<Tensor> Args;
 
 void check_inputs(const Op& op, Args in) {
     const int n = (int)in.size();
@@ -83,8 +83,6 @@ void check_inputs(const Op& op, Args in) {
         TORCH_CHECK_VALUE(w.scalar_type() == op.dtype, "tensors must be ", op.dtype);
     }
 }
-
-const int64_t* index_ptr(const Tensor& t) { return static_cast<const int64_t*>(t.const_data_ptr()); }
 
 // ---------------------------------------------------------------- CUDA kernels
 
@@ -257,21 +255,6 @@ variable_list conv_second(Op& op, at::ArrayRef<Tensor> in, at::ArrayRef<Tensor> 
 
 // ---------------------------------------------------------------- autograd
 
-// The gradients that an autograd node computes.  Plain CUDA tensors that nothing differentiates go straight to the
-// kernels; anything else (tracing modes, tensor subclasses, batched tensors, negated or zero tensors whose memory does not
-// hold their values, derivatives of the derivative) through the dispatcher.
-bool direct(Args in) {
-    using c10::DispatchKey;
-    const auto tls = c10::impl::tls_local_dispatch_key_set().included_;
-    if (at::GradMode::is_enabled() || tls.has(DispatchKey::Python) || tls.has(DispatchKey::PythonTLSSnapshot) ||
-        tls.has(DispatchKey::FuncTorchDynamicLayerFrontMode) || tls.has(DispatchKey::Functionalize))
-        return false;
-    // keys of a dense CUDA tensor; a tensor with any other one is not plain
-    static const uint64_t plain = c10::DispatchKeySet({DispatchKey::CUDA, DispatchKey::ADInplaceOrView, DispatchKey::AutogradCUDA, DispatchKey::AutocastCUDA}).raw_repr();
-    for (const Tensor& t : in)
-        if (!t.defined() || !t.is_cuda() || (t.key_set().raw_repr() & ~plain) != 0) return false;
-    return true;
-}
 Tensor call_forward(const Op& op, Args in) {
     if (direct(in)) return forward_cuda(op, in);
     Stack stack(in.begin(), in.end());

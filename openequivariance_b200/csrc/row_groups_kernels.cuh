@@ -1,0 +1,249 @@
+// Row groups: a stable counting sort of the rows of a batch by their group, the offsets of the groups among the sorted rows
+// and the table of blocks of up to 64 sorted rows of one group.
+//
+//   order[p] = the row at sorted position p, slots[r] = the position of row r, offsets[g] = rows of groups before g.
+//   Rows whose group is not in 0..groups-1 come last (key `groups`).
+//
+// A warp takes a run of rows, 32 at a time.  Lanes with the same key find each other (match_any): a row's rank is the number
+// of earlier rows of its key in the run, counted in shared memory, plus those of lower lanes, so equal keys keep their
+// order without atomics, and every result is the same in every run.
+//   * few rows: one CTA counts, scans and places in one launch (row_groups_small);
+//   * many rows: count (a histogram per run), scan (the runs' histograms, a key per lane), place (every CTA adds up the keys).
+#pragma once
+#include "oeq_common.cuh"
+
+namespace oeq {
+
+constexpr int RG_BLOCK = 64;                    // rows of an entry of the block table
+constexpr int RG_SMALL_WARPS = 32, RG_WARPS = 4;
+
+__device__ __forceinline__ int rg_key(const long long* __restrict__ index, long long r, int groups) {
+    const long long g = index[r];
+    return g >= 0 && g < groups ? (int)g : groups;
+}
+
+// Exclusive sums over a[0..n) in shared memory, a[n] = total, by all threads of the CTA; `part` holds 33 ints.
+__device__ __forceinline__ void rg_scan(int* a, int n, int* part) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int before = 0;
+    for (int i0 = 0; i0 < n; i0 += blockDim.x) {
+        const int i = i0 + threadIdx.x, v = i < n ? a[i] : 0;
+        int s = v;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, s, off);
+            if (lane >= off) s += t;
+        }
+        if (lane == 31) part[warp] = s;
+        __syncthreads();
+        if (warp == 0) {
+            int t = lane < warps ? part[lane] : 0;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, t, off);
+                if (lane >= off) t += u;
+            }
+            if (lane < warps) part[lane] = t;
+        }
+        __syncthreads();
+        const int up = before + (warp ? part[warp - 1] : 0) + s - v;
+        before += part[warps - 1];
+        if (i < n) a[i] = up;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) a[n] = before;
+    __syncthreads();
+}
+
+// The last i with a[i] <= v, of a[0..n] ascending with a[0] <= v.
+__device__ __forceinline__ int rg_find(const int* a, int n, int v) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a[mid] <= v) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Offsets and the threads' share of the block table, from offsets[0..groups] in shared memory; `first` (groups + 1 ints) is
+// overwritten with the number of blocks before each group's.
+__device__ __forceinline__ void rg_tables(const int* offsets, int* first, int* part, int groups, int blocks, long long* __restrict__ offsets_out,
+                                          int* __restrict__ table, long long thread, long long threads) {
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) first[g] = (offsets[g + 1] - offsets[g] + RG_BLOCK - 1) / RG_BLOCK;
+    __syncthreads();
+    rg_scan(first, groups, part);
+    for (long long g = thread; g <= groups; g += threads) offsets_out[g] = offsets[g];
+    for (long long b = thread; b < blocks; b += threads) {
+        int g = -1, p = 0, n = 0;
+        if (b < first[groups]) {
+            g = rg_find(first, groups, (int)b);         // (of groups without rows between, the last starts at the same block)
+            p = offsets[g] + ((int)b - first[g]) * RG_BLOCK;
+            n = min(RG_BLOCK, offsets[g + 1] - p);
+        }
+        table[3 * b] = g;
+        table[3 * b + 1] = p;
+        table[3 * b + 2] = n;
+    }
+}
+
+// Rows [lo, hi) by one warp; visit(row, key, rank): rank among the rows of the key, count[] being what came before.
+template <class F>
+__device__ __forceinline__ void rg_walk(const long long* __restrict__ index, long long lo, long long hi, int groups, int* count, F&& visit) {
+    const int lane = threadIdx.x & 31;
+    constexpr int AHEAD = 4;                    // rows of a lane whose keys are loaded together
+    for (long long r0 = lo; r0 < hi; r0 += 32 * AHEAD) {
+        int key[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) key[i] = r0 + 32 * i + lane < hi ? rg_key(index, r0 + 32 * i + lane, groups) : -1;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const unsigned same = __match_any_sync(0xffffffffu, key[i]), lower = same & ((1u << lane) - 1);
+            const int before = key[i] >= 0 ? count[key[i]] : 0;
+            __syncwarp();
+            if (key[i] >= 0) {
+                visit(r0 + 32 * i + lane, key[i], before + __popc(lower));
+                if (lower == 0) count[key[i]] = before + __popc(same);
+            }
+            __syncwarp();
+        }
+    }
+}
+
+// ---- one CTA.  Shared memory: [32 warps][groups + 1] counts, [groups + 2] offsets, [groups + 2] blocks, 33 ints
+__global__ void __launch_bounds__(32 * RG_SMALL_WARPS) oeq_row_groups_small(const long long* __restrict__ index, int rows, int groups, int blocks,
+                                                                              long long* __restrict__ order, long long* __restrict__ slots,
+                                                                              long long* __restrict__ offsets, int* __restrict__ table) {
+    extern __shared__ int rg_smem[];
+    const int keys = groups + 1, tid = threadIdx.x, warp = tid >> 5;
+    int *offs = rg_smem + RG_SMALL_WARPS * keys, *first = offs + keys + 1, *part = first + keys + 1;
+    for (int i = tid; i < RG_SMALL_WARPS * keys; i += blockDim.x) rg_smem[i] = 0;
+    __syncthreads();
+    const int run = (rows + 32 * RG_SMALL_WARPS - 1) / (32 * RG_SMALL_WARPS) * 32, lo = min(warp * run, rows), hi = min(lo + run, rows);
+    int* mine = rg_smem + warp * keys;
+    rg_walk(index, lo, hi, groups, mine, [](long long, int, int) {});
+    __syncthreads();
+    for (int k = tid; k < keys; k += blockDim.x) {          // warps' counts -> rows of the key in the warps before
+        int s = 0;
+        for (int w = 0; w < RG_SMALL_WARPS; ++w) {
+            const int n = rg_smem[w * keys + k];
+            rg_smem[w * keys + k] = s;
+            s += n;
+        }
+        offs[k] = s;
+    }
+    __syncthreads();
+    rg_scan(offs, keys, part);
+    rg_walk(index, lo, hi, groups, mine, [&](long long r, int key, int rank) {
+        const int p = offs[key] + rank;
+        order[p] = r;
+        slots[r] = p;
+    });
+    rg_tables(offs, first, part, groups, blocks, offsets, table, tid, blockDim.x);
+}
+
+// ---- many rows: runs of `run` rows (a multiple of 32), one per warp; counts [runs][groups + 1], totals [groups + 1]
+__global__ void __launch_bounds__(32 * RG_WARPS) oeq_row_groups_count(const long long* __restrict__ index, long long rows, long long run, int runs,
+                                                                      int groups, int* __restrict__ counts) {
+    extern __shared__ int rg_smem[];
+    const int keys = groups + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.x * RG_WARPS + warp;
+    int* mine = rg_smem + warp * keys;
+    for (int k = lane; k < keys; k += 32) mine[k] = 0;
+    __syncwarp();
+    if (n >= runs) return;
+    const long long lo = n * run, hi = min(lo + run, rows);
+    rg_walk(index, lo, hi, groups, mine, [](long long, int, int) {});
+    for (int k = lane; k < keys; k += 32) counts[(long long)n * keys + k] = mine[k];
+}
+
+// counts[n][k] -> rows of key k in the runs before n.  A CTA takes 32 keys, a warp every 32nd part of the runs.
+__global__ void __launch_bounds__(1024) oeq_row_groups_scan(int* __restrict__ counts, int* __restrict__ totals, int runs, int keys) {
+    __shared__ int sums[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = blockIdx.x * 32 + lane;
+    const int each = (runs + 31) / 32, lo = min(warp * each, runs), hi = min(lo + each, runs);
+    int s = 0;
+    if (k < keys) {
+#pragma unroll 8
+        for (int n = lo; n < hi; ++n) s += counts[(long long)n * keys + k];
+    }
+    sums[warp][lane] = s;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < warp; ++w) before += sums[w][lane];
+    if (k < keys) {
+#pragma unroll 8
+        for (int n = lo; n < hi; ++n) {
+            const int c = counts[(long long)n * keys + k];
+            counts[(long long)n * keys + k] = before;
+            before += c;
+        }
+        if (warp == 31) totals[k] = before;
+    }
+}
+
+// Shared memory: [RG_WARPS][groups + 1] counts, [groups + 2] offsets, [groups + 2] blocks, 33 ints
+__global__ void __launch_bounds__(32 * RG_WARPS) oeq_row_groups_place(const long long* __restrict__ index, long long rows, long long run, int runs,
+                                                                      int groups, int blocks, const int* __restrict__ counts,
+                                                                      const int* __restrict__ totals, long long* __restrict__ order,
+                                                                      long long* __restrict__ slots, long long* __restrict__ offsets,
+                                                                      int* __restrict__ table) {
+    extern __shared__ int rg_smem[];
+    const int keys = groups + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.x * RG_WARPS + warp;
+    int *offs = rg_smem + RG_WARPS * keys, *first = offs + keys + 1, *part = first + keys + 1, *mine = rg_smem + warp * keys;
+    for (int k = threadIdx.x; k < keys; k += blockDim.x) offs[k] = totals[k];
+    __syncthreads();
+    rg_scan(offs, keys, part);
+    if (n < runs) {
+        for (int k = lane; k < keys; k += 32) mine[k] = offs[k] + counts[(long long)n * keys + k];
+        __syncwarp();
+        const long long lo = n * run, hi = min(lo + run, rows);
+        rg_walk(index, lo, hi, groups, mine, [&](long long r, int, int p) {
+            order[p] = r;
+            slots[r] = p;
+        });
+    }
+    rg_tables(offs, first, part, groups, blocks, offsets, table, (long long)blockIdx.x * blockDim.x + threadIdx.x, (long long)gridDim.x * blockDim.x);
+}
+
+// ---- rows that lie in the order of their groups, from the number of rows of each: groups that begin behind the last row end
+// there, and rows behind the last group belong to none.  Shared memory: [groups + 1] offsets, [groups + 2] blocks, 33 ints
+__global__ void __launch_bounds__(512) oeq_row_groups_counts(const long long* __restrict__ counts, long long rows, int groups, int blocks,
+                                                             long long* __restrict__ index, long long* __restrict__ offsets, int* __restrict__ table) {
+    extern __shared__ int rg_smem[];
+    int *offs = rg_smem, *first = offs + groups + 2, *part = first + groups + 2;
+    // (counts are clamped one by one and their sum stays below 2^31 by the scan of clamped partial sums below)
+    __shared__ long long carry[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    long long before = 0;
+    for (int i0 = 0; i0 < groups; i0 += blockDim.x) {
+        const int i = i0 + threadIdx.x;
+        long long v = i < groups ? counts[i] : 0;
+        v = v < 0 ? 0 : (v > rows ? rows : v);
+        long long s = v;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const long long t = __shfl_up_sync(0xffffffffu, s, off);
+            if (lane >= off) s += t;
+        }
+        if (lane == 31) carry[warp] = s;
+        __syncthreads();
+        long long up = before, all = before;
+        for (int w = 0; w < warps; ++w) {
+            if (w < warp) up += carry[w];
+            all += carry[w];
+        }
+        if (i < groups) offs[i + 1] = (int)min(up + s, rows);
+        before = all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) offs[0] = 0;
+    __syncthreads();
+    const long long thread = (long long)blockIdx.x * blockDim.x + threadIdx.x, threads = (long long)gridDim.x * blockDim.x;
+    rg_tables(offs, first, part, groups, blocks, offsets, table, thread, threads);
+    for (long long r = thread; r < rows; r += threads) {
+        const int g = rg_find(offs, groups, (int)r);
+        index[r] = g < groups ? g : -1;
+    }
+}
+
+}  // namespace oeq
