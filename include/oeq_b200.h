@@ -253,6 +253,10 @@ int oeq_grouped_backward_weights(oeq_grouped* h, int dtype, int64_t rows, int64_
                                  const int64_t* order, const int64_t* offsets, void* dW, void* workspace,
                                  size_t workspace_bytes, void* stream);
 
+/* Status of these kernels on the current device (synchronises it): OEQ_OK, or OEQ_ERR_DEVICE_WAIT once a kernel has abandoned a
+ * bounded wait. */
+int oeq_grouped_check(void);
+
 /* Exercises the error path of the kernels' bounded waits without harming the device: one thread polls a barrier
  * that nothing completes `polls` times (at most 2^20), gives up, and the call reports what oeq_*_check would report,
  * OEQ_ERR_DEVICE_WAIT.  The context stays usable.  No counterpart in the reference (its kernels have no waits). */

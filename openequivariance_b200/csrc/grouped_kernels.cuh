@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt(const __grid
     A acc[4][4] = {}, a[4], b[4];
     const int r0 = tid / 16 * 4, c0 = tid % 16 * 4;
     int p = to.path_begin, u0 = 0;
-    auto fetch = [&] {
+    auto fetch = [&]() {
         const GpPath& path = gp.path[p];
         const T* w = w_group + path.w_off;
 #pragma unroll

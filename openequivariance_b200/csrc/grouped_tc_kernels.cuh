@@ -1,0 +1,478 @@
+// Linear maps of irreps with one set of weights for each group of rows, on the 5th-generation tensor cores: FP32 (3xTF32),
+// BF16 and FP16, up to GT_D_MAX components.  FP32 accumulators.
+//
+//   Z[r,o,w,k] = c_o sum_{i,u} W_g[i,o][u,w] X[r,i,u,k],  g = group of row r; dX is the same with W transposed.
+//
+// As a matrix product: M = (row, component) pairs of sorted rows of one group, N = channels of one output block, K = channels of
+// the input blocks with its irrep.  A CTA has one output block (or a tile of its channels) and one range of the sorted rows, the
+// CTAs being dealt to the output blocks by cost, so a CTA meets few groups and keeps a group's weights in shared memory.
+//   * 16 producer warps: a lane reads the 16 d bytes of V = 4 (16-bit types: 8) channels of a row, [channel][component], and writes
+//     d pieces of 16 bytes, one per (row, component), K-major with the 128-byte swizzle.  The transposition that the layout of irreps
+//     asks for costs no extra pass, rows are gathered in sorted order, and FP32 values are split into TF32 hi and lo on the way.
+//     Weights have their output channels along memory: "MN-major" tiles for Z, K-major for dX; neither is transposed.
+//   * one warp, in step, issues the MMAs.  FP32: hi.hi and hi.lo as one MMA over the weights' hi channels followed by lo, lo.hi
+//     into hi.lo's columns: the large and the small products have accumulators of their own.
+//   * 4 epilogue warps add those, scale, and write rows through shared memory, so that a row's values leave in order.
+// Two accumulators: a tile drains while the next is computed.  Every wait is bounded; on expiry a role records a code and all
+// leave.
+#pragma once
+#include "grouped_kernels.cuh"
+#include "tc_common.cuh"
+
+namespace oeq {
+
+constexpr int GT_D_MAX = 9;
+constexpr int GT_PW = 16, GT_EPI = 4, GT_THREADS = (GT_PW + GT_EPI + 1) * 32;
+constexpr int GT_STAGES = 6;                    // most stages of A
+constexpr int GT_STAGING = 33 * 128 * 4;        // 32 channels of a tile's pairs
+constexpr int GT_CONTROL = 1024;                // barriers, the tile's rows
+constexpr int ERR_GT_EMPTY = 81, ERR_GT_FULL = 82, ERR_GT_ACC_FULL = 83, ERR_GT_ACC_EMPTY = 84;
+
+// Set by a kernel whose bounded wait ran out; read by oeq_grouped_check.
+__device__ int gt_status;
+
+struct GtTarget {
+    int n_tiles, n;             // tiles of its channels, channels of a tile (a multiple of 16)
+    int parts, first;           // ranges of rows, first CTA
+    int stages, slots;          // of A, of B
+    int chunks;                 // steps of the sum
+};
+struct GtProblem {
+    GpProblem gp;
+    GtTarget target[GP_BLOCKS];
+};
+
+template <class T> struct GtType {              // 16-bit
+    static constexpr int V = 8, KC = 64, KSTEP = 16, A_BYTES = 16384, N_MAX = 256;
+    static constexpr bool SPLIT = false;
+    __host__ __device__ static constexpr int b_bytes(int n) { return (n + 63) / 64 * 8192; }
+    __host__ __device__ static constexpr int acc(int n) { return n; }
+};
+template <> struct GtType<float> {
+    static constexpr int V = 4, KC = 32, KSTEP = 8, A_BYTES = 32768, N_MAX = 128;
+    static constexpr bool SPLIT = true;
+    __host__ __device__ static constexpr int b_bytes(int n) { return n * 256; }
+    __host__ __device__ static constexpr int acc(int n) { return 2 * n; }
+};
+
+// ---- instruction descriptor and MMA of the type; A is K-major
+template <class T, bool B_MN> __device__ __forceinline__ unsigned gt_idesc(int n) {
+    const unsigned fmt = GtType<T>::SPLIT ? 2u : (sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u);
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | (B_MN ? 1u << 16 : 0u) | ((unsigned)(n >> 3) << 17) | (8u << 24);
+}
+template <class T>
+__device__ __forceinline__ void gt_mma(unsigned leader, unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned accumulate) {
+    if constexpr (GtType<T>::SPLIT) {
+        tc_mma_if(leader, d, a, b, idesc, accumulate);
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u), "r"(leader)
+            : "memory");
+    }
+}
+// ---- operand B [n channels] x [KC steps of the sum]
+// K-major: rows of 128 bytes per channel, FP32: hi channels, then lo.  MN-major, FP32: per 8 steps, blocks of 32 channels by 8 steps
+// (128-byte rows, 32-byte atoms swizzled over four rows), hi channels then lo; 16-bit: per 8 steps, blocks of 64 channels by 8 steps.
+template <class T>
+__device__ __forceinline__ int gt_place_mn(int n, int ch, int k) {
+    if constexpr (GtType<T>::SPLIT) return (k >> 3) * (n * 64) + (ch >> 5) * 1024 + (k & 7) * 128 + (((ch & 31) * 4) ^ ((k & 3) << 5));
+    else return (k >> 3) * ((n + 63) / 64 * 1024) + (ch >> 6) * 1024 + (k & 7) * 128 + ((((ch >> 3) & 7) ^ (k & 7)) << 4);
+}
+template <class T, bool B_MN>
+__device__ __forceinline__ unsigned long long gt_desc_b(unsigned addr, int n) {
+    const unsigned long long base = (unsigned long long)((addr >> 4) & 0x3fff) | (unsigned long long)(1024 >> 4) << 16 | 1ull << 46;
+    if constexpr (!B_MN) return tc_smem_desc(addr);
+    else if constexpr (GtType<T>::SPLIT) return base | (unsigned long long)(512 >> 4) << 32 | 1ull << 61;
+    else return base | (unsigned long long)((n + 63) / 64 * 1024 >> 4) << 32 | 2ull << 61;
+}
+// bytes between two MMAs' steps
+template <class T, bool B_MN> __device__ __forceinline__ int gt_step_b(int n) {
+    if constexpr (!B_MN) return 32;
+    else return GtType<T>::SPLIT ? n * 64 : 2 * ((n + 63) / 64 * 1024);
+}
+
+// ---- values
+__device__ __forceinline__ void gt_split(const float4& v, float4& hi, float4& lo) {
+    hi = make_float4(tf32_hi(v.x), tf32_hi(v.y), tf32_hi(v.z), tf32_hi(v.w));
+    lo = make_float4(v.x - hi.x, v.y - hi.y, v.z - hi.z, v.w - hi.w);         // exact; read as TF32 by the MMA
+}
+// V channels of D components, as 16-byte words: `left` of the channels exist, the others are zero.
+template <class T, int D>
+__device__ __forceinline__ void gt_read(uint4 (&v)[D], const T* __restrict__ src, int left, bool vec) {
+    constexpr int V = GtType<T>::V;
+    if (vec && left >= V) {
+#pragma unroll
+        for (int i = 0; i < D; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        return;
+    }
+    unsigned* w = reinterpret_cast<unsigned*>(v);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4 * D; ++i) w[i] = i / D < left ? __float_as_uint(__ldg(reinterpret_cast<const float*>(src) + i)) : 0u;
+    } else {
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(src);
+#pragma unroll
+        for (int i = 0; i < 4 * D; ++i)
+            w[i] = (2 * i / D < left ? (unsigned)__ldg(h + 2 * i) : 0u) | ((2 * i + 1) / D < left ? (unsigned)__ldg(h + 2 * i + 1) << 16 : 0u);
+    }
+}
+// The V channels of component k.
+template <class T, int D>
+__device__ __forceinline__ uint4 gt_component(const uint4 (&v)[D], int k) {
+    const unsigned* w = reinterpret_cast<const unsigned*>(v);
+    if constexpr (sizeof(T) == 4) {
+        return make_uint4(w[k], w[D + k], w[2 * D + k], w[3 * D + k]);
+    } else {
+        unsigned o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int a = 2 * j * D + k, b = a + D;
+            o[j] = __byte_perm(w[a >> 1], w[b >> 1], (a & 1 ? 0x32 : 0x10) | (b & 1 ? 0x7600 : 0x5400));
+        }
+        return make_uint4(o[0], o[1], o[2], o[3]);
+    }
+}
+
+// ---- a CTA's tiles: up to 128 / d sorted rows of one group
+struct GtWalk {
+    long long pos, hi, end;     // next position, end of the range, end of the group within it
+    int g, rows;
+    __device__ GtWalk(const long long* offsets, int groups, long long lo, long long hi_) : pos(lo), hi(hi_), end(0), g(0), rows(0) {
+        if (lo < hi) {
+            g = gp_group(offsets, groups, lo);
+            end = min(__ldg(offsets + g + 1), hi);
+        }
+    }
+    __device__ bool more() const { return pos < hi; }
+    __device__ void tile(int most) { rows = (int)min((long long)most, end - pos); }
+    __device__ void next(const long long* offsets, int groups) {
+        pos += rows;
+        if (pos >= end && pos < hi) {
+            ++g;
+            end = __ldg(offsets + g + 1);
+            if (end <= pos) {                   // groups without rows between
+                g = gp_group(offsets, groups, pos);
+                end = __ldg(offsets + g + 1);
+            }
+            end = min(end, hi);
+        }
+    }
+};
+
+struct GtArgs {
+    const void *X, *W;
+    const long long *order, *offsets;
+    void* Z;
+    long long rows;
+    int groups;
+    int x_vec, w_vec, z_pair;   // 16-byte pieces of X and W, 4-byte pairs of 16-bit Z are aligned
+};
+struct GtBars {
+    unsigned long long *full, *empty, *acc_full, *acc_empty;
+    unsigned* tmem;
+    int* rows;                  // of the tile that drains
+    __device__ explicit GtBars(unsigned char* control) {
+        full = reinterpret_cast<unsigned long long*>(control);
+        empty = full + GT_STAGES;
+        acc_full = empty + GT_STAGES;
+        acc_empty = acc_full + 2;
+        tmem = reinterpret_cast<unsigned*>(acc_empty + 2);
+        rows = reinterpret_cast<int*>(control + 256);
+    }
+};
+
+// ---------------------------------------------------------------------------- producers
+template <class T, bool TRANS>
+__device__ __forceinline__ void gt_fill_b(unsigned char* dst, const T* __restrict__ w, int ld, int n, int n_left, int k_left, int k_fill, bool vec, int tid) {
+    constexpr int V = GtType<T>::V, KC = GtType<T>::KC;
+    auto put = [&](const uint4 (&v)[1], int at, int at_lo) {
+        if constexpr (GtType<T>::SPLIT) {
+            float4 hi, lo;
+            gt_split(*reinterpret_cast<const float4*>(v), hi, lo);
+            *reinterpret_cast<float4*>(dst + at) = hi;
+            *reinterpret_cast<float4*>(dst + at_lo) = lo;
+        } else {
+            *reinterpret_cast<uint4*>(dst + at) = v[0];
+        }
+    };
+    if constexpr (TRANS) {      // channel ch of the input: W[ch][k], K-major
+#pragma unroll 2
+        for (int i = tid; i < n * 8; i += GT_PW * 32) {
+            const int ch = i >> 3, c = i & 7;
+            if (V * c < k_fill) {
+                uint4 v[1];
+                gt_read<T, 1>(v, w + (long long)ch * ld + V * c, ch < n_left ? k_left - V * c : 0, vec);
+                const int at = tc_swizzle(ch, 4 * c);
+                put(v, at, at + n * 128);
+            }
+        }
+    } else {                    // W[k][ch], MN-major
+        const int pieces = n / V;
+#pragma unroll 2
+        for (int i = tid; i < KC * pieces; i += GT_PW * 32) {
+            const int k = i / pieces, ch = i % pieces * V;
+            if (k < k_fill) {
+                uint4 v[1];
+                gt_read<T, 1>(v, w + (long long)k * ld + ch, k < k_left ? n_left - ch : 0, vec);
+                put(v, gt_place_mn<T>(n, ch, k), GtType<T>::SPLIT ? gt_place_mn<T>(n, n + ch, k) : 0);
+            }
+        }
+    }
+}
+
+template <class T, bool TRANS, int D>
+__device__ __forceinline__ void gt_produce(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, unsigned char* a_base,
+                                           unsigned char* b_base, const GtBars& bars, GtWalk walk, int tid) {
+    constexpr int V = GtType<T>::V, KC = GtType<T>::KC, KSTEP = GtType<T>::KSTEP, TILE_ROWS = 128 / D;
+    const int warp = tid >> 5, lane = tid & 31, c = lane & 7, n = tile_of.n;
+    const bool resident = tile_of.chunks <= tile_of.slots;
+    int it = 0, stage = 0, use = 0, slot = 0, have = -1;        // chunks so far; the group whose weights are in shared memory
+    int turn = 0;                               // warp that has the next four rows: the work goes round
+    for (; walk.more(); walk.next(p.offsets, p.groups)) {
+        walk.tile(TILE_ROWS);
+        const int sets = (walk.rows + 3) >> 2;
+        const T* w_group = static_cast<const T*>(p.W) + (long long)walk.g * gt.gp.w_numel;
+        const bool load_b = !resident || have != walk.g;
+        have = walk.g;
+        if (resident) slot = 0;
+        for (int path_no = to.path_begin; path_no < to.path_end; ++path_no) {
+            const GpPath& path = gt.gp.path[path_no];
+            const bool vec_x = p.x_vec && path.src_off % V == 0 && path.src_mul % V == 0, vec_w = p.w_vec && path.w_off % V == 0 && path.w_ld % V == 0;
+            for (int u0 = 0; u0 < path.src_mul; u0 += KC) {
+                const int left = path.src_mul - u0, k_fill = left >= KC ? KC : (left + KSTEP - 1) / KSTEP * KSTEP;
+                bool ok = true;
+                if (use > 0) ok = warp_wait(ok, bars.empty + stage, (unsigned)(use - 1) & 1, &gt_status, ERR_GT_EMPTY);
+                if (load_b) {
+                    const int last = it - (resident ? tile_of.chunks : tile_of.slots);      // the chunk that used the slot before
+                    if (last >= 0 && last > it - tile_of.stages)
+                        ok = warp_wait(ok, bars.empty + last % tile_of.stages, (unsigned)(last / tile_of.stages) & 1, &gt_status, ERR_GT_EMPTY);
+                }
+                if (!ok) return;
+                unsigned char* a = a_base + stage * GtType<T>::A_BYTES;
+                if (load_b) {
+                    const T* w = w_group + path.w_off + (TRANS ? (long long)n0 * path.w_ld + u0 : (long long)u0 * path.w_ld + n0);
+                    gt_fill_b<T, TRANS>(b_base + slot * GtType<T>::b_bytes(n), w, path.w_ld, n, to.mul - n0, left, k_fill, vec_w, tid);
+                }
+                for (int s = (warp - turn) & (GT_PW - 1); s < sets; s += GT_PW) {
+                    const int r = 4 * s + (lane >> 3);
+                    if (r < walk.rows && V * c < k_fill) {
+                        const T* x = static_cast<const T*>(p.X) + gp_row(p.order, walk.pos + r) * gt.gp.src_dim + path.src_off + (u0 + V * c) * D;
+                        uint4 v[D];
+                        gt_read<T, D>(v, x, left - V * c, vec_x);
+#pragma unroll
+                        for (int k = 0; k < D; ++k) {
+                            const uint4 piece = gt_component<T, D>(v, k);
+                            unsigned char* at = a + tc_swizzle(r * D + k, 4 * c);
+                            if constexpr (GtType<T>::SPLIT) {
+                                float4 hi, lo;
+                                gt_split(*reinterpret_cast<const float4*>(&piece), hi, lo);
+                                *reinterpret_cast<float4*>(at) = hi;
+                                *reinterpret_cast<float4*>(at + 16384) = lo;
+                            } else {
+                                *reinterpret_cast<uint4*>(at) = piece;
+                            }
+                        }
+                    }
+                }
+                turn = (turn + sets) & (GT_PW - 1);
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bars.full + stage);
+                ++it;
+                if (++stage == tile_of.stages) {
+                    stage = 0;
+                    ++use;
+                }
+                if (++slot == tile_of.slots) slot = 0;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------- MMA
+template <class T, bool TRANS>
+__device__ __forceinline__ void gt_multiply(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, unsigned char* a_base,
+                                            unsigned char* b_base, const GtBars& bars, GtWalk walk, int tile_rows, unsigned tmem, unsigned leader) {
+    constexpr int KC = GtType<T>::KC, KSTEP = GtType<T>::KSTEP;
+    constexpr bool B_MN = !TRANS;
+    const int n = tile_of.n, acc = GtType<T>::acc(n), step_b = gt_step_b<T, B_MN>(n) >> 4;
+    const bool resident = tile_of.chunks <= tile_of.slots;
+    const unsigned wide = gt_idesc<T, B_MN>(acc), narrow = gt_idesc<T, B_MN>(n);
+    const unsigned long long a0 = tc_smem_desc(smem_u32(a_base)), b0 = gt_desc_b<T, B_MN>(smem_u32(b_base), n);
+    int stage = 0, use = 0, slot = 0, tiles = 0;
+    for (; walk.more(); walk.next(p.offsets, p.groups), ++tiles) {
+        walk.tile(tile_rows);
+        const int buf = tiles & 1;
+        bool ok = true;
+        if (tiles >= 2) ok = warp_wait(ok, bars.acc_empty + buf, (unsigned)(tiles / 2 - 1) & 1, &gt_status, ERR_GT_ACC_EMPTY);
+        const unsigned d = tmem + (unsigned)(buf * 256);
+        unsigned accumulate = 0;
+        if (resident) slot = 0;
+        for (int path_no = to.path_begin; path_no < to.path_end && ok; ++path_no) {
+            const int mul = gt.gp.path[path_no].src_mul;
+            for (int u0 = 0; u0 < mul && ok; u0 += KC) {
+                ok = warp_wait(ok, bars.full + stage, (unsigned)use & 1, &gt_status, ERR_GT_FULL);
+                if (!ok) break;
+                tc_fence_after();
+                const int steps = (min(KC, mul - u0) + KSTEP - 1) / KSTEP;
+                unsigned long long a = a0 + (unsigned long long)(stage * (GtType<T>::A_BYTES >> 4));
+                unsigned long long b = b0 + (unsigned long long)(slot * (GtType<T>::b_bytes(n) >> 4));
+                for (int s = 0; s < steps; ++s, a += 2, b += step_b) {
+                    gt_mma<T>(leader, d, a, b, wide, accumulate);
+                    if constexpr (GtType<T>::SPLIT) gt_mma<T>(leader, d + (unsigned)n, a + (16384 >> 4), b, narrow, 1);
+                    accumulate = 1;
+                }
+                tc_commit_if(leader, bars.empty + stage);
+                if (++stage == tile_of.stages) {
+                    stage = 0;
+                    ++use;
+                }
+                if (++slot == tile_of.slots) slot = 0;
+            }
+        }
+        if (!ok) return;
+        tc_commit_if(leader, bars.acc_full + buf);
+    }
+}
+
+// ---------------------------------------------------------------------------- epilogue
+template <class T> struct GtPair;
+template <> struct GtPair<__nv_bfloat16> {
+    static __device__ unsigned of(float a, float b) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const unsigned*>(&v);
+    }
+};
+template <> struct GtPair<__half> {
+    static __device__ unsigned of(float a, float b) {
+        const __half2 v = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const unsigned*>(&v);
+    }
+};
+
+template <class T>
+__device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, float* staging,
+                                         const GtBars& bars, GtWalk walk, int tile_rows, unsigned tmem, int warp, int lane) {
+    const int d = to.d, n = tile_of.n, mul = min(n, to.mul - n0), pitch = 33 * d, pair = warp * 32 + lane, r_of = pair / d, k_of = pair % d;
+    const float scale = (float)to.scale;
+    const unsigned quarter = tmem + ((unsigned)(warp * 32) << 16);
+    int tiles = 0;
+    for (; walk.more(); walk.next(p.offsets, p.groups), ++tiles) {
+        walk.tile(tile_rows);
+        const int buf = tiles & 1;
+        if (pair < walk.rows) bars.rows[pair] = (int)gp_row(p.order, walk.pos + pair);       // (read behind the first barrier below)
+        if (!warp_wait(true, bars.acc_full + buf, (unsigned)(tiles / 2) & 1, &gt_status, ERR_GT_ACC_FULL)) return;
+        tc_fence_after();
+        for (int w0 = 0; w0 < mul; w0 += 32) {
+            unsigned v[32], u[GtType<T>::SPLIT ? 32 : 1];
+            const unsigned at = quarter + (unsigned)(buf * 256 + w0);
+            tc_load16(at, v);
+            if (w0 + 16 < n) tc_load16(at + 16, v + 16);
+            if constexpr (GtType<T>::SPLIT) {
+                tc_load16(at + n, u);
+                if (w0 + 16 < n) tc_load16(at + n + 16, u + 16);
+            }
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if (w0 + 32 >= mul) {               // the accumulator has been read
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bars.acc_empty + buf);
+            }
+            if (r_of < walk.rows) {
+                float* to_smem = staging + r_of * pitch + k_of;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    float s = __uint_as_float(v[j]);
+                    if constexpr (GtType<T>::SPLIT) s += __uint_as_float(u[j]);
+                    to_smem[j * d] = s * scale;
+                }
+            }
+            group_sync(1, GT_EPI * 32);
+            const int values = min(32, mul - w0) * d;
+            T* z_col = static_cast<T*>(p.Z) + to.off + (n0 + w0) * d;
+            for (int r = warp; r < walk.rows; r += GT_EPI) {
+                T* z = z_col + (long long)bars.rows[r] * gt.gp.dst_dim;
+                const float* from = staging + r * pitch;
+                if constexpr (sizeof(T) == 4) {
+                    for (int i = lane; i < values; i += 32) z[i] = from[i];
+                } else {
+                    if (p.z_pair && ((to.off | values) & 1) == 0) {
+                        for (int i = 2 * lane; i < values; i += 64) *reinterpret_cast<unsigned*>(z + i) = GtPair<T>::of(from[i], from[i + 1]);
+                    } else {
+                        for (int i = lane; i < values; i += 32) gp_store(z + i, from[i]);
+                    }
+                }
+            }
+            group_sync(1, GT_EPI * 32);
+        }
+    }
+}
+
+template <class T, bool TRANS>
+__global__ void __launch_bounds__(GT_THREADS, 1) oeq_grouped_tc(const __grid_constant__ GtProblem gt, const GtArgs p) {
+    extern __shared__ __align__(16) unsigned char gt_smem[];
+    unsigned char* smem = gt_smem + ((1024u - (smem_u32(gt_smem) & 1023u)) & 1023u);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    int t = 0;
+    while (t + 1 < gt.gp.n_targets && (int)blockIdx.x >= gt.target[t + 1].first) ++t;
+    const GpTarget& to = gt.gp.target[t];
+    const GtTarget& tile_of = gt.target[t];
+    const int local = (int)blockIdx.x - tile_of.first, part = local / tile_of.n_tiles, n0 = local % tile_of.n_tiles * tile_of.n, d = to.d;
+    unsigned char *a_base = smem + GT_CONTROL, *b_base = a_base + tile_of.stages * GtType<T>::A_BYTES;
+    float* staging = reinterpret_cast<float*>(b_base + tile_of.slots * GtType<T>::b_bytes(tile_of.n));
+    const GtBars bars(smem);
+    if (tid == 0) {
+        for (int i = 0; i < GT_STAGES; ++i) {
+            mbar_init(bars.full + i, GT_PW);
+            mbar_init(bars.empty + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bars.acc_full + i, 1);
+            mbar_init(bars.acc_empty + i, GT_EPI);
+        }
+        fence_mbar_init();
+    }
+    constexpr int MMA_WARP = GT_PW + GT_EPI;
+    if (warp == MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(bars.tmem)), "n"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile unsigned*>(bars.tmem), 0);
+    const long long n = min(__ldg(p.offsets + p.groups), p.rows);
+    const bool work = to.path_begin < to.path_end;              // (a block without a path is zero in every row)
+    const GtWalk walk(p.offsets, p.groups, work ? gp_cut(n, part, tile_of.parts) : 0, work ? gp_cut(n, part + 1, tile_of.parts) : 0);
+    const int tile_rows = 128 / d;
+    if (warp < GT_PW) {
+        switch (d) {
+            case 1: gt_produce<T, TRANS, 1>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid); break;
+            case 3: gt_produce<T, TRANS, 3>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid); break;
+            case 5: gt_produce<T, TRANS, 5>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid); break;
+            case 7: gt_produce<T, TRANS, 7>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid); break;
+            default: gt_produce<T, TRANS, 9>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid); break;
+        }
+    } else if (warp < MMA_WARP) {
+        gt_drain<T>(gt, p, tile_of, to, n0, staging, bars, walk, tile_rows, tmem, warp - GT_PW, lane);
+    } else {
+        gt_multiply<T, TRANS>(gt, p, tile_of, to, a_base, b_base, bars, walk, tile_rows, tmem, elect_lane());
+    }
+    // zeros: the rows without a group, every row where the block has no path
+    {
+        const long long from = work ? n : 0, count = p.rows - from;
+        const long long lo = from + gp_cut(count, part, tile_of.parts), hi = from + gp_cut(count, part + 1, tile_of.parts);
+        const int values = min(tile_of.n, to.mul - n0) * d;
+        for (long long at = lo + warp; at < hi; at += GT_THREADS / 32) {
+            T* z = static_cast<T*>(p.Z) + gp_row(p.order, at) * gt.gp.dst_dim + to.off + n0 * d;
+            for (int i = lane; i < values; i += 32) gp_store(z + i, 0.f);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+}
+
+}  // namespace oeq

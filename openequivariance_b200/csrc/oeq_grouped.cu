@@ -6,12 +6,14 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdint>
 #include <string>
 #include <vector>
 
 #include "../../include/oeq_b200.h"
 #include "oeq_internal.h"
 #include "grouped_kernels.cuh"
+#include "grouped_tc_kernels.cuh"
 #include "row_groups_kernels.cuh"
 
 using namespace oeq;
@@ -138,22 +140,102 @@ int simt_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* 
     return join<T>(gp, split, GP_TILE, GP_TILE, rows, groups, offsets, dW, ws, st);
 }
 
+// ---- tensor cores
+// The CTAs, one for each SM, are dealt to the tiles of channels by the time that a range of rows takes: for every (row, component) pair
+// the channels read and written and a fixed part.
+template <class T>
+int tc_plan(const GpProblem& gp, int64_t rows, int sms, GtProblem& gt, int& ctas, size_t& smem) {
+    gt.gp = gp;
+    double cost[GP_BLOCKS] = {};
+    ctas = 0;
+    for (int t = 0; t < gp.n_targets; ++t) {
+        const GpTarget& to = gp.target[t];
+        GtTarget& x = gt.target[t];
+        x = {};
+        if (to.mul == 0) continue;
+        x.n_tiles = (to.mul + GtType<T>::N_MAX - 1) / GtType<T>::N_MAX;
+        x.n = ((to.mul + x.n_tiles - 1) / x.n_tiles + 15) / 16 * 16;
+        x.n_tiles = (to.mul + x.n - 1) / x.n;
+        x.parts = 1;
+        int k = 0;
+        for (int p = to.path_begin; p < to.path_end; ++p) {
+            k += gp.path[p].src_mul;
+            x.chunks += (gp.path[p].src_mul + GtType<T>::KC - 1) / GtType<T>::KC;
+        }
+        cost[t] = to.d * (double)(k + x.n + 32);
+        ctas += x.n_tiles;
+    }
+    for (;;) {                          // the tile whose ranges take longest gets another CTA
+        int most = -1;
+        for (int t = 0; t < gp.n_targets; ++t)
+            if (gt.target[t].parts && gt.target[t].parts < rows && (most < 0 || cost[t] / gt.target[t].parts > cost[most] / gt.target[most].parts)) most = t;
+        if (most < 0 || ctas + gt.target[most].n_tiles > sms) break;
+        ++gt.target[most].parts;
+        ctas += gt.target[most].n_tiles;
+    }
+    const size_t room = SMEM_MOST - GT_CONTROL - 1024 - GT_STAGING;
+    smem = 0;
+    ctas = 0;
+    for (int t = 0; t < gp.n_targets; ++t) {
+        GtTarget& x = gt.target[t];
+        x.first = ctas;
+        ctas += x.n_tiles * x.parts;
+        if (!x.parts) continue;
+        const size_t a = GtType<T>::A_BYTES, b = GtType<T>::b_bytes(x.n);
+        if (2 * a + x.chunks * b <= room) {     // a group's weights stay in shared memory
+            x.slots = std::max(1, x.chunks);
+            x.stages = (int)std::min<size_t>(GT_STAGES, (room - x.slots * b) / a);
+        } else {
+            x.slots = x.stages = (int)std::min<size_t>(GT_STAGES, room / (a + b));
+        }
+        smem = std::max(smem, x.stages * a + x.slots * b);
+    }
+    smem = std::max<size_t>(smem + GT_CONTROL + 1024 + GT_STAGING, 120 * 1024);         // (one CTA an SM: it takes all of the tensor memory)
+    return OEQ_OK;
+}
+
+bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+template <class T, bool TRANS>
+int tc_product(const GpProblem& gp, int64_t rows, int64_t groups, const void* X, const void* W, const int64_t* order, const int64_t* offsets, void* Z,
+               cudaStream_t st) {
+    int sms = 0, ctas = 0;
+    size_t smem = 0;
+    if (int rc = sm_count(sms)) return rc;
+    GtProblem gt{};
+    if (int rc = tc_plan<T>(gp, rows, sms, gt, ctas, smem)) return rc;
+    if (ctas == 0) return OEQ_OK;
+    const GtArgs args{X, W, (const long long*)order, (const long long*)offsets, Z, rows, (int)groups,
+                      aligned(X, 16) && gp.src_dim * sizeof(T) % 16 == 0, aligned(W, 16) && gp.w_numel * sizeof(T) % 16 == 0,
+                      aligned(Z, 4) && gp.dst_dim % 2 == 0};
+    if (int rc = allow_smem(oeq_grouped_tc<T, TRANS>, smem)) return rc;
+    oeq_grouped_tc<T, TRANS><<<ctas, GT_THREADS, smem, st>>>(gt, args);
+    OEQ_CUDA(cudaGetLastError());
+    return OEQ_OK;
+}
+
 int check_call(const oeq_grouped* h, int dtype, int64_t rows, int64_t groups) {
     if (!h) return oeq_fail(OEQ_ERR_INVALID, "null handle");
     if (!known_dtype(dtype)) return oeq_fail(OEQ_ERR_INVALID, "unknown dtype");
     return check_groups(rows, groups);
 }
 
-int product(const GpProblem& gp, int dtype, int64_t rows, int64_t groups, const void* X, const void* W, const int64_t* order, const int64_t* offsets,
+template <bool TRANS>
+int product(const oeq_grouped* h, int dtype, int64_t rows, int64_t groups, const void* X, const void* W, const int64_t* order, const int64_t* offsets,
             const int32_t* blocks, void* Z, void* stream) {
+    const GpProblem& gp = TRANS ? h->backward : h->forward;
     if (rows == 0 || gp.dst_dim == 0) return OEQ_OK;
     if (!offsets || !blocks || !Z || (gp.src_dim && !X) || (gp.w_numel && !W)) return oeq_fail(OEQ_ERR_INVALID, "null pointer");
     const cudaStream_t st = (cudaStream_t)stream;
+    const bool tc = h->d_max <= GT_D_MAX;
     switch (dtype) {
         case OEQ_F64: return simt_product<double>(gp, rows, groups, X, W, order, offsets, blocks, Z, st);
-        case OEQ_F32: return simt_product<float>(gp, rows, groups, X, W, order, offsets, blocks, Z, st);
-        case OEQ_BF16: return simt_product<__nv_bfloat16>(gp, rows, groups, X, W, order, offsets, blocks, Z, st);
-        default: return simt_product<__half>(gp, rows, groups, X, W, order, offsets, blocks, Z, st);
+        case OEQ_F32: return tc ? tc_product<float, TRANS>(gp, rows, groups, X, W, order, offsets, Z, st)
+                                : simt_product<float>(gp, rows, groups, X, W, order, offsets, blocks, Z, st);
+        case OEQ_BF16: return tc ? tc_product<__nv_bfloat16, TRANS>(gp, rows, groups, X, W, order, offsets, Z, st)
+                                 : simt_product<__nv_bfloat16>(gp, rows, groups, X, W, order, offsets, blocks, Z, st);
+        default: return tc ? tc_product<__half, TRANS>(gp, rows, groups, X, W, order, offsets, Z, st)
+                           : simt_product<__half>(gp, rows, groups, X, W, order, offsets, blocks, Z, st);
     }
 }
 
@@ -284,13 +366,13 @@ int64_t oeq_grouped_weight_numel(const oeq_grouped* h) { return h ? h->forward.w
 int oeq_grouped_forward(oeq_grouped* h, int dtype, int64_t rows, int64_t groups, const void* X, const void* W, const int64_t* order, const int64_t* offsets,
                         const int32_t* blocks, void* Z, void* stream) {
     if (int rc = check_call(h, dtype, rows, groups)) return rc;
-    return product(h->forward, dtype, rows, groups, X, W, order, offsets, blocks, Z, stream);
+    return product<false>(h, dtype, rows, groups, X, W, order, offsets, blocks, Z, stream);
 }
 
 int oeq_grouped_backward_input(oeq_grouped* h, int dtype, int64_t rows, int64_t groups, const void* dZ, const void* W, const int64_t* order,
                                const int64_t* offsets, const int32_t* blocks, void* dX, void* stream) {
     if (int rc = check_call(h, dtype, rows, groups)) return rc;
-    return product(h->backward, dtype, rows, groups, dZ, W, order, offsets, blocks, dX, stream);
+    return product<true>(h, dtype, rows, groups, dZ, W, order, offsets, blocks, dX, stream);
 }
 
 size_t oeq_grouped_workspace_bytes(const oeq_grouped* h, int dtype, int64_t rows, int64_t groups) {
@@ -315,6 +397,13 @@ int oeq_grouped_backward_weights(oeq_grouped* h, int dtype, int64_t rows, int64_
         case OEQ_BF16: return simt_weights<__nv_bfloat16>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st);
         default: return simt_weights<__half>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st);
     }
+}
+
+int oeq_grouped_check(void) {
+    int code = 0;
+    OEQ_CUDA(cudaMemcpyFromSymbol(&code, gt_status, sizeof code));
+    if (code) return oeq_fail(OEQ_ERR_DEVICE_WAIT, "a kernel gave up on a bounded wait (code " + std::to_string(code) + ")");
+    return OEQ_OK;
 }
 
 }  // extern "C"

@@ -147,3 +147,8 @@ class GroupedLinear:
         return _grouped_linear(x, weights, groups.order, groups.offsets, groups.blocks, self._number, 0)
 
     __call__ = forward
+
+    @staticmethod
+    def check_device_status():
+        """Raises if a kernel on the current device has abandoned a bounded wait (waits for the device)."""
+        _native.check(_native.lib().oeq_grouped_check())

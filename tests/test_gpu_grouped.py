@@ -14,6 +14,12 @@ pytestmark = pytest.mark.gpu
 F32, F64, BF16, F16 = torch.float32, torch.float64, torch.bfloat16, torch.float16
 
 
+@pytest.fixture(autouse=True)
+def no_wait_was_abandoned():
+    yield
+    oeq.GroupedLinear.check_device_status()
+
+
 def host(t):
     return t.detach().cpu().numpy()
 
