@@ -6,13 +6,15 @@
 // As a matrix product: M = (row, component) pairs of sorted rows of one group, N = channels of one output block, K = channels of
 // the input blocks with its irrep.  A CTA has one output block (or a tile of its channels) and one range of the sorted rows, the
 // CTAs being dealt to the output blocks by cost, so a CTA meets few groups and keeps a group's weights in shared memory.
-//   * 16 producer warps: a lane reads the 16 d bytes of V = 4 (16-bit types: 8) channels of a row, [channel][component], and writes
+//   * 8 producer warps: a lane reads the 16 d bytes of V = 4 (16-bit types: 8) channels of a row, [channel][component], and writes
 //     d pieces of 16 bytes, one per (row, component), K-major with the 128-byte swizzle.  The transposition that the layout of irreps
 //     asks for costs no extra pass, rows are gathered in sorted order, and FP32 values are split into TF32 hi and lo on the way.
+//     Two sets of four warps take the chunks of K in turn: each has its chunk on the way in registers before it waits for a stage.
 //     Weights have their output channels along memory: "MN-major" tiles for Z, K-major for dX; neither is transposed.
 //   * one warp, in step, issues the MMAs.  FP32: hi.hi and hi.lo as one MMA over the weights' hi channels followed by lo, lo.hi
 //     into hi.lo's columns: the large and the small products have accumulators of their own.
-//   * 4 epilogue warps add those, scale, and write rows through shared memory, so that a row's values leave in order.
+//   * 8 epilogue warps, in two groups, add those, scale, and write rows through shared memory, so that a row's values leave in order.  They
+//     also prefetch the rows and weights of the tile after next to L2: the producers' loads then take a third of the time.
 // Two accumulators: a tile drains while the next is computed.  Every wait is bounded; on expiry a role records a code and all
 // leave.
 #pragma once
@@ -22,10 +24,10 @@
 namespace oeq {
 
 constexpr int GT_D_MAX = 9;
-constexpr int GT_PW = 16, GT_EPI = 4, GT_THREADS = (GT_PW + GT_EPI + 1) * 32;
+constexpr int GT_SETS = 2, GT_SET = 4, GT_PW = GT_SETS * GT_SET, GT_EPI_GROUPS = 2, GT_EPI = 4 * GT_EPI_GROUPS, GT_THREADS = (GT_PW + GT_EPI + 1) * 32;
 constexpr int GT_STAGES = 6;                    // most stages of A
-constexpr int GT_STAGING = 33 * 128 * 4;        // 32 channels of a tile's pairs
-constexpr int GT_CONTROL = 1024;                // barriers, the tile's rows
+constexpr int GT_STAGING = 33 * 128 * 4;        // 32 channels of a tile's pairs, for each epilogue group
+constexpr int GT_CONTROL = 1536;                // barriers, rows of the tiles that drain, the CTA's range
 constexpr int ERR_GT_EMPTY = 81, ERR_GT_FULL = 82, ERR_GT_ACC_FULL = 83, ERR_GT_ACC_EMPTY = 84;
 
 // Set by a kernel whose bounded wait ran out; read by oeq_grouped_check.
@@ -35,12 +37,16 @@ struct GtTarget {
     int n_tiles, n;             // tiles of its channels, channels of a tile (a multiple of 16)
     int parts, first;           // ranges of rows, first CTA
     int stages, slots;          // of A, of B
-    int chunks;                 // steps of the sum
+    int chunks;                 // of the sum
+    int extra;                  // time of a group's weights, in rows
 };
 struct GtProblem {
     GpProblem gp;
     GtTarget target[GP_BLOCKS];
 };
+
+// Rows of a tile.  Seven components: 16 rows (112 of 128 pairs) are one piece for every lane of a set, 18 would be two.
+__host__ __device__ constexpr int gt_tile_rows(int d) { return d == 7 ? 16 : 128 / d; }
 
 template <class T> struct GtType {              // 16-bit
     static constexpr int V = 8, KC = 64, KSTEP = 16, A_BYTES = 16384, N_MAX = 256;
@@ -98,26 +104,27 @@ __device__ __forceinline__ void gt_split(const float4& v, float4& hi, float4& lo
     hi = make_float4(tf32_hi(v.x), tf32_hi(v.y), tf32_hi(v.z), tf32_hi(v.w));
     lo = make_float4(v.x - hi.x, v.y - hi.y, v.z - hi.z, v.w - hi.w);         // exact; read as TF32 by the MMA
 }
-// V channels of D components, as 16-byte words: `left` of the channels exist, the others are zero.
-template <class T, int D>
-__device__ __forceinline__ void gt_read(uint4 (&v)[D], const T* __restrict__ src, int left, bool vec) {
-    constexpr int V = GtType<T>::V;
-    if (vec && left >= V) {
+// V channels of D components, as 16-byte words: `left` of the channels exist, the others are zero.  FAST: sixteen bytes at a time, for
+// blocks of whole pieces; no branch, so that the loads of several pieces are on the way together.
+template <class T, int D, bool FAST>
+__device__ __forceinline__ void gt_read(uint4 (&v)[D], const T* __restrict__ src, int left) {
+    if constexpr (FAST) {
 #pragma unroll
-        for (int i = 0; i < D; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
-        return;
-    }
-    unsigned* w = reinterpret_cast<unsigned*>(v);
-    if constexpr (sizeof(T) == 4) {
+        for (int i = 0; i < D; ++i) v[i] = left > 0 ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+    } else if constexpr (sizeof(T) == 4) {
+        unsigned* w = reinterpret_cast<unsigned*>(v);
 #pragma unroll
         for (int i = 0; i < 4 * D; ++i) w[i] = i / D < left ? __float_as_uint(__ldg(reinterpret_cast<const float*>(src) + i)) : 0u;
     } else {
+        unsigned* w = reinterpret_cast<unsigned*>(v);
         const unsigned short* h = reinterpret_cast<const unsigned short*>(src);
 #pragma unroll
         for (int i = 0; i < 4 * D; ++i)
             w[i] = (2 * i / D < left ? (unsigned)__ldg(h + 2 * i) : 0u) | ((2 * i + 1) / D < left ? (unsigned)__ldg(h + 2 * i + 1) << 16 : 0u);
     }
 }
+// Byte offset of 16-byte piece c of row `row` of a K-major tile (128-byte rows, 128-byte swizzle).
+__device__ __forceinline__ int gt_place_k(int row, int c) { return row * 128 + (((row ^ c) & 7) << 4); }
 // The V channels of component k.
 template <class T, int D>
 __device__ __forceinline__ uint4 gt_component(const uint4 (&v)[D], int k) {
@@ -139,11 +146,8 @@ __device__ __forceinline__ uint4 gt_component(const uint4 (&v)[D], int k) {
 struct GtWalk {
     long long pos, hi, end;     // next position, end of the range, end of the group within it
     int g, rows;
-    __device__ GtWalk(const long long* offsets, int groups, long long lo, long long hi_) : pos(lo), hi(hi_), end(0), g(0), rows(0) {
-        if (lo < hi) {
-            g = gp_group(offsets, groups, lo);
-            end = min(__ldg(offsets + g + 1), hi);
-        }
+    __device__ GtWalk(const long long* offsets, int g_, long long lo, long long hi_) : pos(lo), hi(hi_), end(0), g(g_), rows(0) {
+        if (lo < hi) end = min(__ldg(offsets + g + 1), hi);
     }
     __device__ bool more() const { return pos < hi; }
     __device__ void tile(int most) { rows = (int)min((long long)most, end - pos); }
@@ -161,6 +165,58 @@ struct GtWalk {
     }
 };
 
+// The CTA's range of sorted rows, by all threads: part `part` of `parts` equal lengths on an axis where every row has length 1
+// and every group with rows `extra` more, in front of it: the time that its weights take.
+struct GtRange {
+    long long lo, hi;
+    int g;                      // the group that row lo is in
+    int sums[33];
+};
+__device__ __forceinline__ void gt_range(GtRange& out, const long long* __restrict__ offsets, int groups, long long rows, int part, int parts, int extra) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    const int each = (groups + blockDim.x - 1) / blockDim.x, g0 = min(tid * each, groups), g1 = min(g0 + each, groups);
+    const long long n = min(__ldg(offsets + groups), rows);
+    int used = 0;
+    long long at = g0 < g1 ? min(__ldg(offsets + g0), n) : n;
+    const long long first = at;
+    for (int g = g0; g < g1; ++g) {
+        const long long end = min(__ldg(offsets + g + 1), n);
+        used += end > at;
+        at = end;
+    }
+    int s = used;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, s, off);
+        if (lane >= off) s += t;
+    }
+    if (lane == 31) out.sums[warp] = s;
+    if (tid == 0) out.lo = out.hi = n, out.g = 0;
+    __syncthreads();
+    int before = s - used, all = 0;
+    for (int w = 0; w < warps; ++w) {
+        before += w < warp ? out.sums[w] : 0;
+        all += out.sums[w];
+    }
+    const long long length = n + (long long)all * extra, lo = gp_cut(length, part, parts), hi = gp_cut(length, part + 1, parts);
+    at = first;
+    for (int g = g0; g < g1; ++g) {
+        const long long end = min(__ldg(offsets + g + 1), n);
+        if (end > at) {
+            const long long v = at + (long long)before * extra, w = v + extra + (end - at);         // the group's piece of the axis
+            if (lo >= v && lo < w) {
+                const long long p = at + max(lo - v - extra, 0ll);
+                out.lo = p;
+                out.g = g;
+            }
+            if (hi >= v && hi < w) out.hi = at + max(hi - v - extra, 0ll);
+            ++before;
+        }
+        at = end;
+    }
+    __syncthreads();
+}
+
 struct GtArgs {
     const void *X, *W;
     const long long *order, *offsets;
@@ -172,51 +228,45 @@ struct GtArgs {
 struct GtBars {
     unsigned long long *full, *empty, *acc_full, *acc_empty;
     unsigned* tmem;
-    int* rows;                  // of the tile that drains
+    int* rows;                  // of the tile that drains, for each epilogue group
     __device__ explicit GtBars(unsigned char* control) {
         full = reinterpret_cast<unsigned long long*>(control);
         empty = full + GT_STAGES;
         acc_full = empty + GT_STAGES;
         acc_empty = acc_full + 2;
         tmem = reinterpret_cast<unsigned*>(acc_empty + 2);
-        rows = reinterpret_cast<int*>(control + 256);
+        rows = reinterpret_cast<int*>(control + 512);      // (behind the range)
     }
 };
 
 // ---------------------------------------------------------------------------- producers
-template <class T, bool TRANS>
-__device__ __forceinline__ void gt_fill_b(unsigned char* dst, const T* __restrict__ w, int ld, int n, int n_left, int k_left, int k_fill, bool vec, int tid) {
-    constexpr int V = GtType<T>::V, KC = GtType<T>::KC;
-    auto put = [&](const uint4 (&v)[1], int at, int at_lo) {
-        if constexpr (GtType<T>::SPLIT) {
-            float4 hi, lo;
-            gt_split(*reinterpret_cast<const float4*>(v), hi, lo);
-            *reinterpret_cast<float4*>(dst + at) = hi;
-            *reinterpret_cast<float4*>(dst + at_lo) = lo;
-        } else {
-            *reinterpret_cast<uint4*>(dst + at) = v[0];
+// A chunk of weights by the threads of a set, four pieces of 16 bytes of a lane on the way at once.
+template <class T, bool TRANS, bool FAST>
+__device__ __forceinline__ void gt_fill_b(unsigned char* dst, const T* __restrict__ w, int ld, int n, int n_left, int k_left, int k_fill, int member) {
+    constexpr int V = GtType<T>::V, AT_ONCE = 4;
+    const int across = TRANS ? 8 : n / V, pieces = TRANS ? n * 8 : k_fill * across;     // K-major: (channel, piece of K); MN-major: (k, piece of channels)
+    const unsigned magic = (65536 + across - 1) / across;       // i / across for i < 2048, across <= 32
+#pragma unroll 1
+    for (int i0 = member; i0 < pieces; i0 += AT_ONCE * GT_SET * 32) {
+        uint4 v[AT_ONCE][1];
+        int row[AT_ONCE], c[AT_ONCE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int i = min(i0 + j * GT_SET * 32, pieces - 1);        // (the last piece again: the same value to the same place)
+            row[j] = TRANS ? i >> 3 : (int)((i * magic) >> 16);
+            c[j] = TRANS ? i & 7 : i - row[j] * across;
+            gt_read<T, 1, FAST>(v[j], w + (long long)row[j] * ld + c[j] * V, TRANS ? (row[j] < n_left ? k_left - c[j] * V : 0) : (row[j] < k_left ? n_left - c[j] * V : 0));
         }
-    };
-    if constexpr (TRANS) {      // channel ch of the input: W[ch][k], K-major
-#pragma unroll 2
-        for (int i = tid; i < n * 8; i += GT_PW * 32) {
-            const int ch = i >> 3, c = i & 7;
-            if (V * c < k_fill) {
-                uint4 v[1];
-                gt_read<T, 1>(v, w + (long long)ch * ld + V * c, ch < n_left ? k_left - V * c : 0, vec);
-                const int at = tc_swizzle(ch, 4 * c);
-                put(v, at, at + n * 128);
-            }
-        }
-    } else {                    // W[k][ch], MN-major
-        const int pieces = n / V;
-#pragma unroll 2
-        for (int i = tid; i < KC * pieces; i += GT_PW * 32) {
-            const int k = i / pieces, ch = i % pieces * V;
-            if (k < k_fill) {
-                uint4 v[1];
-                gt_read<T, 1>(v, w + (long long)k * ld + ch, k < k_left ? n_left - ch : 0, vec);
-                put(v, gt_place_mn<T>(n, ch, k), GtType<T>::SPLIT ? gt_place_mn<T>(n, n + ch, k) : 0);
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int at = TRANS ? gt_place_k(row[j], c[j]) : gt_place_mn<T>(n, c[j] * V, row[j]);
+            if constexpr (GtType<T>::SPLIT) {
+                float4 hi, lo;
+                gt_split(*reinterpret_cast<const float4*>(v[j]), hi, lo);
+                *reinterpret_cast<float4*>(dst + at) = hi;
+                *reinterpret_cast<float4*>(dst + (TRANS ? at + n * 128 : gt_place_mn<T>(n, n + c[j] * V, row[j]))) = lo;
+            } else {
+                *reinterpret_cast<uint4*>(dst + at) = v[j][0];
             }
         }
     }
@@ -225,61 +275,78 @@ __device__ __forceinline__ void gt_fill_b(unsigned char* dst, const T* __restric
 template <class T, bool TRANS, int D>
 __device__ __forceinline__ void gt_produce(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, unsigned char* a_base,
                                            unsigned char* b_base, const GtBars& bars, GtWalk walk, int tid) {
-    constexpr int V = GtType<T>::V, KC = GtType<T>::KC, KSTEP = GtType<T>::KSTEP, TILE_ROWS = 128 / D;
-    const int warp = tid >> 5, lane = tid & 31, c = lane & 7, n = tile_of.n;
+    constexpr int V = GtType<T>::V, KC = GtType<T>::KC, KSTEP = GtType<T>::KSTEP, TILE_ROWS = gt_tile_rows(D), THREADS = GT_SET * 32;
+    constexpr int PIECES = (TILE_ROWS * 8 + THREADS - 1) / THREADS;             // of V channels by D components, of a lane
+    const int set = tid / THREADS, member = tid % THREADS, lane = tid & 31, c = lane & 7, n = tile_of.n;
     const bool resident = tile_of.chunks <= tile_of.slots;
     int it = 0, stage = 0, use = 0, slot = 0, have = -1;        // chunks so far; the group whose weights are in shared memory
-    int turn = 0;                               // warp that has the next four rows: the work goes round
+    int turn = 0;                               // set that has the next chunk
     for (; walk.more(); walk.next(p.offsets, p.groups)) {
         walk.tile(TILE_ROWS);
-        const int sets = (walk.rows + 3) >> 2;
         const T* w_group = static_cast<const T*>(p.W) + (long long)walk.g * gt.gp.w_numel;
         const bool load_b = !resident || have != walk.g;
         have = walk.g;
         if (resident) slot = 0;
+        int row[PIECES];                        // (past the tile's rows: the last one again)
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const long long at = walk.pos + min((member + i * THREADS) >> 3, walk.rows - 1);
+            row[i] = p.order ? (int)__ldg(p.order + at) : (int)at;
+        }
         for (int path_no = to.path_begin; path_no < to.path_end; ++path_no) {
             const GpPath& path = gt.gp.path[path_no];
             const bool vec_x = p.x_vec && path.src_off % V == 0 && path.src_mul % V == 0, vec_w = p.w_vec && path.w_off % V == 0 && path.w_ld % V == 0;
             for (int u0 = 0; u0 < path.src_mul; u0 += KC) {
-                const int left = path.src_mul - u0, k_fill = left >= KC ? KC : (left + KSTEP - 1) / KSTEP * KSTEP;
-                bool ok = true;
-                if (use > 0) ok = warp_wait(ok, bars.empty + stage, (unsigned)(use - 1) & 1, &gt_status, ERR_GT_EMPTY);
-                if (load_b) {
-                    const int last = it - (resident ? tile_of.chunks : tile_of.slots);      // the chunk that used the slot before
-                    if (last >= 0 && last > it - tile_of.stages)
-                        ok = warp_wait(ok, bars.empty + last % tile_of.stages, (unsigned)(last / tile_of.stages) & 1, &gt_status, ERR_GT_EMPTY);
-                }
-                if (!ok) return;
-                unsigned char* a = a_base + stage * GtType<T>::A_BYTES;
-                if (load_b) {
-                    const T* w = w_group + path.w_off + (TRANS ? (long long)n0 * path.w_ld + u0 : (long long)u0 * path.w_ld + n0);
-                    gt_fill_b<T, TRANS>(b_base + slot * GtType<T>::b_bytes(n), w, path.w_ld, n, to.mul - n0, left, k_fill, vec_w, tid);
-                }
-                for (int s = (warp - turn) & (GT_PW - 1); s < sets; s += GT_PW) {
-                    const int r = 4 * s + (lane >> 3);
-                    if (r < walk.rows && V * c < k_fill) {
-                        const T* x = static_cast<const T*>(p.X) + gp_row(p.order, walk.pos + r) * gt.gp.src_dim + path.src_off + (u0 + V * c) * D;
-                        uint4 v[D];
-                        gt_read<T, D>(v, x, left - V * c, vec_x);
+                if (turn == set) {
+                    const int left = path.src_mul - u0, k_fill = left >= KC ? KC : (left + KSTEP - 1) / KSTEP * KSTEP;
+                    uint4 v[PIECES][D];
+const T* x = static_cast<const T*>(p.X) + path.src_off + (u0 + V * c) * D;
+                    if (vec_x) {
 #pragma unroll
-                        for (int k = 0; k < D; ++k) {
-                            const uint4 piece = gt_component<T, D>(v, k);
-                            unsigned char* at = a + tc_swizzle(r * D + k, 4 * c);
-                            if constexpr (GtType<T>::SPLIT) {
-                                float4 hi, lo;
-                                gt_split(*reinterpret_cast<const float4*>(&piece), hi, lo);
-                                *reinterpret_cast<float4*>(at) = hi;
-                                *reinterpret_cast<float4*>(at + 16384) = lo;
-                            } else {
-                                *reinterpret_cast<uint4*>(at) = piece;
+                        for (int i = 0; i < PIECES; ++i) gt_read<T, D, true>(v[i], x + (long long)row[i] * gt.gp.src_dim, left - V * c);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < PIECES; ++i) gt_read<T, D, false>(v[i], x + (long long)row[i] * gt.gp.src_dim, left - V * c);
+                    }
+                    bool ok = true;
+                    if (use > 0) ok = warp_wait(ok, bars.empty + stage, (unsigned)(use - 1) & 1, &gt_status, ERR_GT_EMPTY);
+                    if (load_b) {
+                        const int last = it - (resident ? tile_of.chunks : tile_of.slots);      // the chunk that used the slot before
+                        if (last >= 0 && last > it - tile_of.stages)
+                            ok = warp_wait(ok, bars.empty + last % tile_of.stages, (unsigned)(last / tile_of.stages) & 1, &gt_status, ERR_GT_EMPTY);
+                    }
+                    if (!ok) return;
+                    unsigned char* a = a_base + stage * GtType<T>::A_BYTES;
+#pragma unroll
+                    for (int i = 0; i < PIECES; ++i) {
+                        const int r = (member + i * THREADS) >> 3;
+                        if (r < walk.rows) {
+#pragma unroll
+                            for (int k = 0; k < D; ++k) {
+                                const uint4 piece = gt_component<T, D>(v[i], k);
+                                unsigned char* at = a + gt_place_k(r * D + k, c);
+                                if constexpr (GtType<T>::SPLIT) {
+                                    float4 hi, lo;
+                                    gt_split(*reinterpret_cast<const float4*>(&piece), hi, lo);
+                                    *reinterpret_cast<float4*>(at) = hi;
+                                    *reinterpret_cast<float4*>(at + 16384) = lo;
+                                } else {
+                                    *reinterpret_cast<uint4*>(at) = piece;
+                                }
                             }
                         }
                     }
+                    if (load_b) {
+                        const T* w = w_group + path.w_off + (TRANS ? (long long)n0 * path.w_ld + u0 : (long long)u0 * path.w_ld + n0);
+                        unsigned char* b = b_base + slot * GtType<T>::b_bytes(n);
+                        if (vec_w) gt_fill_b<T, TRANS, true>(b, w, path.w_ld, n, to.mul - n0, left, k_fill, member);
+                        else gt_fill_b<T, TRANS, false>(b, w, path.w_ld, n, to.mul - n0, left, k_fill, member);
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bars.full + stage);
                 }
-                turn = (turn + sets) & (GT_PW - 1);
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bars.full + stage);
+                if (++turn == GT_SETS) turn = 0;
                 ++it;
                 if (++stage == tile_of.stages) {
                     stage = 0;
@@ -338,7 +405,7 @@ __device__ __forceinline__ void gt_multiply(const GtProblem& gt, const GtArgs& p
 }
 
 // ---------------------------------------------------------------------------- epilogue
-template <class T> struct GtPair;
+template <class T> struct GtPair { static __device__ unsigned of(float, float) { return 0; } };
 template <> struct GtPair<__nv_bfloat16> {
     static __device__ unsigned of(float a, float b) {
         const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
@@ -352,20 +419,99 @@ template <> struct GtPair<__half> {
     }
 };
 
-template <class T>
+// Rows of a tile from shared memory, a warp a row (as pairs of 16-bit values half a warp), U rows on the way together.  Past the
+// tile's rows: the last one again, the same values to the same place.
+template <class T, int D, bool PAIRS, bool FULL>
+__device__ __forceinline__ void gt_write(const float* staging, const int* rows_of, int rows, T* __restrict__ z_col, int dim, int values, int warp, int lane) {
+    constexpr int ROWS = PAIRS ? 8 : 4, U = D == 1 ? 8 : 4, PITCH = 33 * D;
+    const int l = PAIRS ? 2 * (lane & 15) : lane;
+#pragma unroll 1
+    for (int r0 = PAIRS ? 2 * warp + (lane >> 4) : warp; r0 < rows; r0 += ROWS * U) {
+        const float* from[U];
+        T* z[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int r = min(r0 + ROWS * j, rows - 1);
+            from[j] = staging + r * PITCH + l;
+            z[j] = z_col + (long long)rows_of[r] * dim + l;
+        }
+#pragma unroll
+        for (int i = 0; i < D; ++i) {
+            float v[U], w[U];
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                v[j] = from[j][32 * i];
+                if constexpr (PAIRS) w[j] = from[j][32 * i + 1];
+            }
+            if (FULL || 32 * i + l < values) {
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    if constexpr (PAIRS) *reinterpret_cast<unsigned*>(z[j] + 32 * i) = GtPair<T>::of(v[j], w[j]);
+                    else gp_store(z[j] + 32 * i, v[j]);
+                }
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void gt_prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// Rows of a tile, and the weights of its group where they change, to L2 by the epilogue warps.
+template <class T, bool TRANS>
+__device__ __forceinline__ void gt_ahead(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, const GtWalk& walk, bool weights,
+                                         int tid) {
+    constexpr int LINE = 128 / sizeof(T), THREADS = GT_EPI * 32;
+    for (int path_no = to.path_begin; path_no < to.path_end; ++path_no) {
+        const GpPath& path = gt.gp.path[path_no];
+        if (n0 == 0) {                          // (the CTAs of an output block's other channels read the same rows)
+            const int len = path.src_mul * to.d;
+            for (int r = tid >> 3; r < walk.rows; r += THREADS / 8) {
+                const T* x = static_cast<const T*>(p.X) + gp_row(p.order, walk.pos + r) * gt.gp.src_dim + path.src_off;
+                for (int i = (tid & 7) * LINE; i < len; i += 8 * LINE) gt_prefetch(x + i);
+            }
+        }
+        if (weights) {
+            const int n = min(tile_of.n, to.mul - n0), rows = TRANS ? n : path.src_mul, len = TRANS ? path.src_mul : n;
+            const T* w = static_cast<const T*>(p.W) + (long long)walk.g * gt.gp.w_numel + path.w_off + (TRANS ? (long long)n0 * path.w_ld : n0);
+            for (int r = tid >> 2; r < rows; r += THREADS / 4)
+                for (int i = (tid & 3) * LINE; i < len; i += 4 * LINE) gt_prefetch(w + (long long)r * path.w_ld + i);
+        }
+    }
+}
+
+// The chunks of 32 channels of all tiles go to the two groups of four warps in turn.
+template <class T, bool TRANS, int D>
 __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, float* staging,
-                                         const GtBars& bars, GtWalk walk, int tile_rows, unsigned tmem, int warp, int lane) {
-    const int d = to.d, n = tile_of.n, mul = min(n, to.mul - n0), pitch = 33 * d, pair = warp * 32 + lane, r_of = pair / d, k_of = pair % d;
+                                         const GtBars& bars, GtWalk walk, unsigned tmem, int group, int warp, int lane) {
+    constexpr int TILE_ROWS = gt_tile_rows(D), PITCH = 33 * D;
+    const int n = tile_of.n, mul = min(n, to.mul - n0), pair = warp * 32 + lane, r_of = pair / D, k_of = pair % D;
     const float scale = (float)to.scale;
     const unsigned quarter = tmem + ((unsigned)(warp * 32) << 16);
-    int tiles = 0;
+    int* rows_of = bars.rows + 128 * group;
+    staging += group * (GT_STAGING / 4);
+    GtWalk ahead = walk;
+    int have = -1;
+    auto prefetch = [&]() {
+        if (ahead.more()) {
+            ahead.tile(TILE_ROWS);
+            gt_ahead<T, TRANS>(gt, p, tile_of, to, n0, ahead, ahead.g != have, group * 128 + pair);
+            have = ahead.g;
+            ahead.next(p.offsets, p.groups);
+        }
+    };
+    prefetch();
+    prefetch();
+    int tiles = 0, turn = 0;
     for (; walk.more(); walk.next(p.offsets, p.groups), ++tiles) {
-        walk.tile(tile_rows);
+        walk.tile(TILE_ROWS);
         const int buf = tiles & 1;
-        if (pair < walk.rows) bars.rows[pair] = (int)gp_row(p.order, walk.pos + pair);       // (read behind the first barrier below)
+        if (pair < walk.rows) rows_of[pair] = (int)gp_row(p.order, walk.pos + pair);         // (read behind the first barrier below)
+        prefetch();
         if (!warp_wait(true, bars.acc_full + buf, (unsigned)(tiles / 2) & 1, &gt_status, ERR_GT_ACC_FULL)) return;
         tc_fence_after();
-        for (int w0 = 0; w0 < mul; w0 += 32) {
+        bool mine = false;
+        for (int w0 = 0; w0 < mul; w0 += 32, turn ^= 1) {
+            if (turn != group) continue;
+            mine = true;
             unsigned v[32], u[GtType<T>::SPLIT ? 32 : 1];
             const unsigned at = quarter + (unsigned)(buf * 256 + w0);
             tc_load16(at, v);
@@ -375,57 +521,65 @@ __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, c
                 if (w0 + 16 < n) tc_load16(at + n + 16, u + 16);
             }
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            if (w0 + 32 >= mul) {               // the accumulator has been read
+            if (w0 + 32 * GT_EPI_GROUPS >= mul) {           // the group has read its part of the accumulator
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bars.acc_empty + buf);
             }
             if (r_of < walk.rows) {
-                float* to_smem = staging + r_of * pitch + k_of;
+                float* to_smem = staging + r_of * PITCH + k_of;
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
                     float s = __uint_as_float(v[j]);
                     if constexpr (GtType<T>::SPLIT) s += __uint_as_float(u[j]);
-                    to_smem[j * d] = s * scale;
+                    to_smem[j * D] = s * scale;
                 }
             }
-            group_sync(1, GT_EPI * 32);
-            const int values = min(32, mul - w0) * d;
-            T* z_col = static_cast<T*>(p.Z) + to.off + (n0 + w0) * d;
-            for (int r = warp; r < walk.rows; r += GT_EPI) {
-                T* z = z_col + (long long)bars.rows[r] * gt.gp.dst_dim;
-                const float* from = staging + r * pitch;
-                if constexpr (sizeof(T) == 4) {
-                    for (int i = lane; i < values; i += 32) z[i] = from[i];
-                } else {
-                    if (p.z_pair && ((to.off | values) & 1) == 0) {
-                        for (int i = 2 * lane; i < values; i += 64) *reinterpret_cast<unsigned*>(z + i) = GtPair<T>::of(from[i], from[i + 1]);
-                    } else {
-                        for (int i = lane; i < values; i += 32) gp_store(z + i, from[i]);
-                    }
-                }
+            group_sync(1 + group, 128);
+            const int values = min(32, mul - w0) * D;
+            T* z = static_cast<T*>(p.Z) + to.off + (n0 + w0) * D;
+            if (sizeof(T) == 2 && p.z_pair && ((to.off | values) & 1) == 0) {
+                if (values == 32 * D) gt_write<T, D, true, true>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, warp, lane);
+                else gt_write<T, D, true, false>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, warp, lane);
+            } else {
+                if (values == 32 * D) gt_write<T, D, false, true>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, warp, lane);
+                else gt_write<T, D, false, false>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, warp, lane);
             }
-            group_sync(1, GT_EPI * 32);
+            group_sync(1 + group, 128);
+        }
+        if (!mine) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars.acc_empty + buf);
+            group_sync(1 + group, 128);         // (rows_of is written again by all four warps)
         }
     }
 }
 
+// What a role does for blocks of D components.
+template <class T, bool TRANS, int D>
+__device__ __forceinline__ void gt_roles(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, unsigned char* a_base,
+                                         unsigned char* b_base, float* staging, const GtBars& bars, const GtWalk& walk, unsigned tmem, int warp, int tid) {
+    if (warp < GT_PW) gt_produce<T, TRANS, D>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid);
+    else gt_drain<T, TRANS, D>(gt, p, tile_of, to, n0, staging, bars, walk, tmem, (warp - GT_PW) >> 2, warp & 3, tid & 31);
+}
+
 template <class T, bool TRANS>
 __global__ void __launch_bounds__(GT_THREADS, 1) oeq_grouped_tc(const __grid_constant__ GtProblem gt, const GtArgs p) {
-    extern __shared__ __align__(16) unsigned char gt_smem[];
-    unsigned char* smem = gt_smem + ((1024u - (smem_u32(gt_smem) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) unsigned char gt_smem[];
+    unsigned char* smem = gt_smem;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     int t = 0;
     while (t + 1 < gt.gp.n_targets && (int)blockIdx.x >= gt.target[t + 1].first) ++t;
     const GpTarget& to = gt.gp.target[t];
     const GtTarget& tile_of = gt.target[t];
     const int local = (int)blockIdx.x - tile_of.first, part = local / tile_of.n_tiles, n0 = local % tile_of.n_tiles * tile_of.n, d = to.d;
-    unsigned char *a_base = smem + GT_CONTROL, *b_base = a_base + tile_of.stages * GtType<T>::A_BYTES;
+    unsigned char *a_base = smem, *b_base = a_base + tile_of.stages * GtType<T>::A_BYTES;
     float* staging = reinterpret_cast<float*>(b_base + tile_of.slots * GtType<T>::b_bytes(tile_of.n));
-    const GtBars bars(smem);
+    unsigned char* control = reinterpret_cast<unsigned char*>(staging) + GT_EPI_GROUPS * GT_STAGING;
+    const GtBars bars(control);
     if (tid == 0) {
         for (int i = 0; i < GT_STAGES; ++i) {
-            mbar_init(bars.full + i, GT_PW);
+            mbar_init(bars.full + i, GT_SET);
             mbar_init(bars.empty + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -439,30 +593,22 @@ __global__ void __launch_bounds__(GT_THREADS, 1) oeq_grouped_tc(const __grid_con
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(bars.tmem)), "n"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    const bool work = to.path_begin < to.path_end;              // (a block without a path is zero in every row)
+    GtRange& range = *reinterpret_cast<GtRange*>(control + 256);
     tc_fence_before();
-    __syncthreads();
+    gt_range(range, p.offsets, p.groups, p.rows, part, tile_of.parts, tile_of.extra);       // (two barriers)
     tc_fence_after();
     const unsigned tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile unsigned*>(bars.tmem), 0);
-    const long long n = min(__ldg(p.offsets + p.groups), p.rows);
-    const bool work = to.path_begin < to.path_end;              // (a block without a path is zero in every row)
-    const GtWalk walk(p.offsets, p.groups, work ? gp_cut(n, part, tile_of.parts) : 0, work ? gp_cut(n, part + 1, tile_of.parts) : 0);
-    const int tile_rows = 128 / d;
-    if (warp < GT_PW) {
-        switch (d) {
-            case 1: gt_produce<T, TRANS, 1>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid); break;
-            case 3: gt_produce<T, TRANS, 3>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid); break;
-            case 5: gt_produce<T, TRANS, 5>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid); break;
-            case 7: gt_produce<T, TRANS, 7>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid); break;
-            default: gt_produce<T, TRANS, 9>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid); break;
-        }
-    } else if (warp < MMA_WARP) {
-        gt_drain<T>(gt, p, tile_of, to, n0, staging, bars, walk, tile_rows, tmem, warp - GT_PW, lane);
-    } else {
-        gt_multiply<T, TRANS>(gt, p, tile_of, to, a_base, b_base, bars, walk, tile_rows, tmem, elect_lane());
-    }
+    const GtWalk walk(p.offsets, range.g, work ? range.lo : 0, work ? range.hi : 0);
+    if (warp == MMA_WARP) gt_multiply<T, TRANS>(gt, p, tile_of, to, a_base, b_base, bars, walk, gt_tile_rows(d), tmem, elect_lane());
+    else if (d == 1) gt_roles<T, TRANS, 1>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
+    else if (d == 3) gt_roles<T, TRANS, 3>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
+    else if (d == 5) gt_roles<T, TRANS, 5>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
+    else if (d == 7) gt_roles<T, TRANS, 7>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
+    else gt_roles<T, TRANS, 9>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
     // zeros: the rows without a group, every row where the block has no path
     {
-        const long long from = work ? n : 0, count = p.rows - from;
+        const long long from = work ? min(__ldg(p.offsets + p.groups), p.rows) : 0, count = p.rows - from;
         const long long lo = from + gp_cut(count, part, tile_of.parts), hi = from + gp_cut(count, part + 1, tile_of.parts);
         const int values = min(tile_of.n, to.mul - n0) * d;
         for (long long at = lo + warp; at < hi; at += GT_THREADS / 32) {

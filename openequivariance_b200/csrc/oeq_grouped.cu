@@ -162,6 +162,7 @@ int tc_plan(const GpProblem& gp, int64_t rows, int sms, GtProblem& gt, int& ctas
             k += gp.path[p].src_mul;
             x.chunks += (gp.path[p].src_mul + GtType<T>::KC - 1) / GtType<T>::KC;
         }
+        x.extra = 96 / to.d;
         cost[t] = to.d * (double)(k + x.n + 32);
         ctas += x.n_tiles;
     }
@@ -173,7 +174,7 @@ int tc_plan(const GpProblem& gp, int64_t rows, int sms, GtProblem& gt, int& ctas
         ++gt.target[most].parts;
         ctas += gt.target[most].n_tiles;
     }
-    const size_t room = SMEM_MOST - GT_CONTROL - 1024 - GT_STAGING;
+    const size_t fixed = GT_CONTROL + GT_EPI_GROUPS * GT_STAGING, room = SMEM_MOST - fixed;
     smem = 0;
     ctas = 0;
     for (int t = 0; t < gp.n_targets; ++t) {
@@ -190,7 +191,7 @@ int tc_plan(const GpProblem& gp, int64_t rows, int sms, GtProblem& gt, int& ctas
         }
         smem = std::max(smem, x.stages * a + x.slots * b);
     }
-    smem = std::max<size_t>(smem + GT_CONTROL + 1024 + GT_STAGING, 120 * 1024);         // (one CTA an SM: it takes all of the tensor memory)
+    smem = std::max<size_t>(smem + fixed, 120 * 1024);         // (one CTA an SM: it takes all of the tensor memory)
     return OEQ_OK;
 }
 
