@@ -19,6 +19,7 @@ SOURCES = ["oeq_runtime.cu", "oeq_grouped.cu"]
 TORCH_SOURCES = ["oeq_torch.cpp", "oeq_torch_grouped.cpp"]
 # headers of the kernels that are compiled with the library (those of the others are read at run time)
 INCLUDED = ["oeq_internal.h", "oeq_common.cuh", "tc_common.cuh", "grouped_kernels.cuh", "grouped_tc_kernels.cuh",
+            "grouped_tc_dw_kernels.cuh",
             "row_groups_kernels.cuh"]
 
 

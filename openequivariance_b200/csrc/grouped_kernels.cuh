@@ -59,9 +59,6 @@ __device__ __forceinline__ long long gp_row(const long long* __restrict__ order,
 
 // The grouped rows are cut into `parts` equal ranges of sorted positions.
 __device__ __forceinline__ long long gp_cut(long long n, int part, int parts) { return (long long)((unsigned long long)n * part / parts); }
-// The range that position p of n is in.
-__device__ __forceinline__ int gp_part(long long n, long long p, int parts) { return (int)(((unsigned long long)(p + 1) * parts - 1) / (unsigned long long)n); }
-
 constexpr int GP_TILE = 64, GP_STEP = 16, GP_SIMT_THREADS = 256;
 
 // acc[4][4] += a[k][row] b[k][col] over GP_STEP staged steps
@@ -178,7 +175,7 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __g
                                                                        const T* __restrict__ X, const T* __restrict__ dZ,
                                                                        const long long* __restrict__ order, const long long* __restrict__ offsets,
                                                                        long long rows, int groups, T* __restrict__ dW,
-                                                                       typename GpAcc<T>::type* __restrict__ partial) {
+                                                                       typename GpAcc<T>::type* __restrict__ partial, long long* __restrict__ lo_of) {
     typedef typename GpAcc<T>::type A;
     __shared__ __align__(16) A sa[GP_STEP][GP_TILE], sb[GP_STEP][GP_TILE];
     const int tid = threadIdx.x;
@@ -188,9 +185,8 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __g
     const GpTarget& to = gp.target[path.dst];
     const int parts = split.parts[p], part = ((int)blockIdx.x - split.first[p]) % parts, tile_of = ((int)blockIdx.x - split.first[p]) / parts;
     const int w_tiles = (to.mul + GP_TILE - 1) / GP_TILE, u_tile = tile_of / w_tiles * GP_TILE, w_tile = tile_of % w_tiles * GP_TILE, d = to.d;
-    const long long n = min(__ldg(offsets + groups), rows);
-    if (n == 0) return;
-    const long long lo = gp_cut(n, part, parts), hi = gp_cut(n, part + 1, parts);
+    const long long n = min(__ldg(offsets + groups), rows), lo = gp_cut(n, part, parts), hi = gp_cut(n, part + 1, parts);
+    if (tid == 0) lo_of[blockIdx.x] = lo;
     if (lo >= hi) return;
     const int k_s = tid / 16, c_s = tid % 16, r0 = tid / 16 * 4, c0 = tid % 16 * 4;
     int g = gp_group(offsets, groups, lo);
@@ -244,11 +240,11 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __g
 }
 
 // Gradients of the groups that no single range has: the sum of their parts, and zeros where there are no rows.
-// Blocks x over the weights, y over the groups.
+// lo_of: first positions of the CTAs' ranges, ascending over the parts of a tile.  Blocks x over the weights, y over the groups.
 template <class T>
 __global__ void __launch_bounds__(256) oeq_grouped_join(const __grid_constant__ GpProblem gp, const __grid_constant__ GpSplit split,
                                                         const long long* __restrict__ offsets, long long rows, int groups, int tile_u, int tile_w,
-                                                        const typename GpAcc<T>::type* __restrict__ partial, T* __restrict__ dW) {
+                                                        const typename GpAcc<T>::type* __restrict__ partial, const long long* __restrict__ lo_of, T* __restrict__ dW) {
     typedef typename GpAcc<T>::type A;
     const int i = blockIdx.x * 256 + threadIdx.x;
     if (i >= gp.w_numel) return;
@@ -256,18 +252,27 @@ __global__ void __launch_bounds__(256) oeq_grouped_join(const __grid_constant__ 
     while (p + 1 < gp.n_paths && i >= gp.path[p + 1].w_off) ++p;           // (the paths lie in the order of their weights)
     const GpPath& path = gp.path[p];
     const int parts = split.parts[p], u = (i - path.w_off) / path.w_ld, w = (i - path.w_off) % path.w_ld;
+    const int cta = split.first[p] + (u / tile_u * ((path.w_ld + tile_w - 1) / tile_w) + w / tile_w) * parts;
     const long long tile = (long long)tile_u * tile_w, n = min(__ldg(offsets + groups), rows);
-    const A* at = partial + (split.first[p] + (long long)(u / tile_u * ((path.w_ld + tile_w - 1) / tile_w) + w / tile_w) * parts) * 2 * tile +
-                  (long long)(u % tile_u) * tile_w + w % tile_w;
+    const A* at = partial + cta * 2 * tile + (long long)(u % tile_u) * tile_w + w % tile_w;
+    auto part_of = [&](long long position) {    // the last range that begins at or before it
+        int a = 0, b = parts - 1;
+        while (a < b) {
+            const int mid = (a + b + 1) >> 1;
+            if (__ldg(lo_of + cta + mid) <= position) a = mid;
+            else b = mid - 1;
+        }
+        return a;
+    };
     for (int g = blockIdx.y; g < groups; g += gridDim.y) {
         const long long begin = min(__ldg(offsets + g), n), end = min(__ldg(offsets + g + 1), n);
         A s = A(0);
         if (begin < end) {
-            const int j0 = gp_part(n, begin, parts), j1 = gp_part(n, end - 1, parts);
+            const int j0 = part_of(begin), j1 = part_of(end - 1);
             if (j0 == j1) continue;
             s = at[(j0 * 2 + 1) * tile];
             for (int j = j0 + 1; j <= j1; ++j)
-                if (n >= parts || gp_cut(n, j, parts) < gp_cut(n, j + 1, parts)) s += at[j * 2 * tile];    // (a range without rows has no part)
+                if (j == j1 || __ldg(lo_of + cta + j) < __ldg(lo_of + cta + j + 1)) s += at[j * 2 * tile];     // (a range without rows has no part)
             s *= (A)gp.target[path.dst].scale;
         }
         gp_store(dW + (long long)g * gp.w_numel + i, s);

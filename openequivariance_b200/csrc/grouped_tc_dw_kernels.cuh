@@ -1,0 +1,381 @@
+// Weight gradient of the linear maps with one set of weights for each group of rows, on the 5th-generation tensor cores: FP32 (3xTF32),
+// BF16 and FP16, up to GT_D_MAX components.  FP32 sums.
+//
+//   dW_g[i,o][u,w] = c_o sum_{r in g, k} X[r,i,u,k] dZ[r,o,w,k]
+//
+// M = 128 input channels u, N = up to 128 output channels w of one path, and the sum runs over rows and components.  Both operands have their
+// channels along memory, so both are "MN-major": a lane reads the 16 d bytes of V channels of a row and writes d pieces, one into
+// the slot of each component.  A slot of the ring has one component of GdType::ROWS sorted rows of one group, X and dZ, 16 KB.
+//   * 8 producer warps: two sets of four take units of rows in turn (seven and more components: one set, as the slots of two units have
+//     to fit the ring);
+//   * one warp, in step, issues the MMAs: FP32 hi.hi and hi.lo as one, lo.hi into hi.lo's columns;
+//   * 8 warps add the accumulators to sums in registers at the end of a group and after CHAIN slots: an MMA's additions are cut off, not
+//     rounded, and the error grows with the length of a chain (relative, one chain of 750 slots: 1e-5).  The two accumulators alternate.
+// A CTA has one tile of one path and a range of the sorted rows (gt_range); groups that go beyond the range leave a partial tile for
+// oeq_grouped_join.  Every wait is bounded.
+#pragma once
+#include "grouped_tc_kernels.cuh"
+
+namespace oeq {
+
+constexpr int GD_TILE = 128, GD_RING = 12, GD_SLOT = 16384;
+constexpr int GD_PW = 8, GD_EPI = 8, GD_THREADS = (GD_PW + GD_EPI + 1) * 32;
+constexpr int GD_SMEM = GD_RING * GD_SLOT + 1024;
+constexpr int ERR_GD_EMPTY = 91, ERR_GD_FULL = 92, ERR_GD_ACC_FULL = 93, ERR_GD_ACC_EMPTY = 94;
+
+template <class T> struct GdType { static constexpr int ROWS = 32, CHAIN = 256; };
+template <> struct GdType<float> { static constexpr int ROWS = 8, CHAIN = 32; };
+__host__ __device__ constexpr int gd_sets(int d) { return d <= 5 ? 2 : 1; }
+// rows of a unit: whole slots, at most 56 registers of a lane on the way
+template <class T> __host__ __device__ constexpr int gd_unit(int d) { return sizeof(T) == 4 ? (d == 1 ? 32 : (d == 3 ? 16 : 8)) : (d == 1 ? 64 : 32); }
+
+struct GdProblem {
+    GpProblem gp;               // paths in the order of their weights
+    GpSplit split;
+    int extra[GP_PATHS];        // time of a group, in rows
+};
+struct GdArgs {
+    const void *X, *dZ;
+    const long long *order, *offsets;
+    void* dW;
+    float* partial;             // [CTAs][2][128][128]
+    long long* lo;              // [CTAs] first position of each CTA's range
+    long long rows;
+    int groups;
+    int x_vec, z_vec, w_vec;    // rows of X and dZ, weights of dW in 16-byte pieces
+};
+
+// byte offset of V channels from ch of row r (of the slot's) in an operand with `blocks` blocks of channels
+template <class T>
+__device__ __forceinline__ int gd_place(int ch, int r, int blocks) {
+    if constexpr (GtType<T>::SPLIT) return (ch >> 5) * 1024 + r * 128 + (((ch & 31) * 4) ^ ((r & 3) << 5));
+    else return (r >> 3) * (blocks * 1024) + (ch >> 6) * 1024 + (r & 7) * 128 + ((((ch >> 3) & 7) ^ (r & 7)) << 4);
+}
+template <class T>
+__device__ __forceinline__ unsigned long long gd_desc(unsigned addr, int blocks) {
+    const unsigned long long base = (unsigned long long)((addr >> 4) & 0x3fff) | (unsigned long long)(1024 >> 4) << 16 | 1ull << 46;
+    if constexpr (GtType<T>::SPLIT) return base | (unsigned long long)(512 >> 4) << 32 | 1ull << 61;
+    else return base | (unsigned long long)(blocks * 1024 >> 4) << 32 | 2ull << 61;
+}
+
+struct GdBars {
+    unsigned long long *full, *empty, *acc_full, *acc_empty;
+    unsigned* tmem;
+    __device__ explicit GdBars(unsigned char* control) {
+        full = reinterpret_cast<unsigned long long*>(control);
+        empty = full + GD_RING;
+        acc_full = empty + GD_RING;
+        acc_empty = acc_full + 2;
+        tmem = reinterpret_cast<unsigned*>(acc_empty + 2);
+    }
+};
+
+// A unit's place in the chain of sums.
+template <class T> struct GdChain {
+    int slots = 0;              // since the accumulator was begun
+    bool begins = true;         // the unit begins an accumulator
+    bool ends = false, piece_ends = false;              // the unit ends it; ends the group's rows in this range
+    __device__ int unit(const GtWalk& walk, int d) {
+        const int n = (walk.rows + GdType<T>::ROWS - 1) / GdType<T>::ROWS * d;
+        begins = slots == 0;
+        slots += n;
+        piece_ends = walk.pos + walk.rows >= walk.end;
+        ends = piece_ends || slots >= GdType<T>::CHAIN;
+        if (ends) slots = 0;
+        return n;
+    }
+};
+
+// ---------------------------------------------------------------------------- producers
+template <class T, int D, bool FAST>
+__device__ __forceinline__ void gd_fill(const GdArgs& p, const GpProblem& gp, const GtWalk& walk, const T* x, const T* z, int mu, int mw, int n, unsigned char* ring,
+                                        int first, const GdBars& bars, int use, int member, bool& ok) {
+    const int lane = member & 31;
+    constexpr int V = GtType<T>::V, ROWS = GdType<T>::ROWS, THREADS = GD_PW * 32 / gd_sets(D), PASS = D == 1 ? 8 : (D == 3 ? 4 : (D <= 7 ? 2 : 1));
+    const int slots = (walk.rows + ROWS - 1) / ROWS, rows = slots * ROWS, across_x = (mu + V - 1) / V, across_z = (mw + V - 1) / V;
+    const int tasks_x = rows * across_x, tasks = tasks_x + rows * across_z;
+    const unsigned magic_x = (65536 + across_x - 1) / across_x, magic_z = (65536 + across_z - 1) / across_z;     // i / across for i <= 2048
+    bool waited = false;
+    auto wait = [&]() {                         // until every slot of the unit is free again
+        if (waited) return;
+        waited = true;
+        for (int s = 0; s < slots * D && ok; ++s) {
+            const int at_ring = first + s < GD_RING ? first + s : first + s - GD_RING, u = first + s < GD_RING ? use : use + 1;
+            if (u > 0) ok = warp_wait(ok, bars.empty + at_ring, (unsigned)(u - 1) & 1, &gt_status, ERR_GD_EMPTY);
+        }
+    };
+#pragma unroll 1
+    for (int i0 = member; i0 - lane < tasks; i0 += PASS * THREADS) {         // (in step: a warp waits as one)
+        uint4 v[PASS][D];
+        int at[PASS], r_of[PASS];               // channel (of dZ: behind 128), row
+#pragma unroll
+        for (int j = 0; j < PASS; ++j) {
+            const int i = min(i0 + j * THREADS, tasks - 1), is_z = i >= tasks_x, q = is_z ? i - tasks_x : i;
+            const int r = (int)((q * (is_z ? magic_z : magic_x)) >> 16), ch = (q - r * (is_z ? across_z : across_x)) * V;
+            const long long row = gp_row(p.order, walk.pos + min(r, walk.rows - 1));
+            const T* src = (is_z ? z + row * gp.dst_dim : x + row * gp.src_dim) + ch * D;
+            gt_read<T, D, FAST>(v[j], src, r < walk.rows ? (is_z ? mw : mu) - ch : 0);
+            at[j] = is_z ? ch + GD_TILE : ch;
+            r_of[j] = r;
+        }
+        wait();
+        if (!ok) return;
+#pragma unroll
+        for (int j = 0; j < PASS; ++j) {
+            if (i0 + j * THREADS >= tasks) continue;
+            const int is_z = at[j] >= GD_TILE, ch = is_z ? at[j] - GD_TILE : at[j], r = r_of[j] % ROWS;
+            const int place = is_z ? 8192 + gd_place<T>(ch, r, (n + 63) / 64) : gd_place<T>(ch, r, GD_TILE / 64);
+            const int lo = is_z ? 8192 + gd_place<T>(ch + n, r, 0) : place + 4096;
+            int slot = first + r_of[j] / ROWS * D;
+            if (slot >= GD_RING) slot -= GD_RING;
+#pragma unroll
+            for (int k = 0; k < D; ++k) {
+                const uint4 piece = gt_component<T, D>(v[j], k);
+                unsigned char* dst = ring + slot * GD_SLOT;
+                if (++slot == GD_RING) slot = 0;
+                if constexpr (GtType<T>::SPLIT) {
+                    float4 hi, lo4;
+                    gt_split(*reinterpret_cast<const float4*>(&piece), hi, lo4);
+                    *reinterpret_cast<float4*>(dst + place) = hi;
+                    *reinterpret_cast<float4*>(dst + lo) = lo4;
+                } else {
+                    *reinterpret_cast<uint4*>(dst + place) = piece;
+                }
+            }
+        }
+    }
+    wait();                                     // (a warp without a task)
+}
+
+template <class T, int D>
+__device__ __forceinline__ void gd_produce(const GdArgs& p, const GpProblem& gp, const GpPath& path, const GpTarget& to, int u0, int w0, int mu, int mw, int n,
+                                           unsigned char* ring, const GdBars& bars, GtWalk walk, int tid) {
+    constexpr int V = GtType<T>::V, ROWS = GdType<T>::ROWS, SETS = gd_sets(D), THREADS = GD_PW * 32 / SETS, UNIT = gd_unit<T>(D), LINE = 128 / sizeof(T);
+    const int set = tid / THREADS, member = tid % THREADS, lane = tid & 31;
+    const T *x = static_cast<const T*>(p.X) + path.src_off + u0 * D, *z = static_cast<const T*>(p.dZ) + to.off + w0 * D;
+    const bool fast = p.x_vec && p.z_vec && path.src_off % V == 0 && path.src_mul % V == 0 && to.off % V == 0 && to.mul % V == 0;
+    GtWalk ahead = walk;
+    int turn = 0, turn_ahead = 0, first = 0, use = 0;
+    bool ok = true;
+    auto prefetch = [&]() {                     // the set's unit after next, to L2
+        while (ahead.more()) {
+            ahead.tile(UNIT);
+            const bool mine = turn_ahead == set;
+            if (mine) {
+                for (int r = member >> 3; r < ahead.rows; r += THREADS / 8) {
+                    const long long row = gp_row(p.order, ahead.pos + r);
+                    for (int i = (member & 7) * LINE; i < mu * D; i += 8 * LINE) gt_prefetch(x + row * gp.src_dim + i);
+                    for (int i = (member & 7) * LINE; i < mw * D; i += 8 * LINE) gt_prefetch(z + row * gp.dst_dim + i);
+                }
+            }
+            ahead.next(p.offsets, p.groups);
+            if (++turn_ahead == SETS) turn_ahead = 0;
+            if (mine) break;
+        }
+    };
+    prefetch();
+    prefetch();
+    for (; walk.more(); walk.next(p.offsets, p.groups)) {
+        walk.tile(UNIT);
+        const int slots = (walk.rows + ROWS - 1) / ROWS * D;
+        if (turn == set) {
+            prefetch();
+            if (fast) gd_fill<T, D, true>(p, gp, walk, x, z, mu, mw, n, ring, first, bars, use, member, ok);
+            else gd_fill<T, D, false>(p, gp, walk, x, z, mu, mw, n, ring, first, bars, use, member, ok);
+            if (!__all_sync(0xffffffffu, ok)) return;
+            fence_async_smem();
+            __syncwarp();
+            if (lane < slots) mbar_arrive(bars.full + (first + lane < GD_RING ? first + lane : first + lane - GD_RING));
+        }
+        if (++turn == SETS) turn = 0;
+        first += slots;
+        if (first >= GD_RING) {
+            first -= GD_RING;
+            ++use;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------- MMA
+template <class T>
+__device__ __forceinline__ void gd_multiply(const GdArgs& p, int d, int unit, int n, unsigned char* ring, const GdBars& bars, GtWalk walk, unsigned tmem, unsigned leader) {
+    constexpr unsigned MN = 1u << 15 | 1u << 16;
+    const int blocks = (n + 63) / 64;
+    const unsigned wide = gt_idesc<T, false>(GtType<T>::acc(n)) | MN, narrow = gt_idesc<T, false>(n) | MN;
+    const unsigned long long a0 = gd_desc<T>(smem_u32(ring), GD_TILE / 64), b0 = gd_desc<T>(smem_u32(ring) + 8192, blocks);
+    GdChain<T> chain;
+    int slot = 0, use = 0, accs = 0;
+    unsigned accumulate = 0;
+    bool ok = true;
+    for (; walk.more() && ok; walk.next(p.offsets, p.groups)) {
+        walk.tile(unit);
+        const int slots = chain.unit(walk, d), buf = accs & 1;
+        if (chain.begins) {
+            if (accs >= 2) ok = warp_wait(ok, bars.acc_empty + buf, (unsigned)(accs / 2 - 1) & 1, &gt_status, ERR_GD_ACC_EMPTY);
+            accumulate = 0;
+        }
+        const unsigned acc = tmem + (unsigned)(buf * 256);
+        for (int s = 0; s < slots && ok; ++s) {
+            ok = warp_wait(ok, bars.full + slot, (unsigned)use & 1, &gt_status, ERR_GD_FULL);
+            if (!ok) break;
+            tc_fence_after();
+            const unsigned long long a = a0 + (unsigned long long)(slot * (GD_SLOT >> 4)), b = b0 + (unsigned long long)(slot * (GD_SLOT >> 4));
+            if constexpr (GtType<T>::SPLIT) {
+                gt_mma<T>(leader, acc, a, b, wide, accumulate);
+                gt_mma<T>(leader, acc + (unsigned)n, a + (4096 >> 4), b, narrow, 1);
+                accumulate = 1;
+            } else {
+#pragma unroll
+                for (int h = 0; h < GdType<T>::ROWS / 16; ++h) {
+                    gt_mma<T>(leader, acc, a + (unsigned long long)(h * (2 * (GD_TILE / 64) * 1024 >> 4)), b + (unsigned long long)(h * (2 * blocks * 1024 >> 4)), wide, accumulate);
+                    accumulate = 1;
+                }
+            }
+            tc_commit_if(leader, bars.empty + slot);
+            if (++slot == GD_RING) {
+                slot = 0;
+                ++use;
+            }
+        }
+        if (ok && chain.ends) {
+            tc_commit_if(leader, bars.acc_full + buf);
+            ++accs;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------- sums
+// A lane has one input channel, a warp's half of the warps 64 output channels.
+template <class T>
+__device__ __forceinline__ void gd_sum(const GdArgs& p, const GpProblem& gp, const GpPath& path, const GpTarget& to, int d, int unit, int u0, int w0, int mu, int mw, int n,
+                                       const GdBars& bars, GtWalk walk, long long lo, long long hi, unsigned tmem, int warp, int lane) {
+    constexpr int COLS = GD_TILE / 2;
+    const int quarter = warp & 3, c0 = (warp >> 2) * COLS, u = quarter * 32 + lane;
+    const unsigned at = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)c0;
+    const float scale = (float)to.scale;
+    GdChain<T> chain;
+    float sum[COLS];
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) sum[j] = 0.f;
+    int accs = 0;
+    for (; walk.more(); walk.next(p.offsets, p.groups)) {
+        walk.tile(unit);
+        chain.unit(walk, d);
+        if (!chain.ends) continue;
+        const int buf = accs & 1;
+        if (!warp_wait(true, bars.acc_full + buf, (unsigned)(accs / 2) & 1, &gt_status, ERR_GD_ACC_FULL)) return;
+        tc_fence_after();
+#pragma unroll
+        for (int j = 0; j < COLS; j += 16) {
+            if (c0 + j < n) {
+                unsigned v[16], w[16];
+                tc_load16(at + (unsigned)(buf * 256 + j), v);
+                if constexpr (GtType<T>::SPLIT) tc_load16(at + (unsigned)(buf * 256 + n + j), w);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float s = __uint_as_float(v[i]);
+                    if constexpr (GtType<T>::SPLIT) s += __uint_as_float(w[i]);
+                    sum[j + i] += s;
+                }
+            }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars.acc_empty + buf);
+        ++accs;
+        if (!chain.piece_ends) continue;
+        const long long begin = __ldg(p.offsets + walk.g), end = __ldg(p.offsets + walk.g + 1);
+        if (begin >= lo && end <= hi) {
+            if (u < mu) {
+                T* out = static_cast<T*>(p.dW) + (long long)walk.g * gp.w_numel + path.w_off + (long long)(u0 + u) * path.w_ld + w0 + c0;
+                if constexpr (sizeof(T) == 4) {
+                    if (p.w_vec && ((path.w_off | path.w_ld) & 3) == 0) {
+#pragma unroll
+                        for (int j = 0; j < COLS; j += 4)
+                            if (c0 + j < mw)
+                                *reinterpret_cast<float4*>(out + j) = make_float4(sum[j] * scale, sum[j + 1] * scale, sum[j + 2] * scale, sum[j + 3] * scale);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < COLS; ++j)
+                            if (c0 + j < mw) out[j] = sum[j] * scale;
+                    }
+                } else {
+                    if (p.w_vec && ((path.w_off | path.w_ld) & 7) == 0) {
+#pragma unroll
+                        for (int j = 0; j < COLS; j += 8)
+                            if (c0 + j < mw)
+                                *reinterpret_cast<uint4*>(out + j) = make_uint4(GtPair<T>::of(sum[j] * scale, sum[j + 1] * scale), GtPair<T>::of(sum[j + 2] * scale, sum[j + 3] * scale),
+                                                                                GtPair<T>::of(sum[j + 4] * scale, sum[j + 5] * scale), GtPair<T>::of(sum[j + 6] * scale, sum[j + 7] * scale));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < COLS; ++j)
+                            if (c0 + j < mw) gp_store(out + j, sum[j] * scale);
+                    }
+                }
+            }
+        } else if (u < mu) {
+            float* out = p.partial + ((long long)blockIdx.x * 2 + (begin < lo ? 0 : 1)) * (GD_TILE * GD_TILE) + u * GD_TILE + c0;
+#pragma unroll
+            for (int j = 0; j < COLS; j += 4)
+                if (c0 + j < mw) *reinterpret_cast<float4*>(out + j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
+        }
+#pragma unroll
+        for (int j = 0; j < COLS; ++j) sum[j] = 0.f;
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(GD_THREADS, 1) oeq_grouped_tc_dw(const __grid_constant__ GdProblem gd, const GdArgs p) {
+    extern __shared__ __align__(1024) unsigned char gt_smem[];
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    int path_no = 0;
+    while ((int)blockIdx.x >= gd.split.first[path_no + 1]) ++path_no;
+    const GpPath& path = gd.gp.path[path_no];
+    const GpTarget& to = gd.gp.target[path.dst];
+    const int parts = gd.split.parts[path_no], local = (int)blockIdx.x - gd.split.first[path_no], tile = local / parts, part = local % parts, d = to.d;
+    const int w_tiles = (to.mul + GD_TILE - 1) / GD_TILE, u0 = tile / w_tiles * GD_TILE, w0 = tile % w_tiles * GD_TILE;
+    const int mu = min(GD_TILE, path.src_mul - u0), mw = min(GD_TILE, to.mul - w0), n = (mw + 15) / 16 * 16;
+    unsigned char* control = gt_smem + GD_RING * GD_SLOT;
+    const GdBars bars(control);
+    GtRange& range = *reinterpret_cast<GtRange*>(control + 512);
+    constexpr int MMA_WARP = GD_PW + GD_EPI;
+    if (tid == 0) {
+        for (int i = 0; i < GD_RING; ++i) {
+            mbar_init(bars.full + i, GD_PW / gd_sets(d));
+            mbar_init(bars.empty + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bars.acc_full + i, 1);
+            mbar_init(bars.acc_empty + i, GD_EPI);
+        }
+        fence_mbar_init();
+    }
+    if (warp == MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(bars.tmem)), "n"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    gt_range(range, p.offsets, p.groups, p.rows, part, parts, gd.extra[path_no]);
+    tc_fence_after();
+    const unsigned tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile unsigned*>(bars.tmem), 0);
+    const long long lo = range.lo, hi = range.hi;
+    if (tid == 0) p.lo[blockIdx.x] = lo;
+    const GtWalk walk(p.offsets, range.g, lo, hi);
+    if (warp == MMA_WARP) {
+        gd_multiply<T>(p, d, gd_unit<T>(d), n, gt_smem, bars, walk, tmem, elect_lane());
+    } else if (warp >= GD_PW) {
+        gd_sum<T>(p, gd.gp, path, to, d, gd_unit<T>(d), u0, w0, mu, mw, n, bars, walk, lo, hi, tmem, warp - GD_PW, lane);
+    } else {
+        if (d == 1) gd_produce<T, 1>(p, gd.gp, path, to, u0, w0, mu, mw, n, gt_smem, bars, walk, tid);
+        else if (d == 3) gd_produce<T, 3>(p, gd.gp, path, to, u0, w0, mu, mw, n, gt_smem, bars, walk, tid);
+        else if (d == 5) gd_produce<T, 5>(p, gd.gp, path, to, u0, w0, mu, mw, n, gt_smem, bars, walk, tid);
+        else if (d == 7) gd_produce<T, 7>(p, gd.gp, path, to, u0, w0, mu, mw, n, gt_smem, bars, walk, tid);
+        else gd_produce<T, 9>(p, gd.gp, path, to, u0, w0, mu, mw, n, gt_smem, bars, walk, tid);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+}
+
+}  // namespace oeq

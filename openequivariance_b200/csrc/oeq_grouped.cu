@@ -13,6 +13,7 @@
 #include "../../include/oeq_b200.h"
 #include "oeq_internal.h"
 #include "grouped_kernels.cuh"
+#include "grouped_tc_dw_kernels.cuh"
 #include "grouped_tc_kernels.cuh"
 #include "row_groups_kernels.cuh"
 
@@ -116,11 +117,14 @@ GpSplit simt_split(const GpProblem& gp, int64_t rows, int sms) {
     return s;
 }
 
+// The workspace of a weight gradient: the CTAs' first positions, then their partial tiles.
+size_t positions_bytes(const GpProblem& gp, const GpSplit& split) { return ((size_t)split.first[gp.n_paths] * sizeof(int64_t) + 255) / 256 * 256; }
+
 template <class T>
-int join(const GpProblem& gp, const GpSplit& split, int tile_u, int tile_w, int64_t rows, int64_t groups, const int64_t* offsets, void* dW, const void* ws,
-         cudaStream_t st) {
+int join(const GpProblem& gp, const GpSplit& split, int tile, int64_t rows, int64_t groups, const int64_t* offsets, void* dW, const void* ws, cudaStream_t st) {
     const dim3 grid((unsigned)((gp.w_numel + 255) / 256), (unsigned)std::min<int64_t>(groups, 1024));
-    oeq_grouped_join<T><<<grid, 256, 0, st>>>(gp, split, (const long long*)offsets, rows, (int)groups, tile_u, tile_w, (const typename GpAcc<T>::type*)ws, (T*)dW);
+    oeq_grouped_join<T><<<grid, 256, 0, st>>>(gp, split, (const long long*)offsets, rows, (int)groups, tile, tile,
+                                              (const typename GpAcc<T>::type*)((const char*)ws + positions_bytes(gp, split)), (const long long*)ws, (T*)dW);
     OEQ_CUDA(cudaGetLastError());
     return OEQ_OK;
 }
@@ -131,13 +135,11 @@ int simt_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* 
     int sms = 0;
     if (int rc = sm_count(sms)) return rc;
     const GpSplit split = simt_split(gp, rows, sms);
-    if (rows > 0) {
-        oeq_grouped_simt_dw<T><<<split.first[gp.n_paths], GP_SIMT_THREADS, 0, st>>>(gp, split, (const T*)X, (const T*)dZ, (const long long*)order,
-                                                                                    (const long long*)offsets, rows, (int)groups, (T*)dW,
-                                                                                    (typename GpAcc<T>::type*)ws);
-        OEQ_CUDA(cudaGetLastError());
-    }
-    return join<T>(gp, split, GP_TILE, GP_TILE, rows, groups, offsets, dW, ws, st);
+    oeq_grouped_simt_dw<T><<<split.first[gp.n_paths], GP_SIMT_THREADS, 0, st>>>(gp, split, (const T*)X, (const T*)dZ, (const long long*)order,
+                                                                                (const long long*)offsets, rows, (int)groups, (T*)dW,
+                                                                                (typename GpAcc<T>::type*)((char*)ws + positions_bytes(gp, split)), (long long*)ws);
+    OEQ_CUDA(cudaGetLastError());
+    return join<T>(gp, split, GP_TILE, rows, groups, offsets, dW, ws, st);
 }
 
 // ---- tensor cores
@@ -213,6 +215,46 @@ int tc_product(const GpProblem& gp, int64_t rows, int64_t groups, const void* X,
     oeq_grouped_tc<T, TRANS><<<ctas, GT_THREADS, smem, st>>>(gt, args);
     OEQ_CUDA(cudaGetLastError());
     return OEQ_OK;
+}
+
+// CTAs of the tiles of the weight gradient, one for each SM, dealt by the time that a range of rows takes.
+GpSplit tc_split(const GpProblem& gp, int64_t rows, int sms) {
+    GpSplit s{};
+    int tiles[GP_PATHS], ctas = 0;
+    double cost[GP_PATHS];
+    for (int p = 0; p < gp.n_paths; ++p) {
+        const GpTarget& to = gp.target[gp.path[p].dst];
+        tiles[p] = (gp.path[p].src_mul + GD_TILE - 1) / GD_TILE * ((to.mul + GD_TILE - 1) / GD_TILE);
+        cost[p] = to.d * (double)(std::min(GD_TILE, gp.path[p].src_mul) + std::min(GD_TILE, to.mul) + 64);
+        s.parts[p] = 1;
+        ctas += tiles[p];
+    }
+    for (;;) {
+        int most = -1;
+        for (int p = 0; p < gp.n_paths; ++p)
+            if (s.parts[p] < rows && (most < 0 || cost[p] / s.parts[p] > cost[most] / s.parts[most])) most = p;
+        if (most < 0 || ctas + tiles[most] > sms) break;
+        ++s.parts[most];
+        ctas += tiles[most];
+    }
+    for (int p = 0; p < gp.n_paths; ++p) s.first[p + 1] = s.first[p] + tiles[p] * s.parts[p];
+    return s;
+}
+
+template <class T>
+int tc_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* X, const void* dZ, const int64_t* order, const int64_t* offsets, void* dW, void* ws,
+               cudaStream_t st) {
+    int sms = 0;
+    if (int rc = sm_count(sms)) return rc;
+    GdProblem gd{gp, tc_split(gp, rows, sms), {}};
+    for (int p = 0; p < gp.n_paths; ++p) gd.extra[p] = 96 / gp.target[gp.path[p].dst].d;
+    const GdArgs args{X, dZ, (const long long*)order, (const long long*)offsets, dW, (float*)((char*)ws + positions_bytes(gp, gd.split)), (long long*)ws, rows, (int)groups,
+                      aligned(X, 16) && gp.src_dim * sizeof(T) % 16 == 0, aligned(dZ, 16) && gp.dst_dim * sizeof(T) % 16 == 0,
+                      aligned(dW, 16) && gp.w_numel * sizeof(T) % 16 == 0};
+    if (int rc = allow_smem(oeq_grouped_tc_dw<T>, GD_SMEM)) return rc;
+    oeq_grouped_tc_dw<T><<<gd.split.first[gp.n_paths], GD_THREADS, GD_SMEM, st>>>(gd, args);
+    OEQ_CUDA(cudaGetLastError());
+    return join<T>(gp, gd.split, GD_TILE, rows, groups, offsets, dW, ws, st);
 }
 
 int check_call(const oeq_grouped* h, int dtype, int64_t rows, int64_t groups) {
@@ -378,9 +420,12 @@ int oeq_grouped_backward_input(oeq_grouped* h, int dtype, int64_t rows, int64_t 
 
 size_t oeq_grouped_workspace_bytes(const oeq_grouped* h, int dtype, int64_t rows, int64_t groups) {
     int sms = 0;
-    if (!h || rows <= 0 || !known_dtype(dtype) || h->forward.n_paths == 0 || sm_count(sms)) return 0;
-    const GpSplit s = simt_split(h->weights, rows, sms);
-    return (size_t)s.first[h->weights.n_paths] * 2 * GP_TILE * GP_TILE * std::max<size_t>(4, elem_bytes(dtype));
+    if (!h || rows < 0 || !known_dtype(dtype) || h->weights.n_paths == 0 || sm_count(sms)) return 0;
+    const GpProblem& gp = h->weights;
+    const bool tc = dtype != OEQ_F64 && h->d_max <= GT_D_MAX;
+    const GpSplit s = tc ? tc_split(gp, rows, sms) : simt_split(gp, rows, sms);
+    const size_t tile = tc ? GD_TILE * GD_TILE * sizeof(float) : GP_TILE * GP_TILE * std::max<size_t>(4, elem_bytes(dtype));
+    return positions_bytes(gp, s) + (size_t)s.first[gp.n_paths] * 2 * tile;
 }
 
 int oeq_grouped_backward_weights(oeq_grouped* h, int dtype, int64_t rows, int64_t groups, const void* X, const void* dZ, const int64_t* order,
@@ -390,13 +435,17 @@ int oeq_grouped_backward_weights(oeq_grouped* h, int dtype, int64_t rows, int64_
     if (gp.w_numel == 0) return OEQ_OK;
     if (!offsets || !dW || (rows > 0 && (!X || !dZ))) return oeq_fail(OEQ_ERR_INVALID, "null pointer");
     const size_t want = oeq_grouped_workspace_bytes(h, dtype, rows, groups);
-    if (workspace_bytes < want || (want && !workspace)) return oeq_fail(OEQ_ERR_INVALID, "workspace too small");
+    if (want == 0 || workspace_bytes < want || !workspace) return oeq_fail(OEQ_ERR_INVALID, "workspace too small");
     const cudaStream_t st = (cudaStream_t)stream;
+    const bool tc = h->d_max <= GT_D_MAX;
     switch (dtype) {
         case OEQ_F64: return simt_weights<double>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st);
-        case OEQ_F32: return simt_weights<float>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st);
-        case OEQ_BF16: return simt_weights<__nv_bfloat16>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st);
-        default: return simt_weights<__half>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st);
+        case OEQ_F32: return tc ? tc_weights<float>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st)
+                                : simt_weights<float>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st);
+        case OEQ_BF16: return tc ? tc_weights<__nv_bfloat16>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st)
+                                 : simt_weights<__nv_bfloat16>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st);
+        default: return tc ? tc_weights<__half>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st)
+                           : simt_weights<__half>(gp, rows, groups, X, dZ, order, offsets, dW, workspace, st);
     }
 }
 
