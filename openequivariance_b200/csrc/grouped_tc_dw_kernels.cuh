@@ -11,6 +11,7 @@
 //   * one warp, in step, issues the MMAs: FP32 hi.hi and hi.lo as one, lo.hi into hi.lo's columns;
 //   * 8 warps add the accumulators to sums in registers at the end of a group and after CHAIN slots: an MMA's additions are cut off, not
 //     rounded, and the error grows with the length of a chain (relative, one chain of 750 slots: 1e-5).  The two accumulators alternate.
+//     These warps also prefetch the rows of the chain after next to L2.
 // A CTA has one tile of one path and a range of the sorted rows (gt_range); groups that go beyond the range leave a partial tile for
 // oeq_grouped_join.  Every wait is bounded.
 #pragma once
@@ -23,7 +24,7 @@ constexpr int GD_PW = 8, GD_EPI = 8, GD_THREADS = (GD_PW + GD_EPI + 1) * 32;
 constexpr int GD_SMEM = GD_RING * GD_SLOT + 1024;
 constexpr int ERR_GD_EMPTY = 91, ERR_GD_FULL = 92, ERR_GD_ACC_FULL = 93, ERR_GD_ACC_EMPTY = 94;
 
-template <class T> struct GdType { static constexpr int ROWS = 32, CHAIN = 256; };
+template <class T> struct GdType { static constexpr int ROWS = 32, CHAIN = 16; };
 template <> struct GdType<float> { static constexpr int ROWS = 8, CHAIN = 32; };
 __host__ __device__ constexpr int gd_sets(int d) { return d <= 5 ? 2 : 1; }
 // rows of a unit: whole slots, at most 56 registers of a lane on the way
@@ -87,14 +88,16 @@ template <class T> struct GdChain {
 };
 
 // ---------------------------------------------------------------------------- producers
+// The operands of a unit.  1 << lp lanes take a row, each V channels of X and the V channels of the same numbers of dZ.
+struct GdLane {
+    int lp, r0, ch;             // lanes of a row; the lane's first row, its channel
+    int x_left, z_left;         // channels from there on
+};
 template <class T, int D, bool FAST>
-__device__ __forceinline__ void gd_fill(const GdArgs& p, const GpProblem& gp, const GtWalk& walk, const T* x, const T* z, int mu, int mw, int n, unsigned char* ring,
-                                        int first, const GdBars& bars, int use, int member, bool& ok) {
-    const int lane = member & 31;
-    constexpr int V = GtType<T>::V, ROWS = GdType<T>::ROWS, THREADS = GD_PW * 32 / gd_sets(D), PASS = D == 1 ? 8 : (D == 3 ? 4 : (D <= 7 ? 2 : 1));
-    const int slots = (walk.rows + ROWS - 1) / ROWS, rows = slots * ROWS, across_x = (mu + V - 1) / V, across_z = (mw + V - 1) / V;
-    const int tasks_x = rows * across_x, tasks = tasks_x + rows * across_z;
-    const unsigned magic_x = (65536 + across_x - 1) / across_x, magic_z = (65536 + across_z - 1) / across_z;     // i / across for i <= 2048
+__device__ __forceinline__ void gd_fill(const GdArgs& p, const GpProblem& gp, const GtWalk& walk, const GdLane& l, const T* x, const T* z, int n, unsigned char* ring,
+                                        int first, const GdBars& bars, int use, bool& ok) {
+    constexpr int ROWS = GdType<T>::ROWS, THREADS = GD_PW * 32 / gd_sets(D), PASS = D == 1 ? 4 : (D == 3 ? 2 : 1);
+    const int slots = (walk.rows + ROWS - 1) / ROWS, rows = slots * ROWS, step = THREADS >> l.lp, blocks = (n + 63) / 64;
     bool waited = false;
     auto wait = [&]() {                         // until every slot of the unit is free again
         if (waited) return;
@@ -105,84 +108,78 @@ __device__ __forceinline__ void gd_fill(const GdArgs& p, const GpProblem& gp, co
         }
     };
 #pragma unroll 1
-    for (int i0 = member; i0 - lane < tasks; i0 += PASS * THREADS) {         // (in step: a warp waits as one)
-        uint4 v[PASS][D];
-        int at[PASS], r_of[PASS];               // channel (of dZ: behind 128), row
+    for (int q0 = 0; q0 < rows; q0 += PASS * step) {
+        uint4 v[PASS][D], w[PASS][D];
+        long long row[PASS];
 #pragma unroll
         for (int j = 0; j < PASS; ++j) {
-            const int i = min(i0 + j * THREADS, tasks - 1), is_z = i >= tasks_x, q = is_z ? i - tasks_x : i;
-            const int r = (int)((q * (is_z ? magic_z : magic_x)) >> 16), ch = (q - r * (is_z ? across_z : across_x)) * V;
-            const long long row = gp_row(p.order, walk.pos + min(r, walk.rows - 1));
-            const T* src = (is_z ? z + row * gp.dst_dim : x + row * gp.src_dim) + ch * D;
-            gt_read<T, D, FAST>(v[j], src, r < walk.rows ? (is_z ? mw : mu) - ch : 0);
-            at[j] = is_z ? ch + GD_TILE : ch;
-            r_of[j] = r;
+            const long long at = walk.pos + min(l.r0 + q0 + j * step, walk.rows - 1);
+            row[j] = p.order ? __ldg(p.order + at) : at;
+        }
+#pragma unroll
+        for (int j = 0; j < PASS; ++j) {
+            const bool in = l.r0 + q0 + j * step < walk.rows;           // rows behind the group's last: zeros
+            gt_read<T, D, FAST>(v[j], x + row[j] * gp.src_dim, in ? l.x_left : 0);
+            gt_read<T, D, FAST>(w[j], z + row[j] * gp.dst_dim, in ? l.z_left : 0);
         }
         wait();
         if (!ok) return;
 #pragma unroll
         for (int j = 0; j < PASS; ++j) {
-            if (i0 + j * THREADS >= tasks) continue;
-            const int is_z = at[j] >= GD_TILE, ch = is_z ? at[j] - GD_TILE : at[j], r = r_of[j] % ROWS;
-            const int place = is_z ? 8192 + gd_place<T>(ch, r, (n + 63) / 64) : gd_place<T>(ch, r, GD_TILE / 64);
-            const int lo = is_z ? 8192 + gd_place<T>(ch + n, r, 0) : place + 4096;
-            int slot = first + r_of[j] / ROWS * D;
+            const int q = l.r0 + q0 + j * step, r = q % ROWS;
+            if (q >= rows) continue;
+            const int x_at = gd_place<T>(l.ch, r, GD_TILE / 64), z_at = 8192 + gd_place<T>(l.ch, r, blocks), z_lo = 8192 + gd_place<T>(l.ch + n, r, 0);
+            int slot = first + q / ROWS * D;
             if (slot >= GD_RING) slot -= GD_RING;
 #pragma unroll
             for (int k = 0; k < D; ++k) {
-                const uint4 piece = gt_component<T, D>(v[j], k);
                 unsigned char* dst = ring + slot * GD_SLOT;
                 if (++slot == GD_RING) slot = 0;
+                const uint4 a = gt_component<T, D>(v[j], k), b = gt_component<T, D>(w[j], k);
                 if constexpr (GtType<T>::SPLIT) {
-                    float4 hi, lo4;
-                    gt_split(*reinterpret_cast<const float4*>(&piece), hi, lo4);
-                    *reinterpret_cast<float4*>(dst + place) = hi;
-                    *reinterpret_cast<float4*>(dst + lo) = lo4;
+                    float4 hi, lo;
+                    if (l.x_left > 0) {
+                        gt_split(*reinterpret_cast<const float4*>(&a), hi, lo);
+                        *reinterpret_cast<float4*>(dst + x_at) = hi;
+                        *reinterpret_cast<float4*>(dst + x_at + 4096) = lo;
+                    }
+                    if (l.z_left > 0) {
+                        gt_split(*reinterpret_cast<const float4*>(&b), hi, lo);
+                        *reinterpret_cast<float4*>(dst + z_at) = hi;
+                        *reinterpret_cast<float4*>(dst + z_lo) = lo;
+                    }
                 } else {
-                    *reinterpret_cast<uint4*>(dst + place) = piece;
+                    if (l.x_left > 0) *reinterpret_cast<uint4*>(dst + x_at) = a;
+                    if (l.z_left > 0) *reinterpret_cast<uint4*>(dst + z_at) = b;
                 }
             }
         }
     }
-    wait();                                     // (a warp without a task)
 }
 
 template <class T, int D>
 __device__ __forceinline__ void gd_produce(const GdArgs& p, const GpProblem& gp, const GpPath& path, const GpTarget& to, int u0, int w0, int mu, int mw, int n,
                                            unsigned char* ring, const GdBars& bars, GtWalk walk, int tid) {
-    constexpr int V = GtType<T>::V, ROWS = GdType<T>::ROWS, SETS = gd_sets(D), THREADS = GD_PW * 32 / SETS, UNIT = gd_unit<T>(D), LINE = 128 / sizeof(T);
+    constexpr int V = GtType<T>::V, ROWS = GdType<T>::ROWS, SETS = gd_sets(D), THREADS = GD_PW * 32 / SETS, UNIT = gd_unit<T>(D);
     const int set = tid / THREADS, member = tid % THREADS, lane = tid & 31;
-    const T *x = static_cast<const T*>(p.X) + path.src_off + u0 * D, *z = static_cast<const T*>(p.dZ) + to.off + w0 * D;
+    GdLane l;
+    l.lp = 0;
+    while ((V << l.lp) < max(mu, mw)) ++l.lp;
+    l.r0 = member >> l.lp;
+    l.ch = (member & ((1 << l.lp) - 1)) * V;
+    l.x_left = mu - l.ch;
+    l.z_left = mw - l.ch;
+    const T *x = static_cast<const T*>(p.X) + path.src_off + (u0 + l.ch) * D, *z = static_cast<const T*>(p.dZ) + to.off + (w0 + l.ch) * D;
     const bool fast = p.x_vec && p.z_vec && path.src_off % V == 0 && path.src_mul % V == 0 && to.off % V == 0 && to.mul % V == 0;
-    GtWalk ahead = walk;
-    int turn = 0, turn_ahead = 0, first = 0, use = 0;
+    int turn = 0, first = 0, use = 0;
     bool ok = true;
-    auto prefetch = [&]() {                     // the set's unit after next, to L2
-        while (ahead.more()) {
-            ahead.tile(UNIT);
-            const bool mine = turn_ahead == set;
-            if (mine) {
-                for (int r = member >> 3; r < ahead.rows; r += THREADS / 8) {
-                    const long long row = gp_row(p.order, ahead.pos + r);
-                    for (int i = (member & 7) * LINE; i < mu * D; i += 8 * LINE) gt_prefetch(x + row * gp.src_dim + i);
-                    for (int i = (member & 7) * LINE; i < mw * D; i += 8 * LINE) gt_prefetch(z + row * gp.dst_dim + i);
-                }
-            }
-            ahead.next(p.offsets, p.groups);
-            if (++turn_ahead == SETS) turn_ahead = 0;
-            if (mine) break;
-        }
-    };
-    prefetch();
-    prefetch();
     for (; walk.more(); walk.next(p.offsets, p.groups)) {
         walk.tile(UNIT);
         const int slots = (walk.rows + ROWS - 1) / ROWS * D;
         if (turn == set) {
-            prefetch();
-            if (fast) gd_fill<T, D, true>(p, gp, walk, x, z, mu, mw, n, ring, first, bars, use, member, ok);
-            else gd_fill<T, D, false>(p, gp, walk, x, z, mu, mw, n, ring, first, bars, use, member, ok);
-            if (!__all_sync(0xffffffffu, ok)) return;
+            if (fast) gd_fill<T, D, true>(p, gp, walk, l, x, z, n, ring, first, bars, use, ok);
+            else gd_fill<T, D, false>(p, gp, walk, l, x, z, n, ring, first, bars, use, ok);
+            if (!ok) return;
             fence_async_smem();
             __syncwarp();
             if (lane < slots) mbar_arrive(bars.full + (first + lane < GD_RING ? first + lane : first + lane - GD_RING));
@@ -257,26 +254,47 @@ __device__ __forceinline__ void gd_sum(const GdArgs& p, const GpProblem& gp, con
     float sum[COLS];
 #pragma unroll
     for (int j = 0; j < COLS; ++j) sum[j] = 0.f;
+    // rows of the chain after next, to L2
+    constexpr int LINE = 128 / sizeof(T), THREADS = GD_EPI * 32;
+    GtWalk ahead = walk;
+    GdChain<T> chain_ahead;
+    auto prefetch = [&]() {
+        for (bool more = true; more && ahead.more(); ahead.next(p.offsets, p.groups)) {
+            ahead.tile(unit);
+            chain_ahead.unit(ahead, d);
+            more = !chain_ahead.ends;
+            for (int r = (warp * 32 + lane) >> 3; r < ahead.rows; r += THREADS / 8) {
+                const long long row = gp_row(p.order, ahead.pos + r);
+                const T *x = static_cast<const T*>(p.X) + row * gp.src_dim + path.src_off + u0 * d, *z = static_cast<const T*>(p.dZ) + row * gp.dst_dim + to.off + w0 * d;
+                for (int i = (lane & 7) * LINE; i < mu * d; i += 8 * LINE) gt_prefetch(x + i);
+                for (int i = (lane & 7) * LINE; i < mw * d; i += 8 * LINE) gt_prefetch(z + i);
+            }
+        }
+    };
+    prefetch();
+    prefetch();
     int accs = 0;
     for (; walk.more(); walk.next(p.offsets, p.groups)) {
         walk.tile(unit);
         chain.unit(walk, d);
         if (!chain.ends) continue;
+        prefetch();
         const int buf = accs & 1;
         if (!warp_wait(true, bars.acc_full + buf, (unsigned)(accs / 2) & 1, &gt_status, ERR_GD_ACC_FULL)) return;
         tc_fence_after();
 #pragma unroll
         for (int j = 0; j < COLS; j += 16) {
             if (c0 + j < n) {
-                unsigned v[16], w[16];
+                unsigned v[16];
                 tc_load16(at + (unsigned)(buf * 256 + j), v);
-                if constexpr (GtType<T>::SPLIT) tc_load16(at + (unsigned)(buf * 256 + n + j), w);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float s = __uint_as_float(v[i]);
-                    if constexpr (GtType<T>::SPLIT) s += __uint_as_float(w[i]);
-                    sum[j + i] += s;
+                for (int i = 0; i < 16; ++i) sum[j + i] += __uint_as_float(v[i]);
+                if constexpr (GtType<T>::SPLIT) {
+                    tc_load16(at + (unsigned)(buf * 256 + n + j), v);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum[j + i] += __uint_as_float(v[i]);
                 }
             }
         }
