@@ -6,10 +6,10 @@
 // M = 128 input channels u, N = up to 128 output channels w of one path, and the sum runs over rows and components.  Both operands have their
 // channels along memory, so both are "MN-major": a lane reads the 16 d bytes of V channels of a row and writes d pieces, one into
 // the slot of each component.  A slot of the ring has one component of GdType::ROWS sorted rows of one group, X and dZ, 16 KB.
-//   * 8 producer warps: two sets of four take units of rows in turn (seven and more components: one set, as the slots of two units have
-//     to fit the ring);
+//   * 16 producer warps: two sets of eight take units of rows in turn, a lane the same channels of X and dZ; from five components on one
+//     set, half of it for X and half for dZ (the slots of the units under way have to fit the ring);
 //   * one warp, in step, issues the MMAs: FP32 hi.hi and hi.lo as one, lo.hi into hi.lo's columns;
-//   * 8 warps add the accumulators to sums in registers at the end of a group and after CHAIN slots: an MMA's additions are cut off, not
+//   * 8 warps add the accumulators to sums in shared memory at the end of a group and after CHAIN slots: an MMA's additions are cut off, not
 //     rounded, and the error grows with the length of a chain (relative, one chain of 750 slots: 1e-5).  The two accumulators alternate.
 //     These warps also prefetch the rows of the chain after next to L2.
 // A CTA has one tile of one path and a range of the sorted rows (gt_range); groups that go beyond the range leave a partial tile for
@@ -19,16 +19,18 @@
 
 namespace oeq {
 
-constexpr int GD_TILE = 128, GD_RING = 12, GD_SLOT = 16384;
-constexpr int GD_PW = 8, GD_EPI = 8, GD_THREADS = (GD_PW + GD_EPI + 1) * 32;
-constexpr int GD_SMEM = GD_RING * GD_SLOT + 1024;
+constexpr int GD_TILE = 128, GD_RING = 8, GD_SLOT = 16384, GD_SUMS = GD_TILE * GD_TILE * 4;
+constexpr int GD_PW = 16, GD_EPI = 8, GD_THREADS = (GD_PW + GD_EPI + 1) * 32;
+constexpr int GD_SMEM = GD_RING * GD_SLOT + GD_SUMS + 1024;
 constexpr int ERR_GD_EMPTY = 91, ERR_GD_FULL = 92, ERR_GD_ACC_FULL = 93, ERR_GD_ACC_EMPTY = 94;
 
 template <class T> struct GdType { static constexpr int ROWS = 32, CHAIN = 16; };
 template <> struct GdType<float> { static constexpr int ROWS = 8, CHAIN = 32; };
-__host__ __device__ constexpr int gd_sets(int d) { return d <= 5 ? 2 : 1; }
-// rows of a unit: whole slots, at most 56 registers of a lane on the way
-template <class T> __host__ __device__ constexpr int gd_unit(int d) { return sizeof(T) == 4 ? (d == 1 ? 32 : (d == 3 ? 16 : 8)) : (d == 1 ? 64 : 32); }
+// Sets of producers.  A warp waits for the slots of its units alone, so it can tell the phases of a slot apart as long as the units under
+// way, one of each set, fit the ring.
+__host__ __device__ constexpr int gd_sets(int d) { return d <= 3 ? 2 : 1; }
+// rows of a unit: whole slots
+template <class T> __host__ __device__ constexpr int gd_unit(int d) { return sizeof(T) == 4 ? (d == 1 ? 32 : 8) : (d == 1 ? 64 : 32); }
 
 struct GdProblem {
     GpProblem gp;               // paths in the order of their weights
@@ -43,7 +45,7 @@ struct GdArgs {
     long long* lo;              // [CTAs] first position of each CTA's range
     long long rows;
     int groups;
-    int x_vec, z_vec, w_vec;    // rows of X and dZ, weights of dW in 16-byte pieces
+    int w_vec;                  // weights of dW in 16-byte pieces
 };
 
 // byte offset of V channels from ch of row r (of the slot's) in an operand with `blocks` blocks of channels
@@ -88,15 +90,33 @@ template <class T> struct GdChain {
 };
 
 // ---------------------------------------------------------------------------- producers
-// The operands of a unit.  1 << lp lanes take a row, each V channels of X and the V channels of the same numbers of dZ.
+// The operands of a unit: 1 << lp lanes take a row, V channels each.
 struct GdLane {
     int lp, r0, ch;             // lanes of a row; the lane's first row, its channel
-    int x_left, z_left;         // channels from there on
+    int x_left, z_left;         // channels of X and dZ from there on (0: another lane's)
 };
+template <class T, int D>
+__device__ __forceinline__ void gd_put(const uint4 (&v)[D], unsigned char* ring, int slot, int at, int at_lo) {
+#pragma unroll
+    for (int k = 0; k < D; ++k) {
+        unsigned char* dst = ring + slot * GD_SLOT;
+        if (++slot == GD_RING) slot = 0;
+        const uint4 a = gt_component<T, D>(v, k);
+        if constexpr (GtType<T>::SPLIT) {
+            float4 hi, lo;
+            gt_split(*reinterpret_cast<const float4*>(&a), hi, lo);
+            *reinterpret_cast<float4*>(dst + at) = hi;
+            *reinterpret_cast<float4*>(dst + at_lo) = lo;
+        } else {
+            *reinterpret_cast<uint4*>(dst + at) = a;
+        }
+    }
+}
 template <class T, int D, bool FAST>
 __device__ __forceinline__ void gd_fill(const GdArgs& p, const GpProblem& gp, const GtWalk& walk, const GdLane& l, const T* x, const T* z, int n, unsigned char* ring,
                                         int first, const GdBars& bars, int use, bool& ok) {
-    constexpr int ROWS = GdType<T>::ROWS, THREADS = GD_PW * 32 / gd_sets(D), PASS = D == 1 ? 4 : (D == 3 ? 2 : 1);
+    constexpr bool BOTH = gd_sets(D) == 2;      // a lane reads both operands, else x is the lane's operand
+    constexpr int ROWS = GdType<T>::ROWS, THREADS = 256, PASS = D == 1 ? 4 : 1;
     const int slots = (walk.rows + ROWS - 1) / ROWS, rows = slots * ROWS, step = THREADS >> l.lp, blocks = (n + 63) / 64;
     bool waited = false;
     auto wait = [&]() {                         // until every slot of the unit is free again
@@ -109,18 +129,23 @@ __device__ __forceinline__ void gd_fill(const GdArgs& p, const GpProblem& gp, co
     };
 #pragma unroll 1
     for (int q0 = 0; q0 < rows; q0 += PASS * step) {
-        uint4 v[PASS][D], w[PASS][D];
-        long long row[PASS];
+        uint4 v[PASS][D], w[BOTH ? PASS : 1][D];
+        int row[PASS];
 #pragma unroll
         for (int j = 0; j < PASS; ++j) {
-            const long long at = walk.pos + min(l.r0 + q0 + j * step, walk.rows - 1);
-            row[j] = p.order ? __ldg(p.order + at) : at;
+            const int at = walk.pos + min(l.r0 + q0 + j * step, walk.rows - 1);
+            row[j] = p.order ? (int)__ldg(p.order + at) : at;
         }
 #pragma unroll
         for (int j = 0; j < PASS; ++j) {
             const bool in = l.r0 + q0 + j * step < walk.rows;           // rows behind the group's last: zeros
-            gt_read<T, D, FAST>(v[j], x + row[j] * gp.src_dim, in ? l.x_left : 0);
-            gt_read<T, D, FAST>(w[j], z + row[j] * gp.dst_dim, in ? l.z_left : 0);
+            if constexpr (BOTH) {
+                gt_read<T, D, FAST>(v[j], x + (long long)row[j] * gp.src_dim, in ? l.x_left : 0);
+                gt_read<T, D, FAST>(w[j], z + (long long)row[j] * gp.dst_dim, in ? l.z_left : 0);
+            } else {
+                const bool is_x = l.x_left > 0;
+                gt_read<T, D, FAST>(v[j], is_x ? x + (long long)row[j] * gp.src_dim : z + (long long)row[j] * gp.dst_dim, in ? (is_x ? l.x_left : l.z_left) : 0);
+            }
         }
         wait();
         if (!ok) return;
@@ -128,63 +153,43 @@ __device__ __forceinline__ void gd_fill(const GdArgs& p, const GpProblem& gp, co
         for (int j = 0; j < PASS; ++j) {
             const int q = l.r0 + q0 + j * step, r = q % ROWS;
             if (q >= rows) continue;
-            const int x_at = gd_place<T>(l.ch, r, GD_TILE / 64), z_at = 8192 + gd_place<T>(l.ch, r, blocks), z_lo = 8192 + gd_place<T>(l.ch + n, r, 0);
             int slot = first + q / ROWS * D;
             if (slot >= GD_RING) slot -= GD_RING;
-#pragma unroll
-            for (int k = 0; k < D; ++k) {
-                unsigned char* dst = ring + slot * GD_SLOT;
-                if (++slot == GD_RING) slot = 0;
-                const uint4 a = gt_component<T, D>(v[j], k), b = gt_component<T, D>(w[j], k);
-                if constexpr (GtType<T>::SPLIT) {
-                    float4 hi, lo;
-                    if (l.x_left > 0) {
-                        gt_split(*reinterpret_cast<const float4*>(&a), hi, lo);
-                        *reinterpret_cast<float4*>(dst + x_at) = hi;
-                        *reinterpret_cast<float4*>(dst + x_at + 4096) = lo;
-                    }
-                    if (l.z_left > 0) {
-                        gt_split(*reinterpret_cast<const float4*>(&b), hi, lo);
-                        *reinterpret_cast<float4*>(dst + z_at) = hi;
-                        *reinterpret_cast<float4*>(dst + z_lo) = lo;
-                    }
-                } else {
-                    if (l.x_left > 0) *reinterpret_cast<uint4*>(dst + x_at) = a;
-                    if (l.z_left > 0) *reinterpret_cast<uint4*>(dst + z_at) = b;
-                }
+            if (l.x_left > 0) {
+                const int at = gd_place<T>(l.ch, r, GD_TILE / 64);
+                gd_put<T, D>(v[j], ring, slot, at, at + 4096);
             }
+            if (l.z_left > 0) gd_put<T, D>(BOTH ? w[j] : v[j], ring, slot, 8192 + gd_place<T>(l.ch, r, blocks), 8192 + gd_place<T>(l.ch + n, r, 0));
         }
     }
 }
 
-template <class T, int D>
+template <class T, bool FAST, int D>
 __device__ __forceinline__ void gd_produce(const GdArgs& p, const GpProblem& gp, const GpPath& path, const GpTarget& to, int u0, int w0, int mu, int mw, int n,
                                            unsigned char* ring, const GdBars& bars, GtWalk walk, int tid) {
-    constexpr int V = GtType<T>::V, ROWS = GdType<T>::ROWS, SETS = gd_sets(D), THREADS = GD_PW * 32 / SETS, UNIT = gd_unit<T>(D);
-    const int set = tid / THREADS, member = tid % THREADS, lane = tid & 31;
+    constexpr int V = GtType<T>::V, ROWS = GdType<T>::ROWS, SETS = gd_sets(D), UNIT = gd_unit<T>(D);
+    const int half = tid >> 8, member = tid & 255, lane = tid & 31;
     GdLane l;
     l.lp = 0;
     while ((V << l.lp) < max(mu, mw)) ++l.lp;
     l.r0 = member >> l.lp;
     l.ch = (member & ((1 << l.lp) - 1)) * V;
-    l.x_left = mu - l.ch;
-    l.z_left = mw - l.ch;
+    l.x_left = SETS == 2 || half == 0 ? mu - l.ch : 0;
+    l.z_left = SETS == 2 || half == 1 ? mw - l.ch : 0;
     const T *x = static_cast<const T*>(p.X) + path.src_off + (u0 + l.ch) * D, *z = static_cast<const T*>(p.dZ) + to.off + (w0 + l.ch) * D;
-    const bool fast = p.x_vec && p.z_vec && path.src_off % V == 0 && path.src_mul % V == 0 && to.off % V == 0 && to.mul % V == 0;
     int turn = 0, first = 0, use = 0;
     bool ok = true;
     for (; walk.more(); walk.next(p.offsets, p.groups)) {
         walk.tile(UNIT);
         const int slots = (walk.rows + ROWS - 1) / ROWS * D;
-        if (turn == set) {
-            if (fast) gd_fill<T, D, true>(p, gp, walk, l, x, z, n, ring, first, bars, use, ok);
-            else gd_fill<T, D, false>(p, gp, walk, l, x, z, n, ring, first, bars, use, ok);
+        if (SETS == 1 || turn == half) {
+            gd_fill<T, D, FAST>(p, gp, walk, l, x, z, n, ring, first, bars, use, ok);
             if (!ok) return;
             fence_async_smem();
             __syncwarp();
             if (lane < slots) mbar_arrive(bars.full + (first + lane < GD_RING ? first + lane : first + lane - GD_RING));
         }
-        if (++turn == SETS) turn = 0;
+        turn ^= 1;
         first += slots;
         if (first >= GD_RING) {
             first -= GD_RING;
@@ -242,18 +247,18 @@ __device__ __forceinline__ void gd_multiply(const GdArgs& p, int d, int unit, in
 }
 
 // ---------------------------------------------------------------------------- sums
-// A lane has one input channel, a warp's half of the warps 64 output channels.
+// A lane has one input channel and 64 output channels; sums [output channel][input channel].
 template <class T>
 __device__ __forceinline__ void gd_sum(const GdArgs& p, const GpProblem& gp, const GpPath& path, const GpTarget& to, int d, int unit, int u0, int w0, int mu, int mw, int n,
-                                       const GdBars& bars, GtWalk walk, long long lo, long long hi, unsigned tmem, int warp, int lane) {
+                                       const GdBars& bars, float* sums, GtWalk walk, unsigned tmem, int warp, int lane) {
+    const int lo = walk.pos, hi = walk.hi;
     constexpr int COLS = GD_TILE / 2;
     const int quarter = warp & 3, c0 = (warp >> 2) * COLS, u = quarter * 32 + lane;
     const unsigned at = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)c0;
     const float scale = (float)to.scale;
     GdChain<T> chain;
-    float sum[COLS];
-#pragma unroll
-    for (int j = 0; j < COLS; ++j) sum[j] = 0.f;
+    float* sum = sums + c0 * GD_TILE + u;
+    bool begun = false;         // the group's sums hold something
     // rows of the chain after next, to L2
     constexpr int LINE = 128 / sizeof(T), THREADS = GD_EPI * 32;
     GtWalk ahead = walk;
@@ -282,68 +287,51 @@ __device__ __forceinline__ void gd_sum(const GdArgs& p, const GpProblem& gp, con
         const int buf = accs & 1;
         if (!warp_wait(true, bars.acc_full + buf, (unsigned)(accs / 2) & 1, &gt_status, ERR_GD_ACC_FULL)) return;
         tc_fence_after();
+#pragma unroll 1
+        for (int j = 0; j < COLS && c0 + j < n; j += 16) {
+            unsigned v[16], w[GtType<T>::SPLIT ? 16 : 1];
+            tc_load16(at + (unsigned)(buf * 256 + j), v);
+            if constexpr (GtType<T>::SPLIT) tc_load16(at + (unsigned)(buf * 256 + n + j), w);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int j = 0; j < COLS; j += 16) {
-            if (c0 + j < n) {
-                unsigned v[16];
-                tc_load16(at + (unsigned)(buf * 256 + j), v);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                for (int i = 0; i < 16; ++i) sum[j + i] += __uint_as_float(v[i]);
-                if constexpr (GtType<T>::SPLIT) {
-                    tc_load16(at + (unsigned)(buf * 256 + n + j), v);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sum[j + i] += __uint_as_float(v[i]);
-                }
+            for (int i = 0; i < 16; ++i) {
+                float s = __uint_as_float(v[i]);
+                if constexpr (GtType<T>::SPLIT) s += __uint_as_float(w[i]);
+                sum[(j + i) * GD_TILE] = begun ? sum[(j + i) * GD_TILE] + s : s;
             }
         }
+        begun = true;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.acc_empty + buf);
         ++accs;
         if (!chain.piece_ends) continue;
-        const long long begin = __ldg(p.offsets + walk.g), end = __ldg(p.offsets + walk.g + 1);
+        const int begin = (int)__ldg(p.offsets + walk.g), end = GtWalk::end_of(p.offsets, walk.g);
+        begun = false;
+        if (u >= mu) continue;
         if (begin >= lo && end <= hi) {
-            if (u < mu) {
-                T* out = static_cast<T*>(p.dW) + (long long)walk.g * gp.w_numel + path.w_off + (long long)(u0 + u) * path.w_ld + w0 + c0;
-                if constexpr (sizeof(T) == 4) {
-                    if (p.w_vec && ((path.w_off | path.w_ld) & 3) == 0) {
-#pragma unroll
-                        for (int j = 0; j < COLS; j += 4)
-                            if (c0 + j < mw)
-                                *reinterpret_cast<float4*>(out + j) = make_float4(sum[j] * scale, sum[j + 1] * scale, sum[j + 2] * scale, sum[j + 3] * scale);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < COLS; ++j)
-                            if (c0 + j < mw) out[j] = sum[j] * scale;
-                    }
-                } else {
-                    if (p.w_vec && ((path.w_off | path.w_ld) & 7) == 0) {
-#pragma unroll
-                        for (int j = 0; j < COLS; j += 8)
-                            if (c0 + j < mw)
-                                *reinterpret_cast<uint4*>(out + j) = make_uint4(GtPair<T>::of(sum[j] * scale, sum[j + 1] * scale), GtPair<T>::of(sum[j + 2] * scale, sum[j + 3] * scale),
-                                                                                GtPair<T>::of(sum[j + 4] * scale, sum[j + 5] * scale), GtPair<T>::of(sum[j + 6] * scale, sum[j + 7] * scale));
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < COLS; ++j)
-                            if (c0 + j < mw) gp_store(out + j, sum[j] * scale);
-                    }
+            T* out = static_cast<T*>(p.dW) + (long long)walk.g * gp.w_numel + path.w_off + (long long)(u0 + u) * path.w_ld + w0 + c0;
+            auto value = [&](int j) { return sum[j * GD_TILE] * scale; };
+            if (p.w_vec && (path.w_off | path.w_ld) % GtType<T>::V == 0) {
+#pragma unroll 2
+                for (int j = 0; j < COLS && c0 + j < mw; j += GtType<T>::V) {
+                    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out + j) = make_float4(value(j), value(j + 1), value(j + 2), value(j + 3));
+                    else *reinterpret_cast<uint4*>(out + j) = make_uint4(GtPair<T>::of(value(j), value(j + 1)), GtPair<T>::of(value(j + 2), value(j + 3)),
+                                                                         GtPair<T>::of(value(j + 4), value(j + 5)), GtPair<T>::of(value(j + 6), value(j + 7)));
                 }
+            } else {
+                for (int j = 0; j < COLS && c0 + j < mw; ++j) gp_store(out + j, value(j));
             }
-        } else if (u < mu) {
+        } else {
             float* out = p.partial + ((long long)blockIdx.x * 2 + (begin < lo ? 0 : 1)) * (GD_TILE * GD_TILE) + u * GD_TILE + c0;
-#pragma unroll
-            for (int j = 0; j < COLS; j += 4)
-                if (c0 + j < mw) *reinterpret_cast<float4*>(out + j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
+#pragma unroll 4
+            for (int j = 0; j < COLS && c0 + j < mw; j += 4)            // (whole pieces: the tile has room)
+                *reinterpret_cast<float4*>(out + j) = make_float4(sum[j * GD_TILE], sum[(j + 1) * GD_TILE], sum[(j + 2) * GD_TILE], sum[(j + 3) * GD_TILE]);
         }
-#pragma unroll
-        for (int j = 0; j < COLS; ++j) sum[j] = 0.f;
     }
 }
 
-template <class T>
+template <class T, bool FAST>
 __global__ void __launch_bounds__(GD_THREADS, 1) oeq_grouped_tc_dw(const __grid_constant__ GdProblem gd, const GdArgs p) {
     extern __shared__ __align__(1024) unsigned char gt_smem[];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -354,7 +342,8 @@ __global__ void __launch_bounds__(GD_THREADS, 1) oeq_grouped_tc_dw(const __grid_
     const int parts = gd.split.parts[path_no], local = (int)blockIdx.x - gd.split.first[path_no], tile = local / parts, part = local % parts, d = to.d;
     const int w_tiles = (to.mul + GD_TILE - 1) / GD_TILE, u0 = tile / w_tiles * GD_TILE, w0 = tile % w_tiles * GD_TILE;
     const int mu = min(GD_TILE, path.src_mul - u0), mw = min(GD_TILE, to.mul - w0), n = (mw + 15) / 16 * 16;
-    unsigned char* control = gt_smem + GD_RING * GD_SLOT;
+    float* sums = reinterpret_cast<float*>(gt_smem + GD_RING * GD_SLOT);
+    unsigned char* control = gt_smem + GD_RING * GD_SLOT + GD_SUMS;
     const GdBars bars(control);
     GtRange& range = *reinterpret_cast<GtRange*>(control + 512);
     constexpr int MMA_WARP = GD_PW + GD_EPI;
@@ -379,17 +368,16 @@ __global__ void __launch_bounds__(GD_THREADS, 1) oeq_grouped_tc_dw(const __grid_
     const unsigned tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile unsigned*>(bars.tmem), 0);
     const long long lo = range.lo, hi = range.hi;
     if (tid == 0) p.lo[blockIdx.x] = lo;
-    const GtWalk walk(p.offsets, range.g, lo, hi);
+    const GtWalk walk(p.offsets, range.g, (int)lo, (int)hi);
     if (warp == MMA_WARP) {
         gd_multiply<T>(p, d, gd_unit<T>(d), n, gt_smem, bars, walk, tmem, elect_lane());
     } else if (warp >= GD_PW) {
-        gd_sum<T>(p, gd.gp, path, to, d, gd_unit<T>(d), u0, w0, mu, mw, n, bars, walk, lo, hi, tmem, warp - GD_PW, lane);
+        gd_sum<T>(p, gd.gp, path, to, d, gd_unit<T>(d), u0, w0, mu, mw, n, bars, sums, walk, tmem, warp - GD_PW, lane);
     } else {
-        if (d == 1) gd_produce<T, 1>(p, gd.gp, path, to, u0, w0, mu, mw, n, gt_smem, bars, walk, tid);
-        else if (d == 3) gd_produce<T, 3>(p, gd.gp, path, to, u0, w0, mu, mw, n, gt_smem, bars, walk, tid);
-        else if (d == 5) gd_produce<T, 5>(p, gd.gp, path, to, u0, w0, mu, mw, n, gt_smem, bars, walk, tid);
-        else if (d == 7) gd_produce<T, 7>(p, gd.gp, path, to, u0, w0, mu, mw, n, gt_smem, bars, walk, tid);
-        else gd_produce<T, 9>(p, gd.gp, path, to, u0, w0, mu, mw, n, gt_smem, bars, walk, tid);
+        if (d == 1) gd_produce<T, FAST, 1>(p, gd.gp, path, to, u0, w0, mu, mw, n, gt_smem, bars, walk, tid);
+        else if (d == 3) gd_produce<T, FAST, 3>(p, gd.gp, path, to, u0, w0, mu, mw, n, gt_smem, bars, walk, tid);
+        else if (d == 5) gd_produce<T, FAST, 5>(p, gd.gp, path, to, u0, w0, mu, mw, n, gt_smem, bars, walk, tid);
+        else gd_produce<T, FAST, 7>(p, gd.gp, path, to, u0, w0, mu, mw, n, gt_smem, bars, walk, tid);
     }
     tc_fence_before();
     __syncthreads();

@@ -6,10 +6,10 @@
 // As a matrix product: M = (row, component) pairs of sorted rows of one group, N = channels of one output block, K = channels of
 // the input blocks with its irrep.  A CTA has one output block (or a tile of its channels) and one range of the sorted rows, the
 // CTAs being dealt to the output blocks by cost, so a CTA meets few groups and keeps a group's weights in shared memory.
-//   * 8 producer warps: a lane reads the 16 d bytes of V = 4 (16-bit types: 8) channels of a row, [channel][component], and writes
+//   * 16 producer warps: a lane reads the 16 d bytes of V = 4 (16-bit types: 8) channels of a row, [channel][component], and writes
 //     d pieces of 16 bytes, one per (row, component), K-major with the 128-byte swizzle.  The transposition that the layout of irreps
 //     asks for costs no extra pass, rows are gathered in sorted order, and FP32 values are split into TF32 hi and lo on the way.
-//     Two sets of four warps take the chunks of K in turn: each has its chunk on the way in registers before it waits for a stage.
+//     Two sets of eight warps take the chunks of K in turn: each has its chunk on the way in registers before it waits for a stage.
 //     Weights have their output channels along memory: "MN-major" tiles for Z, K-major for dX; neither is transposed.
 //   * one warp, in step, issues the MMAs.  FP32: hi.hi and hi.lo as one MMA over the weights' hi channels followed by lo, lo.hi
 //     into hi.lo's columns: the large and the small products have accumulators of their own.
@@ -23,8 +23,8 @@
 
 namespace oeq {
 
-constexpr int GT_D_MAX = 9;
-constexpr int GT_SETS = 2, GT_SET = 4, GT_PW = GT_SETS * GT_SET, GT_EPI_GROUPS = 2, GT_EPI = 4 * GT_EPI_GROUPS, GT_THREADS = (GT_PW + GT_EPI + 1) * 32;
+constexpr int GT_D_MAX = 7;
+constexpr int GT_SETS = 2, GT_SET = 8, GT_PW = GT_SETS * GT_SET, GT_EPI_GROUPS = 2, GT_EPI = 4 * GT_EPI_GROUPS, GT_THREADS = (GT_PW + GT_EPI + 1) * 32;
 constexpr int GT_STAGES = 6;                    // most stages of A
 constexpr int GT_STAGING = 33 * 128 * 4;        // 32 channels of a tile's pairs, for each epilogue group
 constexpr int GT_CONTROL = 1536;                // barriers, rows of the tiles that drain, the CTA's range
@@ -45,8 +45,7 @@ struct GtProblem {
     GtTarget target[GP_BLOCKS];
 };
 
-// Rows of a tile.  Seven components: 16 rows (112 of 128 pairs) are one piece for every lane of a set, 18 would be two.
-__host__ __device__ constexpr int gt_tile_rows(int d) { return d == 7 ? 16 : 128 / d; }
+__host__ __device__ constexpr int gt_tile_rows(int d) { return 128 / d; }        // rows of a tile
 
 template <class T> struct GtType {              // 16-bit
     static constexpr int V = 8, KC = 64, KSTEP = 16, A_BYTES = 16384, N_MAX = 256;
@@ -144,21 +143,22 @@ __device__ __forceinline__ uint4 gt_component(const uint4 (&v)[D], int k) {
 
 // ---- a CTA's tiles: up to 128 / d sorted rows of one group
 struct GtWalk {
-    long long pos, hi, end;     // next position, end of the range, end of the group within it
+    int pos, hi, end;           // next position, end of the range, end of the group within it
     int g, rows;
-    __device__ GtWalk(const long long* offsets, int g_, long long lo, long long hi_) : pos(lo), hi(hi_), end(0), g(g_), rows(0) {
-        if (lo < hi) end = min(__ldg(offsets + g + 1), hi);
+    __device__ static int end_of(const long long* offsets, int g) { return (int)__ldg(offsets + g + 1); }
+    __device__ GtWalk(const long long* offsets, int g_, int lo, int hi_) : pos(lo), hi(hi_), end(0), g(g_), rows(0) {
+        if (lo < hi) end = min(end_of(offsets, g), hi);
     }
     __device__ bool more() const { return pos < hi; }
-    __device__ void tile(int most) { rows = (int)min((long long)most, end - pos); }
+    __device__ void tile(int most) { rows = min(most, end - pos); }
     __device__ void next(const long long* offsets, int groups) {
         pos += rows;
         if (pos >= end && pos < hi) {
             ++g;
-            end = __ldg(offsets + g + 1);
+            end = end_of(offsets, g);
             if (end <= pos) {                   // groups without rows between
                 g = gp_group(offsets, groups, pos);
-                end = __ldg(offsets + g + 1);
+                end = end_of(offsets, g);
             }
             end = min(end, hi);
         }
@@ -223,7 +223,7 @@ struct GtArgs {
     void* Z;
     long long rows;
     int groups;
-    int x_vec, w_vec, z_pair;   // 16-byte pieces of X and W, 4-byte pairs of 16-bit Z are aligned
+    int z_pair;                 // 4-byte pairs of 16-bit Z are aligned
 };
 struct GtBars {
     unsigned long long *full, *empty, *acc_full, *acc_empty;
@@ -272,7 +272,7 @@ __device__ __forceinline__ void gt_fill_b(unsigned char* dst, const T* __restric
     }
 }
 
-template <class T, bool TRANS, int D>
+template <class T, bool TRANS, bool FAST, int D>
 __device__ __forceinline__ void gt_produce(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, unsigned char* a_base,
                                            unsigned char* b_base, const GtBars& bars, GtWalk walk, int tid) {
     constexpr int V = GtType<T>::V, KC = GtType<T>::KC, KSTEP = GtType<T>::KSTEP, TILE_ROWS = gt_tile_rows(D), THREADS = GT_SET * 32;
@@ -290,24 +290,18 @@ __device__ __forceinline__ void gt_produce(const GtProblem& gt, const GtArgs& p,
         int row[PIECES];                        // (past the tile's rows: the last one again)
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const long long at = walk.pos + min((member + i * THREADS) >> 3, walk.rows - 1);
-            row[i] = p.order ? (int)__ldg(p.order + at) : (int)at;
+            const int at = walk.pos + min((member + i * THREADS) >> 3, walk.rows - 1);
+            row[i] = p.order ? (int)__ldg(p.order + at) : at;
         }
         for (int path_no = to.path_begin; path_no < to.path_end; ++path_no) {
             const GpPath& path = gt.gp.path[path_no];
-            const bool vec_x = p.x_vec && path.src_off % V == 0 && path.src_mul % V == 0, vec_w = p.w_vec && path.w_off % V == 0 && path.w_ld % V == 0;
             for (int u0 = 0; u0 < path.src_mul; u0 += KC) {
                 if (turn == set) {
                     const int left = path.src_mul - u0, k_fill = left >= KC ? KC : (left + KSTEP - 1) / KSTEP * KSTEP;
                     uint4 v[PIECES][D];
 const T* x = static_cast<const T*>(p.X) + path.src_off + (u0 + V * c) * D;
-                    if (vec_x) {
 #pragma unroll
-                        for (int i = 0; i < PIECES; ++i) gt_read<T, D, true>(v[i], x + (long long)row[i] * gt.gp.src_dim, left - V * c);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < PIECES; ++i) gt_read<T, D, false>(v[i], x + (long long)row[i] * gt.gp.src_dim, left - V * c);
-                    }
+                    for (int i = 0; i < PIECES; ++i) gt_read<T, D, FAST>(v[i], x + (long long)row[i] * gt.gp.src_dim, left - V * c);
                     bool ok = true;
                     if (use > 0) ok = warp_wait(ok, bars.empty + stage, (unsigned)(use - 1) & 1, &gt_status, ERR_GT_EMPTY);
                     if (load_b) {
@@ -338,9 +332,7 @@ const T* x = static_cast<const T*>(p.X) + path.src_off + (u0 + V * c) * D;
                     }
                     if (load_b) {
                         const T* w = w_group + path.w_off + (TRANS ? (long long)n0 * path.w_ld + u0 : (long long)u0 * path.w_ld + n0);
-                        unsigned char* b = b_base + slot * GtType<T>::b_bytes(n);
-                        if (vec_w) gt_fill_b<T, TRANS, true>(b, w, path.w_ld, n, to.mul - n0, left, k_fill, member);
-                        else gt_fill_b<T, TRANS, false>(b, w, path.w_ld, n, to.mul - n0, left, k_fill, member);
+                        gt_fill_b<T, TRANS, FAST>(b_base + slot * GtType<T>::b_bytes(n), w, path.w_ld, n, to.mul - n0, left, k_fill, member);
                     }
                     fence_async_smem();
                     __syncwarp();
@@ -512,27 +504,29 @@ __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, c
         for (int w0 = 0; w0 < mul; w0 += 32, turn ^= 1) {
             if (turn != group) continue;
             mine = true;
-            unsigned v[32], u[GtType<T>::SPLIT ? 32 : 1];
-            const unsigned at = quarter + (unsigned)(buf * 256 + w0);
-            tc_load16(at, v);
-            if (w0 + 16 < n) tc_load16(at + 16, v + 16);
-            if constexpr (GtType<T>::SPLIT) {
-                tc_load16(at + n, u);
-                if (w0 + 16 < n) tc_load16(at + n + 16, u + 16);
-            }
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            if (w0 + 32 * GT_EPI_GROUPS >= mul) {           // the group has read its part of the accumulator
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bars.acc_empty + buf);
-            }
-            if (r_of < walk.rows) {
-                float* to_smem = staging + r_of * PITCH + k_of;
+const bool last = w0 + 32 * GT_EPI_GROUPS >= mul;           // the group has read its part of the accumulator then
+            float* to_smem = staging + r_of * PITCH + k_of;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    float s = __uint_as_float(v[j]);
-                    if constexpr (GtType<T>::SPLIT) s += __uint_as_float(u[j]);
-                    to_smem[j * D] = s * scale;
+            for (int h = 0; h < 2; ++h) {
+                unsigned v[16], u[GtType<T>::SPLIT ? 16 : 1];
+                const unsigned at = quarter + (unsigned)(buf * 256 + w0 + 16 * h);
+                if (w0 + 16 * h < n) {
+                    tc_load16(at, v);
+                    if constexpr (GtType<T>::SPLIT) tc_load16(at + n, u);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                }
+                if (last && h == 1) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bars.acc_empty + buf);
+                }
+                if (w0 + 16 * h < n && r_of < walk.rows) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        float s = __uint_as_float(v[j]);
+                        if constexpr (GtType<T>::SPLIT) s += __uint_as_float(u[j]);
+                        to_smem[(16 * h + j) * D] = s * scale;
+                    }
                 }
             }
             group_sync(1 + group, 128);
@@ -556,14 +550,15 @@ __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, c
 }
 
 // What a role does for blocks of D components.
-template <class T, bool TRANS, int D>
+template <class T, bool TRANS, bool FAST, int D>
 __device__ __forceinline__ void gt_roles(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, unsigned char* a_base,
                                          unsigned char* b_base, float* staging, const GtBars& bars, const GtWalk& walk, unsigned tmem, int warp, int tid) {
-    if (warp < GT_PW) gt_produce<T, TRANS, D>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid);
+    if (warp < GT_PW) gt_produce<T, TRANS, FAST, D>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid);
     else gt_drain<T, TRANS, D>(gt, p, tile_of, to, n0, staging, bars, walk, tmem, (warp - GT_PW) >> 2, warp & 3, tid & 31);
 }
 
-template <class T, bool TRANS>
+// FAST: every block of rows and weights is made of whole, aligned 16-byte pieces.
+template <class T, bool TRANS, bool FAST>
 __global__ void __launch_bounds__(GT_THREADS, 1) oeq_grouped_tc(const __grid_constant__ GtProblem gt, const GtArgs p) {
     extern __shared__ __align__(1024) unsigned char gt_smem[];
     unsigned char* smem = gt_smem;
@@ -599,13 +594,12 @@ __global__ void __launch_bounds__(GT_THREADS, 1) oeq_grouped_tc(const __grid_con
     gt_range(range, p.offsets, p.groups, p.rows, part, tile_of.parts, tile_of.extra);       // (two barriers)
     tc_fence_after();
     const unsigned tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile unsigned*>(bars.tmem), 0);
-    const GtWalk walk(p.offsets, range.g, work ? range.lo : 0, work ? range.hi : 0);
+    const GtWalk walk(p.offsets, range.g, work ? (int)range.lo : 0, work ? (int)range.hi : 0);
     if (warp == MMA_WARP) gt_multiply<T, TRANS>(gt, p, tile_of, to, a_base, b_base, bars, walk, gt_tile_rows(d), tmem, elect_lane());
-    else if (d == 1) gt_roles<T, TRANS, 1>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
-    else if (d == 3) gt_roles<T, TRANS, 3>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
-    else if (d == 5) gt_roles<T, TRANS, 5>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
-    else if (d == 7) gt_roles<T, TRANS, 7>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
-    else gt_roles<T, TRANS, 9>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
+    else if (d == 1) gt_roles<T, TRANS, FAST, 1>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
+    else if (d == 3) gt_roles<T, TRANS, FAST, 3>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
+    else if (d == 5) gt_roles<T, TRANS, FAST, 5>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
+    else gt_roles<T, TRANS, FAST, 7>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
     // zeros: the rows without a group, every row where the block has no path
     {
         const long long from = work ? min(__ldg(p.offsets + p.groups), p.rows) : 0, count = p.rows - from;

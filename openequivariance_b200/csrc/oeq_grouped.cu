@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <string>
@@ -46,10 +47,17 @@ int sm_count(int& n) {
     return OEQ_OK;
 }
 
-// Shared memory beyond 48 KB has to be allowed once for a kernel and device; asked for in every call that needs it.
-template <class K>
-int allow_smem(K kernel, size_t bytes) {
-    if (bytes > 48 * 1024) OEQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+// Shared memory beyond 48 KB has to be allowed for a kernel on every device that it runs on: up to the most that any call asks for, at
+// the first call there.
+template <auto KERNEL>
+int allow_smem(size_t most) {
+    static std::atomic<uint64_t> done{0};       // a bit for each device
+    int dev = 0;
+    OEQ_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return OEQ_OK;
+    OEQ_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    done.fetch_or(bit, std::memory_order_release);
     return OEQ_OK;
 }
 
@@ -60,7 +68,9 @@ int check_groups(int64_t rows, int64_t groups) {
 }
 
 // ---------------------------------------------------------------------------- row groups
-size_t small_smem(int64_t groups) { return (RG_SMALL_WARPS * (groups + 1) + 2 * (groups + 2) + 33) * sizeof(int); }
+size_t table_smem(int64_t groups) { return (2 * (groups + 2) + 33) * sizeof(int); }
+size_t walk_smem(int64_t groups) { return RG_WARPS * (groups + 1) * sizeof(int); }
+size_t small_smem(int64_t groups) { return RG_SMALL_WARPS * (groups + 1) * sizeof(int) + table_smem(groups); }
 // One CTA walks 32 rows a step in each of its warps; beyond these many rows the runs of many CTAs are faster.
 bool small_groups(int64_t rows, int64_t groups) { return rows <= 8192 && small_smem(groups) <= SMEM_MOST; }
 struct Runs {
@@ -208,11 +218,17 @@ int tc_product(const GpProblem& gp, int64_t rows, int64_t groups, const void* X,
     GtProblem gt{};
     if (int rc = tc_plan<T>(gp, rows, sms, gt, ctas, smem)) return rc;
     if (ctas == 0) return OEQ_OK;
-    const GtArgs args{X, W, (const long long*)order, (const long long*)offsets, Z, rows, (int)groups,
-                      aligned(X, 16) && gp.src_dim * sizeof(T) % 16 == 0, aligned(W, 16) && gp.w_numel * sizeof(T) % 16 == 0,
-                      aligned(Z, 4) && gp.dst_dim % 2 == 0};
-    if (int rc = allow_smem(oeq_grouped_tc<T, TRANS>, smem)) return rc;
-    oeq_grouped_tc<T, TRANS><<<ctas, GT_THREADS, smem, st>>>(gt, args);
+    const GtArgs args{X, W, (const long long*)order, (const long long*)offsets, Z, rows, (int)groups, aligned(Z, 4) && gp.dst_dim % 2 == 0};
+    constexpr int V = 16 / sizeof(T);
+    bool fast = aligned(X, 16) && aligned(W, 16) && gp.src_dim % V == 0 && gp.w_numel % V == 0;
+    for (int p = 0; p < gp.n_paths; ++p) fast &= gp.path[p].src_off % V == 0 && gp.path[p].src_mul % V == 0 && gp.path[p].w_off % V == 0 && gp.path[p].w_ld % V == 0;
+    if (fast) {
+        if (int rc = allow_smem<oeq_grouped_tc<T, TRANS, true>>(SMEM_MOST)) return rc;
+        oeq_grouped_tc<T, TRANS, true><<<ctas, GT_THREADS, smem, st>>>(gt, args);
+    } else {
+        if (int rc = allow_smem<oeq_grouped_tc<T, TRANS, false>>(SMEM_MOST)) return rc;
+        oeq_grouped_tc<T, TRANS, false><<<ctas, GT_THREADS, smem, st>>>(gt, args);
+    }
     OEQ_CUDA(cudaGetLastError());
     return OEQ_OK;
 }
@@ -249,10 +265,20 @@ int tc_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* X,
     GdProblem gd{gp, tc_split(gp, rows, sms), {}};
     for (int p = 0; p < gp.n_paths; ++p) gd.extra[p] = 96 / gp.target[gp.path[p].dst].d;
     const GdArgs args{X, dZ, (const long long*)order, (const long long*)offsets, dW, (float*)((char*)ws + positions_bytes(gp, gd.split)), (long long*)ws, rows, (int)groups,
-                      aligned(X, 16) && gp.src_dim * sizeof(T) % 16 == 0, aligned(dZ, 16) && gp.dst_dim * sizeof(T) % 16 == 0,
                       aligned(dW, 16) && gp.w_numel * sizeof(T) % 16 == 0};
-    if (int rc = allow_smem(oeq_grouped_tc_dw<T>, GD_SMEM)) return rc;
-    oeq_grouped_tc_dw<T><<<gd.split.first[gp.n_paths], GD_THREADS, GD_SMEM, st>>>(gd, args);
+    constexpr int V = 16 / sizeof(T);
+    bool fast = aligned(X, 16) && aligned(dZ, 16) && gp.src_dim % V == 0 && gp.dst_dim % V == 0;
+    for (int p = 0; p < gp.n_paths; ++p) {
+        const GpTarget& to = gp.target[gp.path[p].dst];
+        fast &= gp.path[p].src_off % V == 0 && gp.path[p].src_mul % V == 0 && to.off % V == 0 && to.mul % V == 0;
+    }
+    if (fast) {
+        if (int rc = allow_smem<oeq_grouped_tc_dw<T, true>>(GD_SMEM)) return rc;
+        oeq_grouped_tc_dw<T, true><<<gd.split.first[gp.n_paths], GD_THREADS, GD_SMEM, st>>>(gd, args);
+    } else {
+        if (int rc = allow_smem<oeq_grouped_tc_dw<T, false>>(GD_SMEM)) return rc;
+        oeq_grouped_tc_dw<T, false><<<gd.split.first[gp.n_paths], GD_THREADS, GD_SMEM, st>>>(gd, args);
+    }
     OEQ_CUDA(cudaGetLastError());
     return join<T>(gp, gd.split, GD_TILE, rows, groups, offsets, dW, ws, st);
 }
@@ -305,15 +331,15 @@ int oeq_row_groups(int64_t rows, int64_t groups, const int64_t* index, int64_t* 
     long long *ord = (long long*)order, *slt = (long long*)slots, *off = (long long*)offsets;
     if (small_groups(rows, groups)) {
         const size_t smem = small_smem(groups);
-        if (int rc = allow_smem(oeq_row_groups_small, smem)) return rc;
+        if (int rc = allow_smem<oeq_row_groups_small>(SMEM_MOST)) return rc;
         oeq_row_groups_small<<<1, 32 * RG_SMALL_WARPS, smem, st>>>(in, (int)rows, (int)groups, n, ord, slt, off, blocks);
     } else {
         const Runs r = runs_of(rows);
         int *counts = (int*)workspace, *totals = counts + (size_t)r.runs * keys;
         const unsigned ctas = (unsigned)((r.runs + RG_WARPS - 1) / RG_WARPS);
-        const size_t smem = (size_t)RG_WARPS * keys * sizeof(int), smem_place = smem + (2 * (groups + 2) + 33) * sizeof(int);
-        if (int rc = allow_smem(oeq_row_groups_count, smem)) return rc;
-        if (int rc = allow_smem(oeq_row_groups_place, smem_place)) return rc;
+        const size_t smem = walk_smem(groups), smem_place = smem + table_smem(groups);
+        if (int rc = allow_smem<oeq_row_groups_count>(walk_smem(OEQ_MOST_GROUPS))) return rc;
+        if (int rc = allow_smem<oeq_row_groups_place>(walk_smem(OEQ_MOST_GROUPS) + table_smem(OEQ_MOST_GROUPS))) return rc;
         oeq_row_groups_count<<<ctas, 32 * RG_WARPS, smem, st>>>(in, rows, r.run, r.runs, (int)groups, counts);
         OEQ_CUDA(cudaGetLastError());
         oeq_row_groups_scan<<<(unsigned)((keys + 31) / 32), 1024, 0, st>>>(counts, totals, r.runs, keys);
@@ -328,8 +354,8 @@ int oeq_row_groups_from_counts(int64_t rows, int64_t groups, const int64_t* coun
     if (int rc = check_groups(rows, groups)) return rc;
     if (!counts || !offsets || (rows > 0 && (!index || !blocks))) return oeq_fail(OEQ_ERR_INVALID, "null pointer");
     const int n = (int)oeq_row_groups_blocks(rows, groups);
-    const size_t smem = (2 * (groups + 2) + 33) * sizeof(int);
-    if (int rc = allow_smem(oeq_row_groups_counts, smem)) return rc;
+    const size_t smem = table_smem(groups);
+    if (int rc = allow_smem<oeq_row_groups_counts>(table_smem(OEQ_MOST_GROUPS))) return rc;
     const unsigned ctas = (unsigned)std::min<int64_t>(296, std::max<int64_t>(1, (rows + 511) / 512));
     oeq_row_groups_counts<<<ctas, 512, smem, (cudaStream_t)stream>>>((const long long*)counts, rows, (int)groups, n, (long long*)index, (long long*)offsets, blocks);
     OEQ_CUDA(cudaGetLastError());
