@@ -5,10 +5,12 @@
 //
 // M = 128 input channels u, N = up to 128 output channels w of one path, and the sum runs over rows and components.  Both operands have their
 // channels along memory, so both are "MN-major": a lane reads the 16 d bytes of V channels of a row and writes d pieces, one into
-// the slot of each component.  A slot of the ring has one component of GdType::ROWS sorted rows of one group, X and dZ, 16 KB.
-//   * 16 producer warps: two sets of eight take units of rows in turn, a lane the same channels of X and dZ; from five components on one
-//     set, half of it for X and half for dZ (the slots of the units under way have to fit the ring);
-//   * one warp, in step, issues the MMAs: FP32 hi.hi and hi.lo as one, lo.hi into hi.lo's columns;
+// the slot of each component.  A slot has one component of GdType::ROWS sorted rows of one group, X and dZ, 16 KB; four of them are
+// a bundle, and there are two bundles.
+//   * 16 producer warps.  One and three components: two sets of eight take units of rows in turn, each with a bundle of its own, a lane the same
+//     channels of X and dZ.  Five and seven: one set, half of it for X and half for dZ, the components of a unit in two bundles;
+//   * one warp, in step, issues the MMAs of a bundle, as many as there are between two waits (a wait for each slot: 575 cycles a slot, where its
+//     MMAs take 192): FP32 hi.hi and hi.lo as one, lo.hi into hi.lo's columns;
 //   * 8 warps add the accumulators to sums in shared memory at the end of a group and after CHAIN slots: an MMA's additions are cut off, not
 //     rounded, and the error grows with the length of a chain (relative, one chain of 750 slots: 1e-5).  The two accumulators alternate.
 //     These warps also prefetch the rows of the chain after next to L2.
@@ -19,18 +21,18 @@
 
 namespace oeq {
 
-constexpr int GD_TILE = 128, GD_RING = 8, GD_SLOT = 16384, GD_SUMS = GD_TILE * GD_TILE * 4;
+constexpr int GD_TILE = 128, GD_BUNDLE = 4, GD_SLOT = 16384, GD_RING = 2 * GD_BUNDLE, GD_SUMS = GD_TILE * GD_TILE * 4;
 constexpr int GD_PW = 16, GD_EPI = 8, GD_THREADS = (GD_PW + GD_EPI + 1) * 32;
 constexpr int GD_SMEM = GD_RING * GD_SLOT + GD_SUMS + 1024;
 constexpr int ERR_GD_EMPTY = 91, ERR_GD_FULL = 92, ERR_GD_ACC_FULL = 93, ERR_GD_ACC_EMPTY = 94;
 
-template <class T> struct GdType { static constexpr int ROWS = 32, CHAIN = 16; };
+template <class T> struct GdType { static constexpr int ROWS = 32, CHAIN = 32; };
 template <> struct GdType<float> { static constexpr int ROWS = 8, CHAIN = 32; };
-// Sets of producers.  A warp waits for the slots of its units alone, so it can tell the phases of a slot apart as long as the units under
-// way, one of each set, fit the ring.
-__host__ __device__ constexpr int gd_sets(int d) { return d <= 3 ? 2 : 1; }
-// rows of a unit: whole slots
-template <class T> __host__ __device__ constexpr int gd_unit(int d) { return sizeof(T) == 4 ? (d == 1 ? 32 : 8) : (d == 1 ? 64 : 32); }
+__host__ __device__ constexpr int gd_sets(int d) { return d <= 3 ? 2 : 1; }     // of producers
+// rows of a unit: with one component a bundle of slots, else one slot of each component
+template <class T> __host__ __device__ constexpr int gd_unit(int d) { return d == 1 ? GD_BUNDLE * GdType<T>::ROWS : GdType<T>::ROWS; }
+// components of a unit's first bundle
+__host__ __device__ constexpr int gd_first(int d) { return d <= GD_BUNDLE ? d : (d + 1) / 2; }
 
 struct GdProblem {
     GpProblem gp;               // paths in the order of their weights
@@ -66,8 +68,8 @@ struct GdBars {
     unsigned* tmem;
     __device__ explicit GdBars(unsigned char* control) {
         full = reinterpret_cast<unsigned long long*>(control);
-        empty = full + GD_RING;
-        acc_full = empty + GD_RING;
+        empty = full + 2;
+        acc_full = empty + 2;
         acc_empty = acc_full + 2;
         tmem = reinterpret_cast<unsigned*>(acc_empty + 2);
     }
@@ -95,38 +97,37 @@ struct GdLane {
     int lp, r0, ch;             // lanes of a row; the lane's first row, its channel
     int x_left, z_left;         // channels of X and dZ from there on (0: another lane's)
 };
-template <class T, int D>
-__device__ __forceinline__ void gd_put(const uint4 (&v)[D], unsigned char* ring, int slot, int at, int at_lo) {
+// Components [K0, K1) of V channels, to the slots from `dst` on.
+template <class T, int D, int K0, int K1>
+__device__ __forceinline__ void gd_put(const uint4 (&v)[D], unsigned char* dst, int lo) {
 #pragma unroll
-    for (int k = 0; k < D; ++k) {
-        unsigned char* dst = ring + slot * GD_SLOT;
-        if (++slot == GD_RING) slot = 0;
+    for (int k = K0; k < K1; ++k) {
         const uint4 a = gt_component<T, D>(v, k);
         if constexpr (GtType<T>::SPLIT) {
-            float4 hi, lo;
-            gt_split(*reinterpret_cast<const float4*>(&a), hi, lo);
-            *reinterpret_cast<float4*>(dst + at) = hi;
-            *reinterpret_cast<float4*>(dst + at_lo) = lo;
+            float4 hi, lo4;
+            gt_split(*reinterpret_cast<const float4*>(&a), hi, lo4);
+            *reinterpret_cast<float4*>(dst + (k - K0) * GD_SLOT) = hi;
+            *reinterpret_cast<float4*>(dst + (k - K0) * GD_SLOT + lo) = lo4;
         } else {
-            *reinterpret_cast<uint4*>(dst + at) = a;
+            *reinterpret_cast<uint4*>(dst + (k - K0) * GD_SLOT) = a;
         }
     }
 }
+// A unit of rows.  `bundle`: that of the first components; `parity` of the wait for it to be free again (no wait: the first use).
 template <class T, int D, bool FAST>
-__device__ __forceinline__ void gd_fill(const GdArgs& p, const GpProblem& gp, const GtWalk& walk, const GdLane& l, const T* x, const T* z, int n, unsigned char* ring,
-                                        int first, const GdBars& bars, int use, bool& ok) {
-    constexpr bool BOTH = gd_sets(D) == 2;      // a lane reads both operands, else x is the lane's operand
-    constexpr int ROWS = GdType<T>::ROWS, THREADS = 256, PASS = D == 1 ? 4 : 1;
-    const int slots = (walk.rows + ROWS - 1) / ROWS, rows = slots * ROWS, step = THREADS >> l.lp, blocks = (n + 63) / 64;
-    bool waited = false;
-    auto wait = [&]() {                         // until every slot of the unit is free again
-        if (waited) return;
-        waited = true;
-        for (int s = 0; s < slots * D && ok; ++s) {
-            const int at_ring = first + s < GD_RING ? first + s : first + s - GD_RING, u = first + s < GD_RING ? use : use + 1;
-            if (u > 0) ok = warp_wait(ok, bars.empty + at_ring, (unsigned)(u - 1) & 1, &gt_status, ERR_GD_EMPTY);
-        }
+__device__ __forceinline__ bool gd_fill(const GdArgs& p, const GpProblem& gp, const GtWalk& walk, const GdLane& l, const T* x, const T* z, int n, unsigned char* ring,
+                                        const GdBars& bars, int bundle, int use) {
+    constexpr bool BOTH = gd_sets(D) == 2;      // a lane reads both operands
+    constexpr int ROWS = GdType<T>::ROWS, THREADS = 256, PASS = D == 1 ? 4 : (sizeof(T) == 4 ? 1 : 2), FIRST = gd_first(D);
+    const int rows = (walk.rows + ROWS - 1) / ROWS * ROWS, step = THREADS >> l.lp, blocks = (n + 63) / 64, lane = threadIdx.x & 31;
+    const bool is_x = l.x_left > 0;
+    auto free_again = [&](int b) { return use == 0 || warp_wait(true, bars.empty + b, (unsigned)(use - 1) & 1, &gt_status, ERR_GD_EMPTY); };
+    auto filled = [&](int b) {
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars.full + b);
     };
+    bool waited = false;
 #pragma unroll 1
     for (int q0 = 0; q0 < rows; q0 += PASS * step) {
         uint4 v[PASS][D], w[BOTH ? PASS : 1][D];
@@ -143,32 +144,49 @@ __device__ __forceinline__ void gd_fill(const GdArgs& p, const GpProblem& gp, co
                 gt_read<T, D, FAST>(v[j], x + (long long)row[j] * gp.src_dim, in ? l.x_left : 0);
                 gt_read<T, D, FAST>(w[j], z + (long long)row[j] * gp.dst_dim, in ? l.z_left : 0);
             } else {
-                const bool is_x = l.x_left > 0;
                 gt_read<T, D, FAST>(v[j], is_x ? x + (long long)row[j] * gp.src_dim : z + (long long)row[j] * gp.dst_dim, in ? (is_x ? l.x_left : l.z_left) : 0);
             }
         }
-        wait();
-        if (!ok) return;
+        if (!waited && !free_again(bundle)) return false;
+        auto place = [&](int j, bool of_x, unsigned char*& dst, int& lo) {
+            const int q = l.r0 + q0 + j * step, r = q % ROWS;
+            const int at = of_x ? gd_place<T>(l.ch, r, GD_TILE / 64) : 8192 + gd_place<T>(l.ch, r, blocks);
+            dst = ring + (bundle * GD_BUNDLE + q / ROWS * (D == 1)) * GD_SLOT + at;
+            lo = of_x ? 4096 : 8192 + gd_place<T>(l.ch + n, r, 0) - at;
+            return q < rows && (of_x ? l.x_left : l.z_left) > 0;
+        };
 #pragma unroll
         for (int j = 0; j < PASS; ++j) {
-            const int q = l.r0 + q0 + j * step, r = q % ROWS;
-            if (q >= rows) continue;
-            int slot = first + q / ROWS * D;
-            if (slot >= GD_RING) slot -= GD_RING;
-            if (l.x_left > 0) {
-                const int at = gd_place<T>(l.ch, r, GD_TILE / 64);
-                gd_put<T, D>(v[j], ring, slot, at, at + 4096);
+            unsigned char* dst;
+            int lo;
+            if (BOTH || is_x) {
+                if (place(j, true, dst, lo)) gd_put<T, D, 0, FIRST>(v[j], dst, lo);
             }
-            if (l.z_left > 0) gd_put<T, D>(BOTH ? w[j] : v[j], ring, slot, 8192 + gd_place<T>(l.ch, r, blocks), 8192 + gd_place<T>(l.ch + n, r, 0));
+            if (BOTH || !is_x) {
+                if (place(j, false, dst, lo)) gd_put<T, D, 0, FIRST>(BOTH ? w[j] : v[j], dst, lo);
+            }
         }
+        if constexpr (FIRST < D) {
+            if (q0 + PASS * step >= rows) filled(bundle);
+            if (!waited && !free_again(bundle ^ 1)) return false;
+#pragma unroll
+            for (int j = 0; j < PASS; ++j) {
+                unsigned char* dst;
+                int lo;
+                if (place(j, is_x, dst, lo)) gd_put<T, D, FIRST, D>(v[j], dst + (1 - 2 * bundle) * (GD_BUNDLE * GD_SLOT), lo);
+            }
+        }
+        waited = true;
     }
+    filled(FIRST < D ? bundle ^ 1 : bundle);
+    return true;
 }
 
 template <class T, bool FAST, int D>
 __device__ __forceinline__ void gd_produce(const GdArgs& p, const GpProblem& gp, const GpPath& path, const GpTarget& to, int u0, int w0, int mu, int mw, int n,
                                            unsigned char* ring, const GdBars& bars, GtWalk walk, int tid) {
-    constexpr int V = GtType<T>::V, ROWS = GdType<T>::ROWS, SETS = gd_sets(D), UNIT = gd_unit<T>(D);
-    const int half = tid >> 8, member = tid & 255, lane = tid & 31;
+    constexpr int V = GtType<T>::V, SETS = gd_sets(D), UNIT = gd_unit<T>(D);
+    const int half = tid >> 8, member = tid & 255;
     GdLane l;
     l.lp = 0;
     while ((V << l.lp) < max(mu, mw)) ++l.lp;
@@ -177,23 +195,13 @@ __device__ __forceinline__ void gd_produce(const GdArgs& p, const GpProblem& gp,
     l.x_left = SETS == 2 || half == 0 ? mu - l.ch : 0;
     l.z_left = SETS == 2 || half == 1 ? mw - l.ch : 0;
     const T *x = static_cast<const T*>(p.X) + path.src_off + (u0 + l.ch) * D, *z = static_cast<const T*>(p.dZ) + to.off + (w0 + l.ch) * D;
-    int turn = 0, first = 0, use = 0;
-    bool ok = true;
-    for (; walk.more(); walk.next(p.offsets, p.groups)) {
+    int units = 0;
+    for (; walk.more(); walk.next(p.offsets, p.groups), ++units) {
         walk.tile(UNIT);
-        const int slots = (walk.rows + ROWS - 1) / ROWS * D;
-        if (SETS == 1 || turn == half) {
-            gd_fill<T, D, FAST>(p, gp, walk, l, x, z, n, ring, first, bars, use, ok);
-            if (!ok) return;
-            fence_async_smem();
-            __syncwarp();
-            if (lane < slots) mbar_arrive(bars.full + (first + lane < GD_RING ? first + lane : first + lane - GD_RING));
-        }
-        turn ^= 1;
-        first += slots;
-        if (first >= GD_RING) {
-            first -= GD_RING;
-            ++use;
+        if (SETS == 1) {
+            if (!gd_fill<T, D, FAST>(p, gp, walk, l, x, z, n, ring, bars, 0, units)) return;
+        } else if ((units & 1) == half) {
+            if (!gd_fill<T, D, FAST>(p, gp, walk, l, x, z, n, ring, bars, half, units >> 1)) return;
         }
     }
 }
@@ -205,11 +213,12 @@ __device__ __forceinline__ void gd_multiply(const GdArgs& p, int d, int unit, in
     const int blocks = (n + 63) / 64;
     const unsigned wide = gt_idesc<T, false>(GtType<T>::acc(n)) | MN, narrow = gt_idesc<T, false>(n) | MN;
     const unsigned long long a0 = gd_desc<T>(smem_u32(ring), GD_TILE / 64), b0 = gd_desc<T>(smem_u32(ring) + 8192, blocks);
+    const int first = gd_first(d), bundles = first < d ? 2 : 1, sets = gd_sets(d);
     GdChain<T> chain;
-    int slot = 0, use = 0, accs = 0;
+    int units = 0, accs = 0;
     unsigned accumulate = 0;
     bool ok = true;
-    for (; walk.more() && ok; walk.next(p.offsets, p.groups)) {
+    for (; walk.more() && ok; walk.next(p.offsets, p.groups), ++units) {
         walk.tile(unit);
         const int slots = chain.unit(walk, d), buf = accs & 1;
         if (chain.begins) {
@@ -217,27 +226,28 @@ __device__ __forceinline__ void gd_multiply(const GdArgs& p, int d, int unit, in
             accumulate = 0;
         }
         const unsigned acc = tmem + (unsigned)(buf * 256);
-        for (int s = 0; s < slots && ok; ++s) {
-            ok = warp_wait(ok, bars.full + slot, (unsigned)use & 1, &gt_status, ERR_GD_FULL);
+        for (int i = 0; i < bundles && ok; ++i) {
+            const int bundle = sets == 2 ? units & 1 : i, n_slots = bundles == 1 ? slots : (i == 0 ? first : d - first);
+            ok = warp_wait(ok, bars.full + bundle, (unsigned)(sets == 2 ? units >> 1 : units) & 1, &gt_status, ERR_GD_FULL);
             if (!ok) break;
             tc_fence_after();
-            const unsigned long long a = a0 + (unsigned long long)(slot * (GD_SLOT >> 4)), b = b0 + (unsigned long long)(slot * (GD_SLOT >> 4));
-            if constexpr (GtType<T>::SPLIT) {
-                gt_mma<T>(leader, acc, a, b, wide, accumulate);
-                gt_mma<T>(leader, acc + (unsigned)n, a + (4096 >> 4), b, narrow, 1);
-                accumulate = 1;
-            } else {
+            unsigned long long a = a0 + (unsigned long long)(bundle * (GD_BUNDLE * GD_SLOT >> 4)), b = b0 + (unsigned long long)(bundle * (GD_BUNDLE * GD_SLOT >> 4));
 #pragma unroll
-                for (int h = 0; h < GdType<T>::ROWS / 16; ++h) {
-                    gt_mma<T>(leader, acc, a + (unsigned long long)(h * (2 * (GD_TILE / 64) * 1024 >> 4)), b + (unsigned long long)(h * (2 * blocks * 1024 >> 4)), wide, accumulate);
+            for (int s = 0; s < GD_BUNDLE; ++s, a += GD_SLOT >> 4, b += GD_SLOT >> 4) {
+                if (s >= n_slots) break;
+                if constexpr (GtType<T>::SPLIT) {
+                    gt_mma<T>(leader, acc, a, b, wide, accumulate);
+                    gt_mma<T>(leader, acc + (unsigned)n, a + (4096 >> 4), b, narrow, 1);
                     accumulate = 1;
+                } else {
+#pragma unroll
+                    for (int h = 0; h < GdType<T>::ROWS / 16; ++h) {
+                        gt_mma<T>(leader, acc, a + (unsigned long long)(h * (2 * (GD_TILE / 64) * 1024 >> 4)), b + (unsigned long long)(h * (2 * blocks * 1024 >> 4)), wide, accumulate);
+                        accumulate = 1;
+                    }
                 }
             }
-            tc_commit_if(leader, bars.empty + slot);
-            if (++slot == GD_RING) {
-                slot = 0;
-                ++use;
-            }
+            tc_commit_if(leader, bars.empty + bundle);
         }
         if (ok && chain.ends) {
             tc_commit_if(leader, bars.acc_full + buf);
@@ -283,7 +293,6 @@ __device__ __forceinline__ void gd_sum(const GdArgs& p, const GpProblem& gp, con
         walk.tile(unit);
         chain.unit(walk, d);
         if (!chain.ends) continue;
-        prefetch();
         const int buf = accs & 1;
         if (!warp_wait(true, bars.acc_full + buf, (unsigned)(accs / 2) & 1, &gt_status, ERR_GD_ACC_FULL)) return;
         tc_fence_after();
@@ -305,6 +314,7 @@ __device__ __forceinline__ void gd_sum(const GdArgs& p, const GpProblem& gp, con
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.acc_empty + buf);
         ++accs;
+        prefetch();
         if (!chain.piece_ends) continue;
         const int begin = (int)__ldg(p.offsets + walk.g), end = GtWalk::end_of(p.offsets, walk.g);
         begun = false;
@@ -348,11 +358,9 @@ __global__ void __launch_bounds__(GD_THREADS, 1) oeq_grouped_tc_dw(const __grid_
     GtRange& range = *reinterpret_cast<GtRange*>(control + 512);
     constexpr int MMA_WARP = GD_PW + GD_EPI;
     if (tid == 0) {
-        for (int i = 0; i < GD_RING; ++i) {
+        for (int i = 0; i < 2; ++i) {
             mbar_init(bars.full + i, GD_PW / gd_sets(d));
             mbar_init(bars.empty + i, 1);
-        }
-        for (int i = 0; i < 2; ++i) {
             mbar_init(bars.acc_full + i, 1);
             mbar_init(bars.acc_empty + i, GD_EPI);
         }
