@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt(const __grid
 // A CTA has a path, a tile of its weights and a range of the sorted rows.  A group that lies within the range is complete; the part of
 // one that began before it goes to slot 0 of the CTA's two partial tiles, the part of one that goes on behind it to slot 1.
 // oeq_grouped_join adds the parts in the order of the ranges: no atomics, the same sums in every run.
+constexpr int GP_PARTS = 1024;                  // most ranges of a path
 struct GpSplit {
     int parts[GP_PATHS];        // ranges of each path
     int first[GP_PATHS + 1];    // its first CTA
@@ -240,42 +241,68 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __g
 }
 
 // Gradients of the groups that no single range has: the sum of their parts, and zeros where there are no rows.
-// lo_of: first positions of the CTAs' ranges, ascending over the parts of a tile.  Blocks x over the weights, y over the groups.
-template <class T>
+// lo_of: first positions of the CTAs' ranges, ascending over the parts of a tile.  CTA (x, y): one of `slices` parts of a tile of
+// TILE x TILE weights, and every gridDim.y-th group.  (A thread for each weight and group, 65 536 x 512x0e to 512x0e BF16, 64 groups: 200 us,
+// most of it to find that a group is complete; by tiles 10.)
+template <class T, int TILE>
 __global__ void __launch_bounds__(256) oeq_grouped_join(const __grid_constant__ GpProblem gp, const __grid_constant__ GpSplit split,
-                                                        const long long* __restrict__ offsets, long long rows, int groups, int tile_u, int tile_w,
+                                                        const long long* __restrict__ offsets, long long rows, int groups, int slices,
                                                         const typename GpAcc<T>::type* __restrict__ partial, const long long* __restrict__ lo_of, T* __restrict__ dW) {
     typedef typename GpAcc<T>::type A;
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= gp.w_numel) return;
-    int p = 0;
-    while (p + 1 < gp.n_paths && i >= gp.path[p + 1].w_off) ++p;           // (the paths lie in the order of their weights)
+    __shared__ int list[GP_PARTS + 1];          // ranges whose parts are added, and their number
+    const int slice = TILE / slices;
+    int p = 0, tile = blockIdx.x / slices;
+    for (;; ++p) {
+        const int tiles = (split.first[p + 1] - split.first[p]) / split.parts[p];
+        if (tile < tiles) break;
+        tile -= tiles;
+    }
     const GpPath& path = gp.path[p];
-    const int parts = split.parts[p], u = (i - path.w_off) / path.w_ld, w = (i - path.w_off) % path.w_ld;
-    const int cta = split.first[p] + (u / tile_u * ((path.w_ld + tile_w - 1) / tile_w) + w / tile_w) * parts;
-    const long long tile = (long long)tile_u * tile_w, n = min(__ldg(offsets + groups), rows);
-    const A* at = partial + cta * 2 * tile + (long long)(u % tile_u) * tile_w + w % tile_w;
-    auto part_of = [&](long long position) {    // the last range that begins at or before it
-        int a = 0, b = parts - 1;
-        while (a < b) {
-            const int mid = (a + b + 1) >> 1;
-            if (__ldg(lo_of + cta + mid) <= position) a = mid;
-            else b = mid - 1;
-        }
-        return a;
-    };
+    const GpTarget& to = gp.target[path.dst];
+    const int parts = split.parts[p], cta = split.first[p] + tile * parts, w_tiles = (to.mul + TILE - 1) / TILE;
+    const int u0 = tile / w_tiles * TILE + blockIdx.x % slices * slice, w0 = tile % w_tiles * TILE, nu = min(slice, path.src_mul - u0), nw = min(TILE, to.mul - w0);
+    if (nu <= 0) return;
+    const A* at = partial + (long long)cta * 2 * (TILE * TILE) + blockIdx.x % slices * slice * TILE;
+    const long long n = min(__ldg(offsets + groups), rows);
+    const A scale = (A)to.scale;
     for (int g = blockIdx.y; g < groups; g += gridDim.y) {
         const long long begin = min(__ldg(offsets + g), n), end = min(__ldg(offsets + g + 1), n);
-        A s = A(0);
+        int j0 = -1, j1 = -1;                   // the last ranges that begin at or before the group's first and last row
         if (begin < end) {
-            const int j0 = part_of(begin), j1 = part_of(end - 1);
+            for (int j = 0; j < parts; j += 256) {
+                const long long lo = j + threadIdx.x < parts ? __ldg(lo_of + cta + j + threadIdx.x) : n;
+                j0 += __syncthreads_count(lo <= begin);
+                j1 += __syncthreads_count(lo <= end - 1);
+            }
             if (j0 == j1) continue;
-            s = at[(j0 * 2 + 1) * tile];
-            for (int j = j0 + 1; j <= j1; ++j)
-                if (j == j1 || __ldg(lo_of + cta + j) < __ldg(lo_of + cta + j + 1)) s += at[j * 2 * tile];     // (a range without rows has no part)
-            s *= (A)gp.target[path.dst].scale;
+            if (threadIdx.x < 32) {             // (a range without rows has no part)
+                int count = 0;
+                for (int j = j0 + 1; j <= j1; j += 32) {
+                    const int k = j + threadIdx.x;
+                    const bool in = k <= j1 && (k == j1 || __ldg(lo_of + cta + k) < __ldg(lo_of + cta + k + 1));
+                    const unsigned all = __ballot_sync(0xffffffffu, in);
+                    if (in) list[count + __popc(all & ((1u << threadIdx.x) - 1))] = k;
+                    count += __popc(all);
+                }
+                if (threadIdx.x == 0) list[GP_PARTS] = count;
+            }
+            __syncthreads();
         }
-        gp_store(dW + (long long)g * gp.w_numel + i, s);
+        T* out = dW + (long long)g * gp.w_numel + path.w_off + (long long)u0 * path.w_ld + w0;
+        for (int i = threadIdx.x; i < nu * TILE; i += 256) {
+            const int u = i / TILE, w = i % TILE;
+            if (w >= nw) continue;
+            A s = A(0);
+            if (begin < end) {
+                s = at[(long long)(j0 * 2 + 1) * (TILE * TILE) + i];
+                const int count = list[GP_PARTS];
+#pragma unroll 8
+                for (int k = 0; k < count; ++k) s += at[(long long)list[k] * 2 * (TILE * TILE) + i];
+                s *= scale;
+            }
+            gp_store(out + (long long)u * path.w_ld + w, s);
+        }
+        __syncthreads();                        // (the list is written again)
     }
 }
 

@@ -13,7 +13,6 @@
 //     MMAs take 192): FP32 hi.hi and hi.lo as one, lo.hi into hi.lo's columns;
 //   * 8 warps add the accumulators to sums in shared memory at the end of a group and after CHAIN slots: an MMA's additions are cut off, not
 //     rounded, and the error grows with the length of a chain (relative, one chain of 750 slots: 1e-5).  The two accumulators alternate.
-//     These warps also prefetch the rows of the chain after next to L2.
 // A CTA has one tile of one path and a range of the sorted rows (gt_range); groups that go beyond the range leave a partial tile for
 // oeq_grouped_join.  Every wait is bounded.
 #pragma once
@@ -269,25 +268,6 @@ __device__ __forceinline__ void gd_sum(const GdArgs& p, const GpProblem& gp, con
     GdChain<T> chain;
     float* sum = sums + c0 * GD_TILE + u;
     bool begun = false;         // the group's sums hold something
-    // rows of the chain after next, to L2
-    constexpr int LINE = 128 / sizeof(T), THREADS = GD_EPI * 32;
-    GtWalk ahead = walk;
-    GdChain<T> chain_ahead;
-    auto prefetch = [&]() {
-        for (bool more = true; more && ahead.more(); ahead.next(p.offsets, p.groups)) {
-            ahead.tile(unit);
-            chain_ahead.unit(ahead, d);
-            more = !chain_ahead.ends;
-            for (int r = (warp * 32 + lane) >> 3; r < ahead.rows; r += THREADS / 8) {
-                const long long row = gp_row(p.order, ahead.pos + r);
-                const T *x = static_cast<const T*>(p.X) + row * gp.src_dim + path.src_off + u0 * d, *z = static_cast<const T*>(p.dZ) + row * gp.dst_dim + to.off + w0 * d;
-                for (int i = (lane & 7) * LINE; i < mu * d; i += 8 * LINE) gt_prefetch(x + i);
-                for (int i = (lane & 7) * LINE; i < mw * d; i += 8 * LINE) gt_prefetch(z + i);
-            }
-        }
-    };
-    prefetch();
-    prefetch();
     int accs = 0;
     for (; walk.more(); walk.next(p.offsets, p.groups)) {
         walk.tile(unit);
@@ -314,7 +294,6 @@ __device__ __forceinline__ void gd_sum(const GdArgs& p, const GpProblem& gp, con
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.acc_empty + buf);
         ++accs;
-        prefetch();
         if (!chain.piece_ends) continue;
         const int begin = (int)__ldg(p.offsets + walk.g), end = GtWalk::end_of(p.offsets, walk.g);
         begun = false;

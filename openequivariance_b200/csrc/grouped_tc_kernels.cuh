@@ -14,7 +14,7 @@
 //   * one warp, in step, issues the MMAs.  FP32: hi.hi and hi.lo as one MMA over the weights' hi channels followed by lo, lo.hi
 //     into hi.lo's columns: the large and the small products have accumulators of their own.
 //   * 8 epilogue warps, in two groups, add those, scale, and write rows through shared memory, so that a row's values leave in order.  They
-//     also prefetch the rows and weights of the tile after next to L2: the producers' loads then take a third of the time.
+//     also prefetch the weights of the tile after next to L2.  (Its rows too: 184 us instead of 149 for 100 000 rows of 128x(0e+1o+2e) BF16.)
 // Two accumulators: a tile drains while the next is computed.  Every wait is bounded; on expiry a role records a code and all
 // leave.
 #pragma once
@@ -447,26 +447,16 @@ __device__ __forceinline__ void gt_write(const float* staging, const int* rows_o
 }
 
 __device__ __forceinline__ void gt_prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-// Rows of a tile, and the weights of its group where they change, to L2 by the epilogue warps.
+// The weights of a group to L2 by the epilogue warps.
 template <class T, bool TRANS>
-__device__ __forceinline__ void gt_ahead(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, const GtWalk& walk, bool weights,
-                                         int tid) {
+__device__ __forceinline__ void gt_ahead(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, int g, int tid) {
     constexpr int LINE = 128 / sizeof(T), THREADS = GT_EPI * 32;
     for (int path_no = to.path_begin; path_no < to.path_end; ++path_no) {
         const GpPath& path = gt.gp.path[path_no];
-        if (n0 == 0) {                          // (the CTAs of an output block's other channels read the same rows)
-            const int len = path.src_mul * to.d;
-            for (int r = tid >> 3; r < walk.rows; r += THREADS / 8) {
-                const T* x = static_cast<const T*>(p.X) + gp_row(p.order, walk.pos + r) * gt.gp.src_dim + path.src_off;
-                for (int i = (tid & 7) * LINE; i < len; i += 8 * LINE) gt_prefetch(x + i);
-            }
-        }
-        if (weights) {
-            const int n = min(tile_of.n, to.mul - n0), rows = TRANS ? n : path.src_mul, len = TRANS ? path.src_mul : n;
-            const T* w = static_cast<const T*>(p.W) + (long long)walk.g * gt.gp.w_numel + path.w_off + (TRANS ? (long long)n0 * path.w_ld : n0);
-            for (int r = tid >> 2; r < rows; r += THREADS / 4)
-                for (int i = (tid & 3) * LINE; i < len; i += 4 * LINE) gt_prefetch(w + (long long)r * path.w_ld + i);
-        }
+        const int n = min(tile_of.n, to.mul - n0), rows = TRANS ? n : path.src_mul, len = TRANS ? path.src_mul : n;
+        const T* w = static_cast<const T*>(p.W) + (long long)g * gt.gp.w_numel + path.w_off + (TRANS ? (long long)n0 * path.w_ld : n0);
+        for (int r = tid >> 2; r < rows; r += THREADS / 4)
+            for (int i = (tid & 3) * LINE; i < len; i += 4 * LINE) gt_prefetch(w + (long long)r * path.w_ld + i);
     }
 }
 
@@ -485,7 +475,7 @@ __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, c
     auto prefetch = [&]() {
         if (ahead.more()) {
             ahead.tile(TILE_ROWS);
-            gt_ahead<T, TRANS>(gt, p, tile_of, to, n0, ahead, ahead.g != have, group * 128 + pair);
+            if (ahead.g != have) gt_ahead<T, TRANS>(gt, p, tile_of, to, n0, ahead.g, group * 128 + pair);
             have = ahead.g;
             ahead.next(p.offsets, p.groups);
         }

@@ -119,7 +119,7 @@ GpSplit simt_split(const GpProblem& gp, int64_t rows, int sms) {
     int columns = 0;
     auto tiles = [&](int p) { return (gp.path[p].src_mul + GP_TILE - 1) / GP_TILE * ((gp.target[gp.path[p].dst].mul + GP_TILE - 1) / GP_TILE); };
     for (int p = 0; p < gp.n_paths; ++p) columns += tiles(p);
-    const int parts = (int)std::max<int64_t>(1, std::min<int64_t>((4 * sms + columns - 1) / std::max(1, columns), rows / 64));
+    const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(GP_PARTS, (4 * sms + columns - 1) / std::max(1, columns)), rows / 64));
     for (int p = 0; p < gp.n_paths; ++p) {
         s.parts[p] = parts;
         s.first[p + 1] = s.first[p] + tiles(p) * parts;
@@ -130,11 +130,15 @@ GpSplit simt_split(const GpProblem& gp, int64_t rows, int sms) {
 // The workspace of a weight gradient: the CTAs' first positions, then their partial tiles.
 size_t positions_bytes(const GpProblem& gp, const GpSplit& split) { return ((size_t)split.first[gp.n_paths] * sizeof(int64_t) + 255) / 256 * 256; }
 
-template <class T>
-int join(const GpProblem& gp, const GpSplit& split, int tile, int64_t rows, int64_t groups, const int64_t* offsets, void* dW, const void* ws, cudaStream_t st) {
-    const dim3 grid((unsigned)((gp.w_numel + 255) / 256), (unsigned)std::min<int64_t>(groups, 1024));
-    oeq_grouped_join<T><<<grid, 256, 0, st>>>(gp, split, (const long long*)offsets, rows, (int)groups, tile, tile,
-                                              (const typename GpAcc<T>::type*)((const char*)ws + positions_bytes(gp, split)), (const long long*)ws, (T*)dW);
+template <class T, int TILE>
+int join(const GpProblem& gp, const GpSplit& split, int64_t rows, int64_t groups, const int64_t* offsets, void* dW, const void* ws, cudaStream_t st) {
+    int tiles = 0;
+    for (int p = 0; p < gp.n_paths; ++p) tiles += (split.first[p + 1] - split.first[p]) / split.parts[p];
+    int slices = 1;                     // some dozen CTAs for every SM: most find a complete group and leave
+    while (slices < TILE / 4 && (int64_t)slices * tiles * groups < 4096) slices *= 2;
+    const dim3 grid((unsigned)(slices * tiles), (unsigned)std::min<int64_t>(groups, 1024));
+    oeq_grouped_join<T, TILE><<<grid, 256, 0, st>>>(gp, split, (const long long*)offsets, rows, (int)groups, slices,
+                                                    (const typename GpAcc<T>::type*)((const char*)ws + positions_bytes(gp, split)), (const long long*)ws, (T*)dW);
     OEQ_CUDA(cudaGetLastError());
     return OEQ_OK;
 }
@@ -149,7 +153,7 @@ int simt_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* 
                                                                                 (const long long*)offsets, rows, (int)groups, (T*)dW,
                                                                                 (typename GpAcc<T>::type*)((char*)ws + positions_bytes(gp, split)), (long long*)ws);
     OEQ_CUDA(cudaGetLastError());
-    return join<T>(gp, split, GP_TILE, rows, groups, offsets, dW, ws, st);
+    return join<T, GP_TILE>(gp, split, rows, groups, offsets, dW, ws, st);
 }
 
 // ---- tensor cores
@@ -248,7 +252,7 @@ GpSplit tc_split(const GpProblem& gp, int64_t rows, int sms) {
     for (;;) {
         int most = -1;
         for (int p = 0; p < gp.n_paths; ++p)
-            if (s.parts[p] < rows && (most < 0 || cost[p] / s.parts[p] > cost[most] / s.parts[most])) most = p;
+            if (s.parts[p] < std::min<int64_t>(rows, GP_PARTS) && (most < 0 || cost[p] / s.parts[p] > cost[most] / s.parts[most])) most = p;
         if (most < 0 || ctas + tiles[most] > sms) break;
         ++s.parts[most];
         ctas += tiles[most];
@@ -280,7 +284,7 @@ int tc_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* X,
         oeq_grouped_tc_dw<T, false><<<gd.split.first[gp.n_paths], GD_THREADS, GD_SMEM, st>>>(gd, args);
     }
     OEQ_CUDA(cudaGetLastError());
-    return join<T>(gp, gd.split, GD_TILE, rows, groups, offsets, dW, ws, st);
+    return join<T, GD_TILE>(gp, gd.split, rows, groups, offsets, dW, ws, st);
 }
 
 int check_call(const oeq_grouped* h, int dtype, int64_t rows, int64_t groups) {
