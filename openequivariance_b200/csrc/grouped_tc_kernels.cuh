@@ -26,7 +26,7 @@ namespace oeq {
 constexpr int GT_D_MAX = 7;
 constexpr int GT_SETS = 2, GT_SET = 8, GT_PW = GT_SETS * GT_SET, GT_EPI_GROUPS = 2, GT_EPI = 4 * GT_EPI_GROUPS, GT_THREADS = (GT_PW + GT_EPI + 1) * 32;
 constexpr int GT_STAGES = 6;                    // most stages of A
-constexpr int GT_STAGING = 33 * 128 * 4;        // 32 channels of a tile's pairs, for each epilogue group
+constexpr int GT_STAGING = 42 * 100 * 4;        // 32 channels of a tile's pairs (three components take most), for each epilogue group
 constexpr int GT_CONTROL = 1536;                // barriers, rows of the tiles that drain, the CTA's range
 constexpr int ERR_GT_EMPTY = 81, ERR_GT_FULL = 82, ERR_GT_ACC_FULL = 83, ERR_GT_ACC_EMPTY = 84;
 
@@ -223,7 +223,7 @@ struct GtArgs {
     void* Z;
     long long rows;
     int groups;
-    int z_pair;                 // 4-byte pairs of 16-bit Z are aligned
+    int z_vec;                  // rows of Z in 16-byte pieces
 };
 struct GtBars {
     unsigned long long *full, *empty, *acc_full, *acc_empty;
@@ -242,7 +242,7 @@ struct GtBars {
 // ---------------------------------------------------------------------------- producers
 // A chunk of weights by the threads of a set, four pieces of 16 bytes of a lane on the way at once.
 template <class T, bool TRANS, bool FAST>
-__device__ __forceinline__ void gt_fill_b(unsigned char* dst, const T* __restrict__ w, int ld, int n, int n_left, int k_left, int k_fill, int member) {
+__device__ __forceinline__ void gt_fill_b(unsigned char* dst, const T* __restrict__ w, int ld, int n, int n_left, int k_left, int k_fill, float scale, int member) {
     constexpr int V = GtType<T>::V, AT_ONCE = 4;
     const int across = TRANS ? 8 : n / V, pieces = TRANS ? n * 8 : k_fill * across;     // K-major: (channel, piece of K); MN-major: (k, piece of channels)
     const unsigned magic = (65536 + across - 1) / across;       // i / across for i < 2048, across <= 32
@@ -262,7 +262,9 @@ __device__ __forceinline__ void gt_fill_b(unsigned char* dst, const T* __restric
             const int at = TRANS ? gt_place_k(row[j], c[j]) : gt_place_mn<T>(n, c[j] * V, row[j]);
             if constexpr (GtType<T>::SPLIT) {
                 float4 hi, lo;
-                gt_split(*reinterpret_cast<const float4*>(v[j]), hi, lo);
+                float4 x = *reinterpret_cast<const float4*>(v[j]);
+                x = make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale);        // (FP32 weights carry the scale; 16-bit ones would be rounded again)
+                gt_split(x, hi, lo);
                 *reinterpret_cast<float4*>(dst + at) = hi;
                 *reinterpret_cast<float4*>(dst + (TRANS ? at + n * 128 : gt_place_mn<T>(n, n + c[j] * V, row[j]))) = lo;
             } else {
@@ -277,7 +279,7 @@ __device__ __forceinline__ void gt_produce(const GtProblem& gt, const GtArgs& p,
                                            unsigned char* b_base, const GtBars& bars, GtWalk walk, int tid) {
     constexpr int V = GtType<T>::V, KC = GtType<T>::KC, KSTEP = GtType<T>::KSTEP, TILE_ROWS = gt_tile_rows(D), THREADS = GT_SET * 32;
     constexpr int PIECES = (TILE_ROWS * 8 + THREADS - 1) / THREADS;             // of V channels by D components, of a lane
-    const int set = tid / THREADS, member = tid % THREADS, lane = tid & 31, c = lane & 7, n = tile_of.n;
+    const int set = tid / THREADS, member = tid % THREADS, lane = tid & 31, c = lane & 7, r0 = member >> 3, n = tile_of.n;
     const bool resident = tile_of.chunks <= tile_of.slots;
     int it = 0, stage = 0, use = 0, slot = 0, have = -1;        // chunks so far; the group whose weights are in shared memory
     int turn = 0;                               // set that has the next chunk
@@ -290,7 +292,7 @@ __device__ __forceinline__ void gt_produce(const GtProblem& gt, const GtArgs& p,
         int row[PIECES];                        // (past the tile's rows: the last one again)
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int at = walk.pos + min((member + i * THREADS) >> 3, walk.rows - 1);
+            const int at = walk.pos + min(r0 + i * (THREADS / 8), walk.rows - 1);
             row[i] = p.order ? (int)__ldg(p.order + at) : at;
         }
         for (int path_no = to.path_begin; path_no < to.path_end; ++path_no) {
@@ -313,7 +315,7 @@ const T* x = static_cast<const T*>(p.X) + path.src_off + (u0 + V * c) * D;
                     unsigned char* a = a_base + stage * GtType<T>::A_BYTES;
 #pragma unroll
                     for (int i = 0; i < PIECES; ++i) {
-                        const int r = (member + i * THREADS) >> 3;
+                        const int r = r0 + i * (THREADS / 8);
                         if (r < walk.rows) {
 #pragma unroll
                             for (int k = 0; k < D; ++k) {
@@ -332,7 +334,7 @@ const T* x = static_cast<const T*>(p.X) + path.src_off + (u0 + V * c) * D;
                     }
                     if (load_b) {
                         const T* w = w_group + path.w_off + (TRANS ? (long long)n0 * path.w_ld + u0 : (long long)u0 * path.w_ld + n0);
-                        gt_fill_b<T, TRANS, FAST>(b_base + slot * GtType<T>::b_bytes(n), w, path.w_ld, n, to.mul - n0, left, k_fill, member);
+                        gt_fill_b<T, TRANS, FAST>(b_base + slot * GtType<T>::b_bytes(n), w, path.w_ld, n, to.mul - n0, left, k_fill, (float)to.scale, member);
                     }
                     fence_async_smem();
                     __syncwarp();
@@ -411,37 +413,44 @@ template <> struct GtPair<__half> {
     }
 };
 
-// Rows of a tile from shared memory, a warp a row (as pairs of 16-bit values half a warp), U rows on the way together.  Past the
-// tile's rows: the last one again, the same values to the same place.
-template <class T, int D, bool PAIRS, bool FULL>
-__device__ __forceinline__ void gt_write(const float* staging, const int* rows_of, int rows, T* __restrict__ z_col, int dim, int values, int warp, int lane) {
-    constexpr int ROWS = PAIRS ? 8 : 4, U = D == 1 ? 8 : 4, PITCH = 33 * D;
-    const int l = PAIRS ? 2 * (lane & 15) : lane;
+// The staged values of a tile's rows, [row][channel][component] of 32 channels: rows of 128 bytes whose 16-byte pieces are swizzled (one
+// component: a lane writes whole pieces), else rows with 16 bytes of padding (a lane writes single values; two lanes meet in a bank).
+template <int D> __host__ __device__ constexpr int gt_pitch() { return D == 1 ? 32 : 32 * D + 4; }
+template <int D> __device__ __forceinline__ int gt_staged(int r, int i) { return D == 1 ? r * 32 + ((i ^ (4 * (r & 7)))) : r * gt_pitch<D>() + i; }
+
+// Rows of a tile from shared memory by the 128 threads of a group.  VEC: 16 bytes a thread; U of them are on the way together, past the
+// last one the last one again (the same values to the same place).
+template <class T, int D, bool VEC>
+__device__ __forceinline__ void gt_write(const float* staging, const int* rows_of, int rows, T* __restrict__ z_col, int dim, int values, int thread) {
+    if constexpr (VEC) {
+        constexpr int V = 16 / sizeof(T), ROW = 32 * D / V, U = sizeof(T) == 4 ? 4 : 2;          // pieces of a row
+        const int pieces = rows * ROW;
 #pragma unroll 1
-    for (int r0 = PAIRS ? 2 * warp + (lane >> 4) : warp; r0 < rows; r0 += ROWS * U) {
-        const float* from[U];
-        T* z[U];
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const int r = min(r0 + ROWS * j, rows - 1);
-            from[j] = staging + r * PITCH + l;
-            z[j] = z_col + (long long)rows_of[r] * dim + l;
-        }
-#pragma unroll
-        for (int i = 0; i < D; ++i) {
-            float v[U], w[U];
+        for (int i0 = thread; i0 < pieces; i0 += U * 128) {
+            float4 v[U][V / 4];
+            T* z[U];
+            bool in[U];
 #pragma unroll
             for (int j = 0; j < U; ++j) {
-                v[j] = from[j][32 * i];
-                if constexpr (PAIRS) w[j] = from[j][32 * i + 1];
-            }
-            if (FULL || 32 * i + l < values) {
+                const int i = min(i0 + 128 * j, pieces - 1), r = i / ROW, c = (i - r * ROW) * V;
 #pragma unroll
-                for (int j = 0; j < U; ++j) {
-                    if constexpr (PAIRS) *reinterpret_cast<unsigned*>(z[j] + 32 * i) = GtPair<T>::of(v[j], w[j]);
-                    else gp_store(z[j] + 32 * i, v[j]);
-                }
+                for (int h = 0; h < V / 4; ++h) v[j][h] = *reinterpret_cast<const float4*>(staging + gt_staged<D>(r, c + 4 * h));
+                z[j] = z_col + (long long)rows_of[r] * dim + c;
+                in[j] = c < values;
             }
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                if (!in[j]) continue;
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(z[j]) = v[j][0];
+                else *reinterpret_cast<uint4*>(z[j]) = make_uint4(GtPair<T>::of(v[j][0].x, v[j][0].y), GtPair<T>::of(v[j][0].z, v[j][0].w),
+                                                                  GtPair<T>::of(v[j][1].x, v[j][1].y), GtPair<T>::of(v[j][1].z, v[j][1].w));
+            }
+        }
+    } else {
+        constexpr int ROW = 32 * D;
+        for (int i = thread; i < rows * ROW; i += 128) {
+            const int r = i / ROW, c = i - r * ROW;
+            if (c < values) gp_store(z_col + (long long)rows_of[r] * dim + c, staging[gt_staged<D>(r, c)]);
         }
     }
 }
@@ -464,7 +473,7 @@ __device__ __forceinline__ void gt_ahead(const GtProblem& gt, const GtArgs& p, c
 template <class T, bool TRANS, int D>
 __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, float* staging,
                                          const GtBars& bars, GtWalk walk, unsigned tmem, int group, int warp, int lane) {
-    constexpr int TILE_ROWS = gt_tile_rows(D), PITCH = 33 * D;
+    constexpr int TILE_ROWS = gt_tile_rows(D), PITCH = gt_pitch<D>();
     const int n = tile_of.n, mul = min(n, to.mul - n0), pair = warp * 32 + lane, r_of = pair / D, k_of = pair % D;
     const float scale = (float)to.scale;
     const unsigned quarter = tmem + ((unsigned)(warp * 32) << 16);
@@ -511,24 +520,27 @@ const bool last = w0 + 32 * GT_EPI_GROUPS >= mul;           // the group has rea
                     if (lane == 0) mbar_arrive(bars.acc_empty + buf);
                 }
                 if (w0 + 16 * h < n && r_of < walk.rows) {
+                    float s[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        float s = __uint_as_float(v[j]);
-                        if constexpr (GtType<T>::SPLIT) s += __uint_as_float(u[j]);
-                        to_smem[(16 * h + j) * D] = s * scale;
+                        if constexpr (GtType<T>::SPLIT) s[j] = __uint_as_float(v[j]) + __uint_as_float(u[j]);
+                        else s[j] = __uint_as_float(v[j]) * scale;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        if constexpr (D == 1) *reinterpret_cast<float4*>(staging + gt_staged<1>(r_of, 16 * h + j)) = make_float4(s[j], s[j + 1], s[j + 2], s[j + 3]);
+                        else {
+#pragma unroll
+                            for (int i = j; i < j + 4; ++i) to_smem[(16 * h + i) * D] = s[i];
+                        }
                     }
                 }
             }
             group_sync(1 + group, 128);
             const int values = min(32, mul - w0) * D;
             T* z = static_cast<T*>(p.Z) + to.off + (n0 + w0) * D;
-            if (sizeof(T) == 2 && p.z_pair && ((to.off | values) & 1) == 0) {
-                if (values == 32 * D) gt_write<T, D, true, true>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, warp, lane);
-                else gt_write<T, D, true, false>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, warp, lane);
-            } else {
-                if (values == 32 * D) gt_write<T, D, false, true>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, warp, lane);
-                else gt_write<T, D, false, false>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, warp, lane);
-            }
+            if (p.z_vec && (to.off | values) % (16 / (int)sizeof(T)) == 0) gt_write<T, D, true>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
+            else gt_write<T, D, false>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
             group_sync(1 + group, 128);
         }
         if (!mine) {

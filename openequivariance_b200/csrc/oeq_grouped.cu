@@ -222,7 +222,7 @@ int tc_product(const GpProblem& gp, int64_t rows, int64_t groups, const void* X,
     GtProblem gt{};
     if (int rc = tc_plan<T>(gp, rows, sms, gt, ctas, smem)) return rc;
     if (ctas == 0) return OEQ_OK;
-    const GtArgs args{X, W, (const long long*)order, (const long long*)offsets, Z, rows, (int)groups, aligned(Z, 4) && gp.dst_dim % 2 == 0};
+    const GtArgs args{X, W, (const long long*)order, (const long long*)offsets, Z, rows, (int)groups, aligned(Z, 16) && gp.dst_dim * sizeof(T) % 16 == 0};
     constexpr int V = 16 / sizeof(T);
     bool fast = aligned(X, 16) && aligned(W, 16) && gp.src_dim % V == 0 && gp.w_numel % V == 0;
     for (int p = 0; p < gp.n_paths; ++p) fast &= gp.path[p].src_off % V == 0 && gp.path[p].src_mul % V == 0 && gp.path[p].w_off % V == 0 && gp.path[p].w_ld % V == 0;
