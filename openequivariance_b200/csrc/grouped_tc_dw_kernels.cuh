@@ -13,6 +13,7 @@
 //     MMAs take 192): FP32 hi.hi and hi.lo as one, lo.hi into hi.lo's columns;
 //   * 8 warps add the accumulators to sums in shared memory at the end of a group and after CHAIN slots: an MMA's additions are cut off, not
 //     rounded, and the error grows with the length of a chain (relative, one chain of 750 slots: 1e-5).  The two accumulators alternate.
+//   * 3 warps prefetch rows to L2, up to two units ahead of the MMAs.
 // A CTA has one tile of one path and a range of the sorted rows (gt_range); groups that go beyond the range leave a partial tile for
 // oeq_grouped_join.  Every wait is bounded.
 #pragma once
@@ -21,7 +22,7 @@
 namespace oeq {
 
 constexpr int GD_TILE = 128, GD_BUNDLE = 4, GD_SLOT = 16384, GD_RING = 2 * GD_BUNDLE, GD_SUMS = GD_TILE * GD_TILE * 4;
-constexpr int GD_PW = 16, GD_EPI = 8, GD_THREADS = (GD_PW + GD_EPI + 1) * 32;
+constexpr int GD_PW = 16, GD_EPI = 8, GD_THREADS = (GD_PW + GD_EPI + 1 + GT_AHEAD) * 32;
 constexpr int GD_SMEM = GD_RING * GD_SLOT + GD_SUMS + 1024;
 constexpr int ERR_GD_EMPTY = 91, ERR_GD_FULL = 92, ERR_GD_ACC_FULL = 93, ERR_GD_ACC_EMPTY = 94;
 
@@ -65,12 +66,14 @@ __device__ __forceinline__ unsigned long long gd_desc(unsigned addr, int blocks)
 struct GdBars {
     unsigned long long *full, *empty, *acc_full, *acc_empty;
     unsigned* tmem;
+    volatile int* progress;     // units whose MMAs are on their way
     __device__ explicit GdBars(unsigned char* control) {
         full = reinterpret_cast<unsigned long long*>(control);
         empty = full + 2;
         acc_full = empty + 2;
         acc_empty = acc_full + 2;
         tmem = reinterpret_cast<unsigned*>(acc_empty + 2);
+        progress = reinterpret_cast<volatile int*>(tmem + 1);
     }
 };
 
@@ -248,10 +251,23 @@ __device__ __forceinline__ void gd_multiply(const GdArgs& p, int d, int unit, in
             }
             tc_commit_if(leader, bars.empty + bundle);
         }
+        if (leader) *bars.progress = units + 1;
         if (ok && chain.ends) {
             tc_commit_if(leader, bars.acc_full + buf);
             ++accs;
         }
+    }
+}
+
+// ---------------------------------------------------------------------------- prefetch
+template <class T>
+__device__ __forceinline__ void gd_ahead(const GdArgs& p, const GpProblem& gp, const GpPath& path, const GpTarget& to, int d, int unit, int u0, int w0, int mu, int mw,
+                                         const GdBars& bars, GtWalk walk, int tid) {
+    for (int units = 0; walk.more(); walk.next(p.offsets, p.groups), ++units) {
+        walk.tile(unit);
+        if (!gt_follow(bars.progress, units, 2)) continue;
+        gt_prefetch_rows<T>(static_cast<const T*>(p.X) + path.src_off + u0 * d, gp.src_dim, mu * d, p.order, walk.pos, walk.rows, tid);
+        gt_prefetch_rows<T>(static_cast<const T*>(p.dZ) + to.off + w0 * d, gp.dst_dim, mw * d, p.order, walk.pos, walk.rows, tid);
     }
 }
 
@@ -343,6 +359,7 @@ __global__ void __launch_bounds__(GD_THREADS, 1) oeq_grouped_tc_dw(const __grid_
             mbar_init(bars.acc_full + i, 1);
             mbar_init(bars.acc_empty + i, GD_EPI);
         }
+        *bars.progress = 0;
         fence_mbar_init();
     }
     if (warp == MMA_WARP) {
@@ -356,7 +373,9 @@ __global__ void __launch_bounds__(GD_THREADS, 1) oeq_grouped_tc_dw(const __grid_
     const long long lo = range.lo, hi = range.hi;
     if (tid == 0) p.lo[blockIdx.x] = lo;
     const GtWalk walk(p.offsets, range.g, (int)lo, (int)hi);
-    if (warp == MMA_WARP) {
+    if (warp > MMA_WARP) {
+        gd_ahead<T>(p, gd.gp, path, to, d, gd_unit<T>(d), u0, w0, mu, mw, bars, walk, tid - (MMA_WARP + 1) * 32);
+    } else if (warp == MMA_WARP) {
         gd_multiply<T>(p, d, gd_unit<T>(d), n, gt_smem, bars, walk, tmem, elect_lane());
     } else if (warp >= GD_PW) {
         gd_sum<T>(p, gd.gp, path, to, d, gd_unit<T>(d), u0, w0, mu, mw, n, bars, sums, walk, tmem, warp - GD_PW, lane);

@@ -6,15 +6,18 @@
 // As a matrix product: M = (row, component) pairs of sorted rows of one group, N = channels of one output block, K = channels of
 // the input blocks with its irrep.  A CTA has one output block (or a tile of its channels) and one range of the sorted rows, the
 // CTAs being dealt to the output blocks by cost, so a CTA meets few groups and keeps a group's weights in shared memory.
-//   * 16 producer warps: a lane reads the 16 d bytes of V = 4 (16-bit types: 8) channels of a row, [channel][component], and writes
+//   * 12 producer warps: a lane reads the 16 d bytes of V = 4 (16-bit types: 8) channels of a row, [channel][component], and writes
 //     d pieces of 16 bytes, one per (row, component), K-major with the 128-byte swizzle.  The transposition that the layout of irreps
 //     asks for costs no extra pass, rows are gathered in sorted order, and FP32 values are split into TF32 hi and lo on the way.
-//     Two sets of eight warps take the chunks of K in turn: each has its chunk on the way in registers before it waits for a stage.
+//     Three sets of four warps take the chunks of K in turn: each has its chunk on the way in registers before it waits for a stage, and the
+//     time of a load, some 2 000 cycles, passes once for three chunks.  (With fewer stages than sets the sets wait for their stages one after
+//     the other, by a barrier that goes round: a set that waited out of turn could not tell a stage's phases apart.)
 //     Weights have their output channels along memory: "MN-major" tiles for Z, K-major for dX; neither is transposed.
 //   * one warp, in step, issues the MMAs.  FP32: hi.hi and hi.lo as one MMA over the weights' hi channels followed by lo, lo.hi
 //     into hi.lo's columns: the large and the small products have accumulators of their own.
-//   * 8 epilogue warps, in two groups, add those, scale, and write rows through shared memory, so that a row's values leave in order.  They
-//     also prefetch the weights of the tile after next to L2.  (Its rows too: 184 us instead of 149 for 100 000 rows of 128x(0e+1o+2e) BF16.)
+//   * 8 epilogue warps, in two groups, add those, scale, and write rows through shared memory, so that a row's values leave in order.
+//   * 3 warps prefetch rows and weights to L2, up to two tiles ahead of the MMAs: a producer's loads are half of its time, and registers for
+//     more of them on the way there are none.
 // Two accumulators: a tile drains while the next is computed.  Every wait is bounded; on expiry a role records a code and all
 // leave.
 #pragma once
@@ -24,11 +27,11 @@
 namespace oeq {
 
 constexpr int GT_D_MAX = 7;
-constexpr int GT_SETS = 2, GT_SET = 8, GT_PW = GT_SETS * GT_SET, GT_EPI_GROUPS = 2, GT_EPI = 4 * GT_EPI_GROUPS, GT_THREADS = (GT_PW + GT_EPI + 1) * 32;
+constexpr int GT_SETS = 3, GT_SET = 4, GT_PW = GT_SETS * GT_SET, GT_EPI_GROUPS = 2, GT_EPI = 4 * GT_EPI_GROUPS, GT_AHEAD = 3, GT_THREADS = (GT_PW + GT_EPI + 1 + GT_AHEAD) * 32;
 constexpr int GT_STAGES = 6;                    // most stages of A
 constexpr int GT_STAGING = 42 * 100 * 4;        // 32 channels of a tile's pairs (three components take most), for each epilogue group
 constexpr int GT_CONTROL = 1536;                // barriers, rows of the tiles that drain, the CTA's range
-constexpr int ERR_GT_EMPTY = 81, ERR_GT_FULL = 82, ERR_GT_ACC_FULL = 83, ERR_GT_ACC_EMPTY = 84;
+constexpr int ERR_GT_EMPTY = 81, ERR_GT_FULL = 82, ERR_GT_ACC_FULL = 83, ERR_GT_ACC_EMPTY = 84, ERR_GT_TURN = 85;
 
 // Set by a kernel whose bounded wait ran out; read by oeq_grouped_check.
 __device__ int gt_status;
@@ -45,7 +48,8 @@ struct GtProblem {
     GtTarget target[GP_BLOCKS];
 };
 
-__host__ __device__ constexpr int gt_tile_rows(int d) { return 128 / d; }        // rows of a tile
+// Rows of a tile.  Seven components: 16 rows (112 of 128 pairs) are one piece for every lane of a set, 18 would be two.
+__host__ __device__ constexpr int gt_tile_rows(int d) { return d == 7 ? 16 : 128 / d; }
 
 template <class T> struct GtType {              // 16-bit
     static constexpr int V = 8, KC = 64, KSTEP = 16, A_BYTES = 16384, N_MAX = 256;
@@ -226,15 +230,18 @@ struct GtArgs {
     int z_vec;                  // rows of Z in 16-byte pieces
 };
 struct GtBars {
-    unsigned long long *full, *empty, *acc_full, *acc_empty;
+    unsigned long long *full, *empty, *acc_full, *acc_empty, *turn;
     unsigned* tmem;
+    volatile int* progress;     // tiles whose MMAs are on their way
     int* rows;                  // of the tile that drains, for each epilogue group
     __device__ explicit GtBars(unsigned char* control) {
         full = reinterpret_cast<unsigned long long*>(control);
         empty = full + GT_STAGES;
         acc_full = empty + GT_STAGES;
         acc_empty = acc_full + 2;
-        tmem = reinterpret_cast<unsigned*>(acc_empty + 2);
+        turn = acc_empty + 2;
+        tmem = reinterpret_cast<unsigned*>(turn + GT_SETS);
+        progress = reinterpret_cast<volatile int*>(tmem + 1);
         rows = reinterpret_cast<int*>(control + 512);      // (behind the range)
     }
 };
@@ -280,7 +287,7 @@ __device__ __forceinline__ void gt_produce(const GtProblem& gt, const GtArgs& p,
     constexpr int V = GtType<T>::V, KC = GtType<T>::KC, KSTEP = GtType<T>::KSTEP, TILE_ROWS = gt_tile_rows(D), THREADS = GT_SET * 32;
     constexpr int PIECES = (TILE_ROWS * 8 + THREADS - 1) / THREADS;             // of V channels by D components, of a lane
     const int set = tid / THREADS, member = tid % THREADS, lane = tid & 31, c = lane & 7, r0 = member >> 3, n = tile_of.n;
-    const bool resident = tile_of.chunks <= tile_of.slots;
+    const bool resident = tile_of.chunks <= tile_of.slots, in_turn = tile_of.stages < GT_SETS;
     int it = 0, stage = 0, use = 0, slot = 0, have = -1;        // chunks so far; the group whose weights are in shared memory
     int turn = 0;                               // set that has the next chunk
     for (; walk.more(); walk.next(p.offsets, p.groups)) {
@@ -305,6 +312,7 @@ const T* x = static_cast<const T*>(p.X) + path.src_off + (u0 + V * c) * D;
 #pragma unroll
                     for (int i = 0; i < PIECES; ++i) gt_read<T, D, FAST>(v[i], x + (long long)row[i] * gt.gp.src_dim, left - V * c);
                     bool ok = true;
+                    if (in_turn && it > 0) ok = warp_wait(ok, bars.turn + set, (unsigned)(it / GT_SETS - (set == 0)) & 1, &gt_status, ERR_GT_TURN);
                     if (use > 0) ok = warp_wait(ok, bars.empty + stage, (unsigned)(use - 1) & 1, &gt_status, ERR_GT_EMPTY);
                     if (load_b) {
                         const int last = it - (resident ? tile_of.chunks : tile_of.slots);      // the chunk that used the slot before
@@ -312,6 +320,7 @@ const T* x = static_cast<const T*>(p.X) + path.src_off + (u0 + V * c) * D;
                             ok = warp_wait(ok, bars.empty + last % tile_of.stages, (unsigned)(last / tile_of.stages) & 1, &gt_status, ERR_GT_EMPTY);
                     }
                     if (!ok) return;
+                    if (in_turn && lane == 0) mbar_arrive(bars.turn + (set + 1) % GT_SETS);
                     unsigned char* a = a_base + stage * GtType<T>::A_BYTES;
 #pragma unroll
                     for (int i = 0; i < PIECES; ++i) {
@@ -395,6 +404,7 @@ __device__ __forceinline__ void gt_multiply(const GtProblem& gt, const GtArgs& p
         }
         if (!ok) return;
         tc_commit_if(leader, bars.acc_full + buf);
+        if (leader) *bars.progress = tiles + 1;
     }
 }
 
@@ -455,20 +465,63 @@ __device__ __forceinline__ void gt_write(const float* staging, const int* rows_o
     }
 }
 
+// ---------------------------------------------------------------------------- prefetch
 __device__ __forceinline__ void gt_prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-// The weights of a group to L2 by the epilogue warps.
+// `len` values of sorted rows [pos, pos + rows), from `base` on in each: 1 << lp lanes a row, four rows' numbers on the way together.
+template <class T>
+__device__ __forceinline__ void gt_prefetch_rows(const T* base, int dim, int len, const long long* __restrict__ order, int pos, int rows, int tid) {
+    constexpr int LINE = 128 / sizeof(T), U = 4;
+    int lp = 0;
+    while (lp < 3 && (LINE << lp) < len) ++lp;
+    const int step = GT_AHEAD * 32 >> lp, i0 = (tid & ((1 << lp) - 1)) * LINE;
+    for (int r0 = tid >> lp; r0 < rows; r0 += U * step) {
+        int row[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int at = pos + min(r0 + j * step, rows - 1);
+            row[j] = order ? (int)__ldg(order + at) : at;
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            if (r0 + j * step < rows)
+                for (int i = i0; i < len; i += LINE << lp) gt_prefetch(base + (long long)row[j] * dim + i);
+    }
+}
+// Waits until `progress` is at least `least`, after a while no longer.  Whether work `item` is still ahead: what is late is left out.
+// (Nothing depends on what a prefetch does.)
+__device__ __forceinline__ bool gt_follow(volatile int* progress, int item, int distance) {
+    int now = 0;
+    for (int i = 0; i < 1 << 14; ++i) {
+        now = __shfl_sync(0xffffffffu, *progress, 0);
+        if (now >= item - distance) break;
+        __nanosleep(100);
+    }
+    return now < item;
+}
 template <class T, bool TRANS>
-__device__ __forceinline__ void gt_ahead(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, int g, int tid) {
-    constexpr int LINE = 128 / sizeof(T), THREADS = GT_EPI * 32;
-    for (int path_no = to.path_begin; path_no < to.path_end; ++path_no) {
-        const GpPath& path = gt.gp.path[path_no];
-        const int n = min(tile_of.n, to.mul - n0), rows = TRANS ? n : path.src_mul, len = TRANS ? path.src_mul : n;
-        const T* w = static_cast<const T*>(p.W) + (long long)g * gt.gp.w_numel + path.w_off + (TRANS ? (long long)n0 * path.w_ld : n0);
-        for (int r = tid >> 2; r < rows; r += THREADS / 4)
-            for (int i = (tid & 3) * LINE; i < len; i += 4 * LINE) gt_prefetch(w + (long long)r * path.w_ld + i);
+__device__ __forceinline__ void gt_ahead(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, const GtBars& bars, GtWalk walk,
+                                         int tile_rows, int tid) {
+    constexpr int LINE = 128 / sizeof(T), THREADS = GT_AHEAD * 32;
+    int have = -1, tiles = 0;
+    for (; walk.more(); walk.next(p.offsets, p.groups), ++tiles) {
+        walk.tile(tile_rows);
+        if (!gt_follow(bars.progress, tiles, 2)) continue;
+        for (int path_no = to.path_begin; path_no < to.path_end; ++path_no) {
+            const GpPath& path = gt.gp.path[path_no];
+            if (walk.g != have) {               // weights
+                const int n = min(tile_of.n, to.mul - n0), rows = TRANS ? n : path.src_mul, len = TRANS ? path.src_mul : n;
+                const T* w = static_cast<const T*>(p.W) + (long long)walk.g * gt.gp.w_numel + path.w_off + (TRANS ? (long long)n0 * path.w_ld : n0);
+                for (int r = tid >> 2; r < rows; r += THREADS / 4)
+                    for (int i = (tid & 3) * LINE; i < len; i += 4 * LINE) gt_prefetch(w + (long long)r * path.w_ld + i);
+            }
+            if (n0 == 0)                        // (the CTAs of an output block's other channels read the same rows)
+                gt_prefetch_rows<T>(static_cast<const T*>(p.X) + path.src_off, gt.gp.src_dim, path.src_mul * to.d, p.order, walk.pos, walk.rows, tid);
+        }
+        have = walk.g;
     }
 }
 
+// ---------------------------------------------------------------------------- epilogue
 // The chunks of 32 channels of all tiles go to the two groups of four warps in turn.
 template <class T, bool TRANS, int D>
 __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, float* staging,
@@ -479,24 +532,11 @@ __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, c
     const unsigned quarter = tmem + ((unsigned)(warp * 32) << 16);
     int* rows_of = bars.rows + 128 * group;
     staging += group * (GT_STAGING / 4);
-    GtWalk ahead = walk;
-    int have = -1;
-    auto prefetch = [&]() {
-        if (ahead.more()) {
-            ahead.tile(TILE_ROWS);
-            if (ahead.g != have) gt_ahead<T, TRANS>(gt, p, tile_of, to, n0, ahead.g, group * 128 + pair);
-            have = ahead.g;
-            ahead.next(p.offsets, p.groups);
-        }
-    };
-    prefetch();
-    prefetch();
     int tiles = 0, turn = 0;
     for (; walk.more(); walk.next(p.offsets, p.groups), ++tiles) {
         walk.tile(TILE_ROWS);
         const int buf = tiles & 1;
         if (pair < walk.rows) rows_of[pair] = (int)gp_row(p.order, walk.pos + pair);         // (read behind the first barrier below)
-        prefetch();
         if (!warp_wait(true, bars.acc_full + buf, (unsigned)(tiles / 2) & 1, &gt_status, ERR_GT_ACC_FULL)) return;
         tc_fence_after();
         bool mine = false;
@@ -583,6 +623,8 @@ __global__ void __launch_bounds__(GT_THREADS, 1) oeq_grouped_tc(const __grid_con
             mbar_init(bars.acc_full + i, 1);
             mbar_init(bars.acc_empty + i, GT_EPI);
         }
+        for (int i = 0; i < GT_SETS; ++i) mbar_init(bars.turn + i, GT_SET);
+        *bars.progress = 0;
         fence_mbar_init();
     }
     constexpr int MMA_WARP = GT_PW + GT_EPI;
@@ -597,7 +639,8 @@ __global__ void __launch_bounds__(GT_THREADS, 1) oeq_grouped_tc(const __grid_con
     tc_fence_after();
     const unsigned tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile unsigned*>(bars.tmem), 0);
     const GtWalk walk(p.offsets, range.g, work ? (int)range.lo : 0, work ? (int)range.hi : 0);
-    if (warp == MMA_WARP) gt_multiply<T, TRANS>(gt, p, tile_of, to, a_base, b_base, bars, walk, gt_tile_rows(d), tmem, elect_lane());
+    if (warp > MMA_WARP) gt_ahead<T, TRANS>(gt, p, tile_of, to, n0, bars, walk, gt_tile_rows(d), tid - (MMA_WARP + 1) * 32);
+    else if (warp == MMA_WARP) gt_multiply<T, TRANS>(gt, p, tile_of, to, a_base, b_base, bars, walk, gt_tile_rows(d), tmem, elect_lane());
     else if (d == 1) gt_roles<T, TRANS, FAST, 1>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
     else if (d == 3) gt_roles<T, TRANS, FAST, 3>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
     else if (d == 5) gt_roles<T, TRANS, FAST, 5>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
