@@ -1,4 +1,5 @@
-// Linear maps of irreps with one set of weights for each group of rows, on the FMA units: every type, every degree.
+// Linear maps of irreps with one set of weights for each group of rows, on the FMA units (FP64: the FP64 tensor
+// units): every type, every degree.
 //
 //   Z[r,o,w,k] = c_o sum_{i,u} W_g[i,o][u,w] X[r,i,u,k],  g = group of row r          (product; dX with W transposed)
 //   dW_g[i,o][u,w] = c_o sum_{r in g, k} X[r,i,u,k] dZ[r,o,w,k]                        (weight gradient)
@@ -59,29 +60,54 @@ __device__ __forceinline__ long long gp_row(const long long* __restrict__ order,
 
 // The grouped rows are cut into `parts` equal ranges of sorted positions.
 __device__ __forceinline__ long long gp_cut(long long n, int part, int parts) { return (long long)((unsigned long long)n * part / parts); }
-// Staged rows are two values longer than a tile: 16 steps by two rows, which a warp writes, lie in different banks (16 in one: 120 us instead of
-// 45 for 10 007 rows of 64x(0e+1o+2e) FP64).
-constexpr int GP_TILE = 64, GP_PITCH = GP_TILE + 2, GP_STEP = 16, GP_SIMT_THREADS = 256;
-
-template <class A> struct alignas(2 * sizeof(A)) GpTwo { A x, y; };
-// acc[4][4] += a[k][row] b[k][col] over GP_STEP staged steps
-template <class A>
-__device__ __forceinline__ void gp_multiply(const A (*a)[GP_PITCH], const A (*b)[GP_PITCH], int r0, int c0, A (&acc)[4][4]) {
+constexpr int GP_TILE = 64, GP_STEP = 16, GP_SIMT_THREADS = 256;
+// A 64 x 64 product by 256 threads, 16 values each, over GP_STEP staged steps.  PITCH of a staged step: 16 steps by two rows, which a warp
+// writes, and what it reads lie in different banks (a pitch of 64: 120 us instead of 102 for 10 007 rows of 64x(0e+1o+2e) FP64).
+template <class A> struct GpProduct {           // FMA: 4 rows by 4 columns of a thread
+    static constexpr int PITCH = GP_TILE + 2;
+    A acc[16] = {};
+    static __device__ int row(int i) { return threadIdx.x / 16 * 4 + (i >> 2); }
+    static __device__ int col(int i) { return threadIdx.x % 16 * 4 + (i & 3); }
+    __device__ void multiply(const A (*a)[PITCH], const A (*b)[PITCH]) {
 #pragma unroll
-    for (int k = 0; k < GP_STEP; ++k) {
-        A x[4], y[4];
+        for (int k = 0; k < GP_STEP; ++k) {
+            A x[4], y[4];
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {        // (r0, c0 and the pitch are even)
-            const GpTwo<A> p = *reinterpret_cast<const GpTwo<A>*>(&a[k][r0 + i]), q = *reinterpret_cast<const GpTwo<A>*>(&b[k][c0 + i]);
-            x[i] = p.x; x[i + 1] = p.y;
-            y[i] = q.x; y[i + 1] = q.y;
+            for (int i = 0; i < 4; ++i) {
+                x[i] = a[k][row(4 * i)];
+                y[i] = b[k][col(i)];
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[i] += x[i >> 2] * y[i & 3];
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] += x[i] * y[j];
     }
-}
+};
+// FP64: mma.m8n8k4, rounded as FMAs are; a warp has 16 rows by 32 columns, six values to read for eight products of 8 x 8 x 4 where the FMAs
+// of a thread read eight for sixteen.
+template <> struct GpProduct<double> {
+    static constexpr int PITCH = GP_TILE + 10;
+    double acc[16] = {};
+    static __device__ int row(int i) { return (threadIdx.x >> 6) * 16 + (i >> 3) * 8 + (threadIdx.x & 31) / 4; }
+    static __device__ int col(int i) { return (threadIdx.x >> 5 & 1) * 32 + (i >> 1 & 3) * 8 + 2 * (threadIdx.x & 3) + (i & 1); }
+    __device__ void multiply(const double (*a)[PITCH], const double (*b)[PITCH]) {
+        const int k0 = threadIdx.x & 3, m0 = row(0), n0 = (threadIdx.x >> 5 & 1) * 32 + (threadIdx.x & 31) / 4;
+#pragma unroll
+        for (int k = 0; k < GP_STEP; k += 4) {
+            double x[2], y[4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) x[i] = a[k + k0][m0 + 8 * i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = b[k + k0][n0 + 8 * j];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    double* c = acc + 8 * i + 2 * j;
+                    asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};" : "+d"(c[0]), "+d"(c[1]) : "d"(x[i]), "d"(y[j]));
+                }
+        }
+    }
+};
 
 // ---------------------------------------------------------------------------- product
 // CTA (x, y): entry x of the block table and column y; a column is a target block, 64 of its channels and 64 of the block's up
@@ -92,7 +118,7 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt(const __grid
                                                                     const int* __restrict__ table, int blocks, long long rows, int groups,
                                                                     T* __restrict__ Z) {
     typedef typename GpAcc<T>::type A;
-    __shared__ __align__(16) A sa[GP_STEP][GP_PITCH], sb[GP_STEP][GP_PITCH];
+    __shared__ __align__(16) A sa[GP_STEP][GpProduct<A>::PITCH], sb[GP_STEP][GpProduct<A>::PITCH];
     const int tid = threadIdx.x;
     if ((int)blockIdx.x >= blocks) {            // rows without a group: zeros
         const long long n = min(__ldg(offsets + groups), rows), part = (long long)(blockIdx.x - blocks) * gridDim.y + blockIdx.y;
@@ -123,8 +149,8 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt(const __grid
     }
     const T* w_group = W + (long long)g * gp.w_numel;
     const int kb = gp.transposed ? tid % GP_STEP : tid / 16 % GP_STEP, cb = gp.transposed ? tid / GP_STEP : tid % 16;
-    A acc[4][4] = {}, a[4], b[4];
-    const int r0 = tid / 16 * 4, c0 = tid % 16 * 4;
+    GpProduct<A> product;
+    A a[4], b[4];
     int p = to.path_begin, u0 = 0;
     auto fetch = [&]() {
         const GpPath& path = gp.path[p];
@@ -153,16 +179,13 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt(const __grid
         __syncthreads();
         more = p < to.path_end;
         if (more) fetch();
-        gp_multiply(sa, sb, r0, c0, acc);
+        product.multiply(sa, sb);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int pair = pair0 + r0 + i;
-        if (pair >= pairs) break;
-        T* z = Z + gp_row(order, first + pair / d) * gp.dst_dim + to.off + pair % d;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (c_tile + c0 + j < to.mul) gp_store(z + (c_tile + c0 + j) * d, (A)(acc[i][j] * (A)to.scale));
+    for (int i = 0; i < 16; ++i) {
+        const int pair = pair0 + product.row(i), c = c_tile + product.col(i);
+        if (pair >= pairs || c >= to.mul) continue;
+        gp_store(Z + gp_row(order, first + pair / d) * gp.dst_dim + to.off + pair % d + c * d, (A)(product.acc[i] * (A)to.scale));
     }
 }
 
@@ -182,7 +205,7 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __g
                                                                        long long rows, int groups, T* __restrict__ dW,
                                                                        typename GpAcc<T>::type* __restrict__ partial, long long* __restrict__ lo_of) {
     typedef typename GpAcc<T>::type A;
-    __shared__ __align__(16) A sa[GP_STEP][GP_PITCH], sb[GP_STEP][GP_PITCH];
+    __shared__ __align__(16) A sa[GP_STEP][GpProduct<A>::PITCH], sb[GP_STEP][GpProduct<A>::PITCH];
     const int tid = threadIdx.x;
     int p = 0;
     while ((int)blockIdx.x >= split.first[p + 1]) ++p;
@@ -193,7 +216,7 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __g
     const long long n = min(__ldg(offsets + groups), rows), lo = gp_cut(n, part, parts), hi = gp_cut(n, part + 1, parts);
     if (tid == 0) lo_of[blockIdx.x] = lo;
     if (lo >= hi) return;
-    const int k_s = tid / 16, c_s = tid % 16, r0 = tid / 16 * 4, c0 = tid % 16 * 4;
+    const int k_s = tid / 16, c_s = tid % 16;
     int g = gp_group(offsets, groups, lo);
     for (long long at = lo; at < hi;) {
         long long begin = __ldg(offsets + g), end = __ldg(offsets + g + 1);
@@ -203,7 +226,8 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __g
         }
         const long long stop = min(end, hi);
         const long long pairs = (stop - at) * d;
-        A acc[4][4] = {}, a[4], b[4];
+        GpProduct<A> product;
+        A a[4], b[4];
         auto fetch = [&](long long k0) {
             const long long k = k0 + k_s;
             const bool in = k < pairs;
@@ -226,19 +250,16 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __g
             }
             __syncthreads();
             if (k0 + GP_STEP < pairs) fetch(k0 + GP_STEP);
-            gp_multiply(sa, sb, r0, c0, acc);
+            product.multiply(sa, sb);
         }
         const bool whole = begin >= lo && end <= hi;
         A* tile = whole ? nullptr : partial + ((long long)blockIdx.x * 2 + (begin < lo ? 0 : 1)) * (GP_TILE * GP_TILE);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int u = u_tile + r0 + i, w = w_tile + c0 + j;
-                if (!whole) tile[(r0 + i) * GP_TILE + c0 + j] = acc[i][j];
-                else if (u < path.src_mul && w < to.mul)
-                    gp_store(dW + (long long)g * gp.w_numel + path.w_off + (long long)u * path.w_ld + w, (A)(acc[i][j] * (A)to.scale));
-            }
+        for (int i = 0; i < 16; ++i) {
+            const int r = product.row(i), c = product.col(i), u = u_tile + r, w = w_tile + c;
+            if (!whole) tile[r * GP_TILE + c] = product.acc[i];
+            else if (u < path.src_mul && w < to.mul) gp_store(dW + (long long)g * gp.w_numel + path.w_off + (long long)u * path.w_ld + w, (A)(product.acc[i] * (A)to.scale));
+        }
         at = stop;
         ++g;
     }
