@@ -78,7 +78,7 @@ struct Runs {
     int runs;
 };
 Runs runs_of(int64_t rows) {
-    const int64_t run = std::max<int64_t>(256, ((rows + 1183) / 1184 + 31) / 32 * 32);
+    const int64_t run = std::max<int64_t>(256, ((rows + RG_RUNS - 1) / RG_RUNS + 31) / 32 * 32);
     return {run, (int)std::max<int64_t>(1, (rows + run - 1) / run)};
 }
 
@@ -162,6 +162,7 @@ int simt_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* 
 template <class T>
 int tc_plan(const GpProblem& gp, int64_t rows, int sms, GtProblem& gt, int& ctas, size_t& smem) {
     gt.gp = gp;
+    const size_t fixed = GT_CONTROL + GT_EPI_GROUPS * GT_STAGING, room = SMEM_MOST - fixed;
     double cost[GP_BLOCKS] = {};
     ctas = 0;
     for (int t = 0; t < gp.n_targets; ++t) {
@@ -169,15 +170,25 @@ int tc_plan(const GpProblem& gp, int64_t rows, int sms, GtProblem& gt, int& ctas
         GtTarget& x = gt.target[t];
         x = {};
         if (to.mul == 0) continue;
-        x.n_tiles = (to.mul + GtType<T>::N_MAX - 1) / GtType<T>::N_MAX;
-        x.n = ((to.mul + x.n_tiles - 1) / x.n_tiles + 15) / 16 * 16;
-        x.n_tiles = (to.mul + x.n - 1) / x.n;
         x.parts = 1;
         int k = 0;
         for (int p = to.path_begin; p < to.path_end; ++p) {
             k += gp.path[p].src_mul;
             x.chunks += (gp.path[p].src_mul + GtType<T>::KC - 1) / GtType<T>::KC;
         }
+        // Channels of a tile.  Every tile reads the rows again, and a tile whose weights do not stay in shared memory fills them in again for
+        // every 128 pairs: n / 128 of the work that the rows are.
+        double least = 0;
+        for (int most = GtType<T>::N_MAX; most >= GtType<T>::N_MAX / 4; most /= 2) {
+            const int tiles = (to.mul + most - 1) / most, n = ((to.mul + tiles - 1) / tiles + 15) / 16 * 16;
+            const bool stays = 2 * (size_t)GtType<T>::A_BYTES + (size_t)x.chunks * GtType<T>::b_bytes(n) <= room;
+            const double work = ((to.mul + n - 1) / n) * (1.0 + (stays ? 0.0 : n / 128.0));
+            if (x.n == 0 || work < least) {
+                x.n = n;
+                least = work;
+            }
+        }
+        x.n_tiles = (to.mul + x.n - 1) / x.n;
         x.extra = 96 / to.d;
         cost[t] = to.d * (double)(k + x.n + 32);
         ctas += x.n_tiles;
@@ -190,7 +201,6 @@ int tc_plan(const GpProblem& gp, int64_t rows, int sms, GtProblem& gt, int& ctas
         ++gt.target[most].parts;
         ctas += gt.target[most].n_tiles;
     }
-    const size_t fixed = GT_CONTROL + GT_EPI_GROUPS * GT_STAGING, room = SMEM_MOST - fixed;
     smem = 0;
     ctas = 0;
     for (int t = 0; t < gp.n_targets; ++t) {

@@ -15,7 +15,7 @@
 namespace oeq {
 
 constexpr int RG_BLOCK = 64;                    // rows of an entry of the block table
-constexpr int RG_SMALL_WARPS = 32, RG_WARPS = 4;
+constexpr int RG_SMALL_WARPS = 32, RG_WARPS = 4, RG_RUNS = 1184;           // most runs: eight warps an SM
 
 __device__ __forceinline__ int rg_key(const long long* __restrict__ index, long long r, int groups) {
     const long long g = index[r];
@@ -91,13 +91,14 @@ __device__ __forceinline__ void rg_tables(const int* offsets, int* first, int* p
 template <class F>
 __device__ __forceinline__ void rg_walk(const long long* __restrict__ index, long long lo, long long hi, int groups, int* count, F&& visit) {
     const int lane = threadIdx.x & 31;
-    constexpr int AHEAD = 4;                    // rows of a lane whose keys are loaded together
+    constexpr int AHEAD = 9;                    // rows of a lane whose keys are loaded together
     for (long long r0 = lo; r0 < hi; r0 += 32 * AHEAD) {
         int key[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) key[i] = r0 + 32 * i + lane < hi ? rg_key(index, r0 + 32 * i + lane, groups) : -1;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
+            if (r0 + 32 * i >= hi) break;
             const unsigned same = __match_any_sync(0xffffffffu, key[i]), lower = same & ((1u << lane) - 1);
             const int before = key[i] >= 0 ? count[key[i]] : 0;
             __syncwarp();
@@ -161,24 +162,22 @@ __global__ void __launch_bounds__(1024) oeq_row_groups_scan(int* __restrict__ co
     __shared__ int sums[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = blockIdx.x * 32 + lane;
     const int each = (runs + 31) / 32, lo = min(warp * each, runs), hi = min(lo + each, runs);
+    int c[RG_RUNS / 32];                        // all on the way at once
+#pragma unroll
+    for (int i = 0; i < RG_RUNS / 32; ++i) c[i] = lo + i < hi && k < keys ? counts[(long long)(lo + i) * keys + k] : 0;
     int s = 0;
-    if (k < keys) {
-#pragma unroll 8
-        for (int n = lo; n < hi; ++n) s += counts[(long long)n * keys + k];
-    }
+#pragma unroll
+    for (int i = 0; i < RG_RUNS / 32; ++i) s += c[i];
     sums[warp][lane] = s;
     __syncthreads();
     int before = 0;
     for (int w = 0; w < warp; ++w) before += sums[w][lane];
-    if (k < keys) {
-#pragma unroll 8
-        for (int n = lo; n < hi; ++n) {
-            const int c = counts[(long long)n * keys + k];
-            counts[(long long)n * keys + k] = before;
-            before += c;
-        }
-        if (warp == 31) totals[k] = before;
+#pragma unroll
+    for (int i = 0; i < RG_RUNS / 32; ++i) {
+        if (lo + i < hi && k < keys) counts[(long long)(lo + i) * keys + k] = before;
+        before += c[i];
     }
+    if (warp == 31 && k < keys) totals[k] = before;
 }
 
 // Shared memory: [RG_WARPS][groups + 1] counts, [groups + 2] offsets, [groups + 2] blocks, 33 ints
