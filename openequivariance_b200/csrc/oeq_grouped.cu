@@ -70,9 +70,10 @@ int check_groups(int64_t rows, int64_t groups) {
 // ---------------------------------------------------------------------------- row groups
 size_t table_smem(int64_t groups) { return (2 * (groups + 2) + 33) * sizeof(int); }
 size_t walk_smem(int64_t groups) { return RG_WARPS * (groups + 1) * sizeof(int); }
-size_t small_smem(int64_t groups) { return RG_SMALL_WARPS * (groups + 1) * sizeof(int) + table_smem(groups); }
-// One CTA walks 32 rows a step in each of its warps; beyond these many rows the runs of many CTAs are faster.
-bool small_groups(int64_t rows, int64_t groups) { return rows <= 8192 && small_smem(groups) <= SMEM_MOST; }
+size_t small_smem(int64_t groups) { return (RG_SMALL_WARPS + 1) * (groups + 1) * sizeof(int) + table_smem(groups); }
+// A cluster's warps walk 32 rows a step each; beyond these many rows the runs of many CTAs are faster (89 groups, cluster / runs: 50 000 rows
+// 17 / 20 us, 262 144 rows 41 / 21).
+bool small_groups(int64_t rows, int64_t groups) { return rows <= 65536 && small_smem(groups) <= SMEM_MOST; }
 struct Runs {
     int64_t run;        // rows of a run
     int runs;
@@ -157,10 +158,13 @@ int simt_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* 
 }
 
 // ---- tensor cores
-// The CTAs, one for each SM, are dealt to the tiles of channels by the time that a range of rows takes: for every (row, component) pair
-// the channels read and written and a fixed part.
+// The time of a group's weights, in (row, component) pairs.
+constexpr int GROUP_PAIRS = 96;
+// The CTAs, one for each SM, are dealt to the tiles of channels by the time that they take: for every (row, component) pair, and for
+// those that a group's weights count for, the channels read and written and a fixed part.  (By the rows alone 4 999 rows in 89
+// groups take 58 us: an output of scalars, with as many weights as the others, has a ninth of the CTAs.)
 template <class T>
-int tc_plan(const GpProblem& gp, int64_t rows, int sms, GtProblem& gt, int& ctas, size_t& smem) {
+int tc_plan(const GpProblem& gp, int64_t rows, int64_t groups, int sms, GtProblem& gt, int& ctas, size_t& smem) {
     gt.gp = gp;
     const size_t fixed = GT_CONTROL + GT_EPI_GROUPS * GT_STAGING, room = SMEM_MOST - fixed;
     double cost[GP_BLOCKS] = {};
@@ -189,8 +193,8 @@ int tc_plan(const GpProblem& gp, int64_t rows, int sms, GtProblem& gt, int& ctas
             }
         }
         x.n_tiles = (to.mul + x.n - 1) / x.n;
-        x.extra = 96 / to.d;
-        cost[t] = to.d * (double)(k + x.n + 32);
+        x.extra = GROUP_PAIRS / to.d;
+        cost[t] = ((double)rows * to.d + (double)std::min(rows, groups) * GROUP_PAIRS) * (k + x.n + 32);
         ctas += x.n_tiles;
     }
     for (;;) {                          // the tile whose ranges take longest gets another CTA
@@ -230,7 +234,7 @@ int tc_product(const GpProblem& gp, int64_t rows, int64_t groups, const void* X,
     size_t smem = 0;
     if (int rc = sm_count(sms)) return rc;
     GtProblem gt{};
-    if (int rc = tc_plan<T>(gp, rows, sms, gt, ctas, smem)) return rc;
+    if (int rc = tc_plan<T>(gp, rows, groups, sms, gt, ctas, smem)) return rc;
     if (ctas == 0) return OEQ_OK;
     const GtArgs args{X, W, (const long long*)order, (const long long*)offsets, Z, rows, (int)groups, aligned(Z, 16) && gp.dst_dim * sizeof(T) % 16 == 0};
     constexpr int V = 16 / sizeof(T);
@@ -248,14 +252,14 @@ int tc_product(const GpProblem& gp, int64_t rows, int64_t groups, const void* X,
 }
 
 // CTAs of the tiles of the weight gradient, one for each SM, dealt by the time that a range of rows takes.
-GpSplit tc_split(const GpProblem& gp, int64_t rows, int sms) {
+GpSplit tc_split(const GpProblem& gp, int64_t rows, int64_t groups, int sms) {
     GpSplit s{};
     int tiles[GP_PATHS], ctas = 0;
     double cost[GP_PATHS];
     for (int p = 0; p < gp.n_paths; ++p) {
         const GpTarget& to = gp.target[gp.path[p].dst];
         tiles[p] = (gp.path[p].src_mul + GD_TILE - 1) / GD_TILE * ((to.mul + GD_TILE - 1) / GD_TILE);
-        cost[p] = to.d * (double)(std::min(GD_TILE, gp.path[p].src_mul) + std::min(GD_TILE, to.mul) + 64);
+        cost[p] = ((double)rows * to.d + (double)std::min(rows, groups) * GROUP_PAIRS) * (std::min(GD_TILE, gp.path[p].src_mul) + std::min(GD_TILE, to.mul) + 64);
         s.parts[p] = 1;
         ctas += tiles[p];
     }
@@ -276,8 +280,8 @@ int tc_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* X,
                cudaStream_t st) {
     int sms = 0;
     if (int rc = sm_count(sms)) return rc;
-    GdProblem gd{gp, tc_split(gp, rows, sms), {}};
-    for (int p = 0; p < gp.n_paths; ++p) gd.extra[p] = 96 / gp.target[gp.path[p].dst].d;
+    GdProblem gd{gp, tc_split(gp, rows, groups, sms), {}};
+    for (int p = 0; p < gp.n_paths; ++p) gd.extra[p] = GROUP_PAIRS / gp.target[gp.path[p].dst].d;
     const GdArgs args{X, dZ, (const long long*)order, (const long long*)offsets, dW, (float*)((char*)ws + positions_bytes(gp, gd.split)), (long long*)ws, rows, (int)groups,
                       aligned(dW, 16) && gp.w_numel * sizeof(T) % 16 == 0};
     constexpr int V = 16 / sizeof(T);
@@ -345,8 +349,21 @@ int oeq_row_groups(int64_t rows, int64_t groups, const int64_t* index, int64_t* 
     long long *ord = (long long*)order, *slt = (long long*)slots, *off = (long long*)offsets;
     if (small_groups(rows, groups)) {
         const size_t smem = small_smem(groups);
-        if (int rc = allow_smem<oeq_row_groups_small>(SMEM_MOST)) return rc;
-        oeq_row_groups_small<<<1, 32 * RG_SMALL_WARPS, smem, st>>>(in, (int)rows, (int)groups, n, ord, slt, off, blocks);
+        if (int rc = allow_smem<oeq_row_groups_cluster>(SMEM_MOST)) return rc;
+        int ctas = 1;                   // two steps of a warp as long as there are CTAs for that
+        while (ctas < 8 && rows > (int64_t)ctas * 64 * RG_SMALL_WARPS) ctas *= 2;
+        cudaLaunchAttribute cluster;
+        cluster.id = cudaLaunchAttributeClusterDimension;
+        cluster.val.clusterDim.x = (unsigned)ctas;
+        cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3((unsigned)ctas);
+        config.blockDim = dim3(32 * RG_SMALL_WARPS);
+        config.dynamicSmemBytes = smem;
+        config.stream = st;
+        config.attrs = &cluster;
+        config.numAttrs = 1;
+        OEQ_CUDA(cudaLaunchKernelEx(&config, oeq_row_groups_cluster, in, (int)rows, (int)groups, n, ord, slt, off, (int*)blocks));
     } else {
         const Runs r = runs_of(rows);
         int *counts = (int*)workspace, *totals = counts + (size_t)r.runs * keys;
@@ -356,7 +373,7 @@ int oeq_row_groups(int64_t rows, int64_t groups, const int64_t* index, int64_t* 
         if (int rc = allow_smem<oeq_row_groups_place>(walk_smem(OEQ_MOST_GROUPS) + table_smem(OEQ_MOST_GROUPS))) return rc;
         oeq_row_groups_count<<<ctas, 32 * RG_WARPS, smem, st>>>(in, rows, r.run, r.runs, (int)groups, counts);
         OEQ_CUDA(cudaGetLastError());
-        oeq_row_groups_scan<<<(unsigned)((keys + 31) / 32), 1024, 0, st>>>(counts, totals, r.runs, keys);
+        oeq_row_groups_scan<<<(unsigned)((keys + 7) / 8), 1024, 0, st>>>(counts, totals, r.runs, keys);
         OEQ_CUDA(cudaGetLastError());
         oeq_row_groups_place<<<ctas, 32 * RG_WARPS, smem_place, st>>>(in, rows, r.run, r.runs, (int)groups, n, counts, totals, ord, slt, off, blocks);
     }
@@ -463,7 +480,7 @@ size_t oeq_grouped_workspace_bytes(const oeq_grouped* h, int dtype, int64_t rows
     if (!h || rows < 0 || !known_dtype(dtype) || h->weights.n_paths == 0 || sm_count(sms)) return 0;
     const GpProblem& gp = h->weights;
     const bool tc = dtype != OEQ_F64 && h->d_max <= GT_D_MAX;
-    const GpSplit s = tc ? tc_split(gp, rows, sms) : simt_split(gp, rows, sms);
+    const GpSplit s = tc ? tc_split(gp, rows, groups, sms) : simt_split(gp, rows, sms);
     const size_t tile = tc ? GD_TILE * GD_TILE * sizeof(float) : GP_TILE * GP_TILE * std::max<size_t>(4, elem_bytes(dtype));
     return positions_bytes(gp, s) + (size_t)s.first[gp.n_paths] * 2 * tile;
 }

@@ -4,12 +4,15 @@
 //   order[p] = the row at sorted position p, slots[r] = the position of row r, offsets[g] = rows of groups before g.
 //   Rows whose group is not in 0..groups-1 come last (key `groups`).
 //
-// A warp takes a run of rows, 32 at a time.  Lanes with the same key find each other (match_any): a row's rank is the number
-// of earlier rows of its key in the run, counted in shared memory, plus those of lower lanes, so equal keys keep their
-// order without atomics, and every result is the same in every run.
-//   * few rows: one CTA counts, scans and places in one launch (row_groups_small);
-//   * many rows: count (a histogram per run), scan (the runs' histograms, a key per lane), place (every CTA adds up the keys).
+// A warp takes a run of rows, 32 at a time.  Lanes with the same key find each other by a ballot for each bit of the keys (match_any
+// takes a round for each key that occurs: 0.6 us for 32 rows of 89 groups): a row's rank is the number of earlier rows of its key
+// in the run, counted in shared memory, plus those of lower lanes, so equal keys keep their order, and every result is the same in every run.
+//   * up to 262 144 rows: a cluster of up to eight CTAs counts, scans and places in one launch, the CTAs' counts read from one another's
+//     shared memory (row_groups_cluster);
+//   * more rows or many groups: count (a histogram per run), scan (the runs' histograms, a key per lane), place (every CTA adds up the keys).
 #pragma once
+#include <cooperative_groups.h>
+
 #include "oeq_common.cuh"
 
 namespace oeq {
@@ -87,42 +90,65 @@ __device__ __forceinline__ void rg_tables(const int* offsets, int* first, int* p
     }
 }
 
-// Rows [lo, hi) by one warp; visit(row, key, rank): rank among the rows of the key, count[] being what came before.
+constexpr int RG_AHEAD = 8;                     // rows of a lane whose keys are loaded together
 template <class F>
-__device__ __forceinline__ void rg_walk(const long long* __restrict__ index, long long lo, long long hi, int groups, int* count, F&& visit) {
+__device__ __forceinline__ void rg_rows(const long long* __restrict__ index, long long lo, long long hi, int groups, F&& rows) {
     const int lane = threadIdx.x & 31;
-    constexpr int AHEAD = 9;                    // rows of a lane whose keys are loaded together
-    for (long long r0 = lo; r0 < hi; r0 += 32 * AHEAD) {
-        int key[AHEAD];
+    for (long long r0 = lo; r0 < hi; r0 += 32 * RG_AHEAD) {
+        int key[RG_AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) key[i] = r0 + 32 * i + lane < hi ? rg_key(index, r0 + 32 * i + lane, groups) : -1;
+        for (int i = 0; i < RG_AHEAD; ++i) key[i] = r0 + 32 * i + lane < hi ? rg_key(index, r0 + 32 * i + lane, groups) : -1;
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
+        for (int i = 0; i < RG_AHEAD; ++i) {
             if (r0 + 32 * i >= hi) break;
-            const unsigned same = __match_any_sync(0xffffffffu, key[i]), lower = same & ((1u << lane) - 1);
-            const int before = key[i] >= 0 ? count[key[i]] : 0;
-            __syncwarp();
-            if (key[i] >= 0) {
-                visit(r0 + 32 * i + lane, key[i], before + __popc(lower));
-                if (lower == 0) count[key[i]] = before + __popc(same);
-            }
-            __syncwarp();
+            rows(r0 + 32 * i + lane, key[i]);
         }
     }
 }
+// Counts of the keys of rows [lo, hi) into the warp's count[].
+__device__ __forceinline__ void rg_count(const long long* __restrict__ index, long long lo, long long hi, int groups, int* count) {
+    rg_rows(index, lo, hi, groups, [&](long long, int key) {
+        if (key >= 0) atomicAdd(count + key, 1);
+    });
+    __syncwarp();
+}
+// visit(row, key, position) of rows [lo, hi), count[] being the position of the first row of each key.
+template <class F>
+__device__ __forceinline__ void rg_place(const long long* __restrict__ index, long long lo, long long hi, int groups, int* count, F&& visit) {
+    const int lane = threadIdx.x & 31, bits = 32 - __clz(groups);
+    rg_rows(index, lo, hi, groups, [&](long long r, int key) {
+        unsigned same = __ballot_sync(0xffffffffu, key >= 0);
+        for (int b = 0; b < bits; ++b) {
+            const unsigned set = __ballot_sync(0xffffffffu, key >> b & 1);
+            same &= key >> b & 1 ? set : ~set;
+        }
+        const unsigned lower = same & ((1u << lane) - 1);
+        const int before = key >= 0 ? count[key] : 0;
+        __syncwarp();
+        if (key >= 0) {
+            visit(r, key, before + __popc(lower));
+            if (lower == 0) count[key] = before + __popc(same);
+        }
+        __syncwarp();
+    });
+}
 
-// ---- one CTA.  Shared memory: [32 warps][groups + 1] counts, [groups + 2] offsets, [groups + 2] blocks, 33 ints
-__global__ void __launch_bounds__(32 * RG_SMALL_WARPS) oeq_row_groups_small(const long long* __restrict__ index, int rows, int groups, int blocks,
-                                                                              long long* __restrict__ order, long long* __restrict__ slots,
-                                                                              long long* __restrict__ offsets, int* __restrict__ table) {
+// ---- a cluster of CTAs.  Shared memory: [32 warps][groups + 1] counts, [groups + 1] totals of the CTA, [groups + 2] offsets, [groups + 2]
+// blocks, 33 ints
+__global__ void __launch_bounds__(32 * RG_SMALL_WARPS) oeq_row_groups_cluster(const long long* __restrict__ index, int rows, int groups, int blocks,
+                                                                                long long* __restrict__ order, long long* __restrict__ slots,
+                                                                                long long* __restrict__ offsets, int* __restrict__ table) {
     extern __shared__ int rg_smem[];
+    const auto cluster = cooperative_groups::this_cluster();
+    const int ctas = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
     const int keys = groups + 1, tid = threadIdx.x, warp = tid >> 5;
-    int *offs = rg_smem + RG_SMALL_WARPS * keys, *first = offs + keys + 1, *part = first + keys + 1;
+    int *totals = rg_smem + RG_SMALL_WARPS * keys, *offs = totals + keys, *first = offs + keys + 1, *part = first + keys + 1;
     for (int i = tid; i < RG_SMALL_WARPS * keys; i += blockDim.x) rg_smem[i] = 0;
     __syncthreads();
-    const int run = (rows + 32 * RG_SMALL_WARPS - 1) / (32 * RG_SMALL_WARPS) * 32, lo = min(warp * run, rows), hi = min(lo + run, rows);
+    const int run = (rows + 32 * RG_SMALL_WARPS * ctas - 1) / (32 * RG_SMALL_WARPS * ctas) * 32;
+    const int lo = (int)min((long long)(cta * RG_SMALL_WARPS + warp) * run, (long long)rows), hi = min(lo + run, rows);
     int* mine = rg_smem + warp * keys;
-    rg_walk(index, lo, hi, groups, mine, [](long long, int, int) {});
+    rg_count(index, lo, hi, groups, mine);
     __syncthreads();
     for (int k = tid; k < keys; k += blockDim.x) {          // warps' counts -> rows of the key in the warps before
         int s = 0;
@@ -131,16 +157,28 @@ __global__ void __launch_bounds__(32 * RG_SMALL_WARPS) oeq_row_groups_small(cons
             rg_smem[w * keys + k] = s;
             s += n;
         }
-        offs[k] = s;
+        totals[k] = s;
     }
-    __syncthreads();
+    cluster.sync();
+    for (int k = tid; k < keys; k += blockDim.x) {
+        int all = 0, before = 0;
+        for (int c = 0; c < ctas; ++c) {
+            const int n = *cluster.map_shared_rank(totals + k, c);
+            before += c < cta ? n : 0;
+            all += n;
+        }
+        offs[k] = all;
+        for (int w = 0; w < RG_SMALL_WARPS; ++w) rg_smem[w * keys + k] += before;
+    }
+    cluster.sync();                             // (a CTA's totals are read until here)
     rg_scan(offs, keys, part);
-    rg_walk(index, lo, hi, groups, mine, [&](long long r, int key, int rank) {
-        const int p = offs[key] + rank;
+    for (int k = tid & 31; k < keys; k += 32) mine[k] += offs[k];
+    __syncwarp();
+    rg_place(index, lo, hi, groups, mine, [&](long long r, int, int p) {
         order[p] = r;
         slots[r] = p;
     });
-    rg_tables(offs, first, part, groups, blocks, offsets, table, tid, blockDim.x);
+    rg_tables(offs, first, part, groups, blocks, offsets, table, (long long)cta * blockDim.x + tid, (long long)ctas * blockDim.x);
 }
 
 // ---- many rows: runs of `run` rows (a multiple of 32), one per warp; counts [runs][groups + 1], totals [groups + 1]
@@ -153,31 +191,49 @@ __global__ void __launch_bounds__(32 * RG_WARPS) oeq_row_groups_count(const long
     __syncwarp();
     if (n >= runs) return;
     const long long lo = n * run, hi = min(lo + run, rows);
-    rg_walk(index, lo, hi, groups, mine, [](long long, int, int) {});
+    rg_count(index, lo, hi, groups, mine);
     for (int k = lane; k < keys; k += 32) counts[(long long)n * keys + k] = mine[k];
 }
 
-// counts[n][k] -> rows of key k in the runs before n.  A CTA takes 32 keys, a warp every 32nd part of the runs.
+// counts[n][k] -> rows of key k in the runs before n.  A CTA takes eight keys, eight threads of each of 128 spans of the runs.
+// (32 keys and 32 spans a CTA: 13 us for 1 184 runs of 90 keys, three CTAs.)
 __global__ void __launch_bounds__(1024) oeq_row_groups_scan(int* __restrict__ counts, int* __restrict__ totals, int runs, int keys) {
-    __shared__ int sums[32][33];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = blockIdx.x * 32 + lane;
-    const int each = (runs + 31) / 32, lo = min(warp * each, runs), hi = min(lo + each, runs);
-    int c[RG_RUNS / 32];                        // all on the way at once
+    constexpr int SPANS = 128, EACH = (RG_RUNS + SPANS - 1) / SPANS;
+    __shared__ int sums[8][SPANS + 4];
+    const int key = threadIdx.x & 7, span = threadIdx.x >> 3, k = blockIdx.x * 8 + key, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int each = (runs + SPANS - 1) / SPANS, lo = min(span * each, runs), hi = min(lo + each, runs);
+    int c[EACH], s = 0;                         // all on the way at once
 #pragma unroll
-    for (int i = 0; i < RG_RUNS / 32; ++i) c[i] = lo + i < hi && k < keys ? counts[(long long)(lo + i) * keys + k] : 0;
-    int s = 0;
+    for (int i = 0; i < EACH; ++i) c[i] = lo + i < hi && k < keys ? counts[(long long)(lo + i) * keys + k] : 0;
 #pragma unroll
-    for (int i = 0; i < RG_RUNS / 32; ++i) s += c[i];
-    sums[warp][lane] = s;
+    for (int i = 0; i < EACH; ++i) s += c[i];
+    sums[key][span] = s;
     __syncthreads();
-    int before = 0;
-    for (int w = 0; w < warp; ++w) before += sums[w][lane];
+    if (warp < 8) {                             // spans of key `warp`, four a lane
+        int v[4], all = 0;
 #pragma unroll
-    for (int i = 0; i < RG_RUNS / 32; ++i) {
+        for (int i = 0; i < 4; ++i) {
+            v[i] = all;
+            all += sums[warp][4 * lane + i];
+        }
+        int up = all;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, up, off);
+            if (lane >= off) up += t;
+        }
+        if (lane == 31 && blockIdx.x * 8 + warp < keys) totals[blockIdx.x * 8 + warp] = up;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[warp][4 * lane + i] = up - all + v[i];
+    }
+    __syncthreads();
+    int before = sums[key][span];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
         if (lo + i < hi && k < keys) counts[(long long)(lo + i) * keys + k] = before;
         before += c[i];
     }
-    if (warp == 31 && k < keys) totals[k] = before;
 }
 
 // Shared memory: [RG_WARPS][groups + 1] counts, [groups + 2] offsets, [groups + 2] blocks, 33 ints
@@ -196,7 +252,7 @@ __global__ void __launch_bounds__(32 * RG_WARPS) oeq_row_groups_place(const long
         for (int k = lane; k < keys; k += 32) mine[k] = offs[k] + counts[(long long)n * keys + k];
         __syncwarp();
         const long long lo = n * run, hi = min(lo + run, rows);
-        rg_walk(index, lo, hi, groups, mine, [&](long long r, int, int p) {
+        rg_place(index, lo, hi, groups, mine, [&](long long r, int, int p) {
             order[p] = r;
             slots[r] = p;
         });
