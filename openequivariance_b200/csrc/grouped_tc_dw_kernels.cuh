@@ -6,7 +6,8 @@
 // M = 128 input channels u, N = up to 128 output channels w of one path, and the sum runs over rows and components.  Both operands have their
 // channels along memory, so both are "MN-major": a lane reads the 16 d bytes of V channels of a row and writes d pieces, one into
 // the slot of each component.  A slot has one component of GdType::ROWS sorted rows of one group, X and dZ, 16 KB; four of them are
-// a bundle, and there are two bundles.
+// a bundle, and there are two bundles (16-bit types of one component: four of two, which are filled by copies without registers, two of a
+// set on the way at once).
 //   * 16 producer warps.  One and three components: two sets of eight take units of rows in turn, each with a bundle of its own, a lane the same
 //     channels of X and dZ.  Five and seven: one set, half of it for X and half for dZ, the components of a unit in two bundles;
 //   * one warp, in step, issues the MMAs of a bundle, as many as there are between two waits (a wait for each slot: 575 cycles a slot, where its
@@ -21,7 +22,7 @@
 
 namespace oeq {
 
-constexpr int GD_TILE = 128, GD_BUNDLE = 4, GD_SLOT = 16384, GD_RING = 2 * GD_BUNDLE, GD_SUMS = GD_TILE * GD_TILE * 4;
+constexpr int GD_TILE = 128, GD_SLOT = 16384, GD_RING = 8, GD_BUNDLES = 4, GD_SUMS = GD_TILE * GD_TILE * 4;
 constexpr int GD_PW = 16, GD_EPI = 8, GD_THREADS = (GD_PW + GD_EPI + 1 + GT_AHEAD) * 32;
 constexpr int GD_SMEM = GD_RING * GD_SLOT + GD_SUMS + 1024;
 constexpr int ERR_GD_EMPTY = 91, ERR_GD_FULL = 92, ERR_GD_ACC_FULL = 93, ERR_GD_ACC_EMPTY = 94;
@@ -29,10 +30,12 @@ constexpr int ERR_GD_EMPTY = 91, ERR_GD_FULL = 92, ERR_GD_ACC_FULL = 93, ERR_GD_
 template <class T> struct GdType { static constexpr int ROWS = 32, CHAIN = 32; };
 template <> struct GdType<float> { static constexpr int ROWS = 8, CHAIN = 32; };
 __host__ __device__ constexpr int gd_sets(int d) { return d <= 3 ? 2 : 1; }     // of producers
+template <class T> __host__ __device__ constexpr int gd_bundles(int d) { return sizeof(T) == 2 && d == 1 ? 4 : 2; }
+template <class T> __host__ __device__ constexpr int gd_bundle(int d) { return GD_RING / gd_bundles<T>(d); }       // slots
 // rows of a unit: with one component a bundle of slots, else one slot of each component
-template <class T> __host__ __device__ constexpr int gd_unit(int d) { return d == 1 ? GD_BUNDLE * GdType<T>::ROWS : GdType<T>::ROWS; }
+template <class T> __host__ __device__ constexpr int gd_unit(int d) { return d == 1 ? gd_bundle<T>(d) * GdType<T>::ROWS : GdType<T>::ROWS; }
 // components of a unit's first bundle
-__host__ __device__ constexpr int gd_first(int d) { return d <= GD_BUNDLE ? d : (d + 1) / 2; }
+__host__ __device__ constexpr int gd_first(int d) { return d <= 4 ? d : (d + 1) / 2; }
 
 struct GdProblem {
     GpProblem gp;               // paths in the order of their weights
@@ -69,8 +72,8 @@ struct GdBars {
     volatile int* progress;     // units whose MMAs are on their way
     __device__ explicit GdBars(unsigned char* control) {
         full = reinterpret_cast<unsigned long long*>(control);
-        empty = full + 2;
-        acc_full = empty + 2;
+        empty = full + GD_BUNDLES;
+        acc_full = empty + GD_BUNDLES;
         acc_empty = acc_full + 2;
         tmem = reinterpret_cast<unsigned*>(acc_empty + 2);
         progress = reinterpret_cast<volatile int*>(tmem + 1);
@@ -120,7 +123,7 @@ template <class T, int D, bool FAST>
 __device__ __forceinline__ bool gd_fill(const GdArgs& p, const GpProblem& gp, const GtWalk& walk, const GdLane& l, const T* x, const T* z, int n, unsigned char* ring,
                                         const GdBars& bars, int bundle, int use) {
     constexpr bool BOTH = gd_sets(D) == 2;      // a lane reads both operands
-    constexpr int ROWS = GdType<T>::ROWS, THREADS = 256, PASS = D == 1 ? 4 : (sizeof(T) == 4 ? 1 : 2), FIRST = gd_first(D);
+    constexpr int ROWS = GdType<T>::ROWS, THREADS = 256, PASS = D == 1 ? 4 : (sizeof(T) == 4 ? 1 : 2), FIRST = gd_first(D), BUNDLE = gd_bundle<T>(D);
     const int rows = (walk.rows + ROWS - 1) / ROWS * ROWS, step = THREADS >> l.lp, blocks = (n + 63) / 64, lane = threadIdx.x & 31;
     const bool is_x = l.x_left > 0;
     auto free_again = [&](int b) { return use == 0 || warp_wait(true, bars.empty + b, (unsigned)(use - 1) & 1, &gt_status, ERR_GD_EMPTY); };
@@ -153,7 +156,7 @@ __device__ __forceinline__ bool gd_fill(const GdArgs& p, const GpProblem& gp, co
         auto place = [&](int j, bool of_x, unsigned char*& dst, int& lo) {
             const int q = l.r0 + q0 + j * step, r = q % ROWS;
             const int at = of_x ? gd_place<T>(l.ch, r, GD_TILE / 64) : 8192 + gd_place<T>(l.ch, r, blocks);
-            dst = ring + (bundle * GD_BUNDLE + q / ROWS * (D == 1)) * GD_SLOT + at;
+            dst = ring + (bundle * BUNDLE + q / ROWS * (D == 1)) * GD_SLOT + at;
             lo = of_x ? 4096 : 8192 + gd_place<T>(l.ch + n, r, 0) - at;
             return q < rows && (of_x ? l.x_left : l.z_left) > 0;
         };
@@ -175,13 +178,39 @@ __device__ __forceinline__ bool gd_fill(const GdArgs& p, const GpProblem& gp, co
             for (int j = 0; j < PASS; ++j) {
                 unsigned char* dst;
                 int lo;
-                if (place(j, is_x, dst, lo)) gd_put<T, D, FIRST, D>(v[j], dst + (1 - 2 * bundle) * (GD_BUNDLE * GD_SLOT), lo);
+                if (place(j, is_x, dst, lo)) gd_put<T, D, FIRST, D>(v[j], dst + (1 - 2 * bundle) * (BUNDLE * GD_SLOT), lo);
             }
         }
         waited = true;
     }
     filled(FIRST < D ? bundle ^ 1 : bundle);
     return true;
+}
+
+// A unit of one component of a 16-bit type: copies.  Rows behind the group's last are zeros.
+template <class T>
+__device__ __forceinline__ void gd_copy(const GdArgs& p, const GpProblem& gp, const GtWalk& walk, const GdLane& l, const T* x, const T* z, int n, unsigned char* dst) {
+    constexpr int ROWS = GdType<T>::ROWS, U = 4;
+    const int rows = (walk.rows + ROWS - 1) / ROWS * ROWS, step = 256 >> l.lp, blocks = (n + 63) / 64;
+#pragma unroll 1
+    for (int q0 = l.r0; q0 < rows; q0 += U * step) {
+        int row[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int at = walk.pos + min(q0 + j * step, walk.rows - 1);
+            row[j] = p.order ? (int)__ldg(p.order + at) : at;
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int q = q0 + j * step;
+            if (q >= rows) continue;
+            unsigned char* slot = dst + q / ROWS * GD_SLOT;
+            const bool in = q < walk.rows;
+            if (l.x_left > 0) gt_copy(slot + gd_place<T>(l.ch, q % ROWS, GD_TILE / 64), x + (long long)row[j] * gp.src_dim, in);
+            if (l.z_left > 0) gt_copy(slot + 8192 + gd_place<T>(l.ch, q % ROWS, blocks), z + (long long)row[j] * gp.dst_dim, in);
+        }
+    }
+    gt_copies_commit();
 }
 
 template <class T, bool FAST, int D>
@@ -197,15 +226,37 @@ __device__ __forceinline__ void gd_produce(const GdArgs& p, const GpProblem& gp,
     l.x_left = SETS == 2 || half == 0 ? mu - l.ch : 0;
     l.z_left = SETS == 2 || half == 1 ? mw - l.ch : 0;
     const T *x = static_cast<const T*>(p.X) + path.src_off + (u0 + l.ch) * D, *z = static_cast<const T*>(p.dZ) + to.off + (w0 + l.ch) * D;
+    constexpr int BUNDLES = gd_bundles<T>(D);
+    constexpr bool ASYNC = FAST && BUNDLES == 4;
+    int held = -1;                              // the bundle whose copies are on their way
+    auto hand_over = [&](bool all) {
+        if (held < 0) return;
+        if (all) gt_copies_wait<0>();
+        else gt_copies_wait<1>();
+        fence_async_smem();
+        __syncwarp();
+        if ((tid & 31) == 0) mbar_arrive(bars.full + held);
+        held = -1;
+    };
     int units = 0;
     for (; walk.more(); walk.next(p.offsets, p.groups), ++units) {
         walk.tile(UNIT);
-        if (SETS == 1) {
-            if (!gd_fill<T, D, FAST>(p, gp, walk, l, x, z, n, ring, bars, 0, units)) return;
-        } else if ((units & 1) == half) {
-            if (!gd_fill<T, D, FAST>(p, gp, walk, l, x, z, n, ring, bars, half, units >> 1)) return;
+        if (SETS == 2 && (units & 1) != half) continue;
+        const int bundle = SETS == 1 ? 0 : units % BUNDLES, use = SETS == 1 ? units : units / BUNDLES;
+        if constexpr (ASYNC) {
+            // a set that has to wait hands over first what it holds: the MMAs that it waits for may need it
+            if (use > 0 && !__all_sync(0xffffffffu, mbar_test(bars.empty + bundle, (unsigned)(use - 1) & 1))) {
+                hand_over(true);
+                if (!warp_wait(true, bars.empty + bundle, (unsigned)(use - 1) & 1, &gt_status, ERR_GD_EMPTY)) return;
+            }
+            gd_copy<T>(p, gp, walk, l, x, z, n, ring + bundle * gd_bundle<T>(D) * GD_SLOT);
+            hand_over(false);
+            held = bundle;
+        } else {
+            if (!gd_fill<T, D, FAST>(p, gp, walk, l, x, z, n, ring, bars, bundle, use)) return;
         }
     }
+    if constexpr (ASYNC) hand_over(true);
 }
 
 // ---------------------------------------------------------------------------- MMA
@@ -215,7 +266,7 @@ __device__ __forceinline__ void gd_multiply(const GdArgs& p, int d, int unit, in
     const int blocks = (n + 63) / 64;
     const unsigned wide = gt_idesc<T, false>(GtType<T>::acc(n)) | MN, narrow = gt_idesc<T, false>(n) | MN;
     const unsigned long long a0 = gd_desc<T>(smem_u32(ring), GD_TILE / 64), b0 = gd_desc<T>(smem_u32(ring) + 8192, blocks);
-    const int first = gd_first(d), bundles = first < d ? 2 : 1, sets = gd_sets(d);
+    const int first = gd_first(d), bundles = first < d ? 2 : 1, sets = gd_sets(d), turns = gd_bundles<T>(d), bundle_bytes = gd_bundle<T>(d) * GD_SLOT;
     GdChain<T> chain;
     int units = 0, accs = 0;
     unsigned accumulate = 0;
@@ -229,13 +280,13 @@ __device__ __forceinline__ void gd_multiply(const GdArgs& p, int d, int unit, in
         }
         const unsigned acc = tmem + (unsigned)(buf * 256);
         for (int i = 0; i < bundles && ok; ++i) {
-            const int bundle = sets == 2 ? units & 1 : i, n_slots = bundles == 1 ? slots : (i == 0 ? first : d - first);
-            ok = warp_wait(ok, bars.full + bundle, (unsigned)(sets == 2 ? units >> 1 : units) & 1, &gt_status, ERR_GD_FULL);
+            const int bundle = sets == 2 ? units % turns : i, n_slots = bundles == 1 ? slots : (i == 0 ? first : d - first);
+            ok = warp_wait(ok, bars.full + bundle, (unsigned)(sets == 2 ? units / turns : units) & 1, &gt_status, ERR_GD_FULL);
             if (!ok) break;
             tc_fence_after();
-            unsigned long long a = a0 + (unsigned long long)(bundle * (GD_BUNDLE * GD_SLOT >> 4)), b = b0 + (unsigned long long)(bundle * (GD_BUNDLE * GD_SLOT >> 4));
+            unsigned long long a = a0 + (unsigned long long)(bundle * (bundle_bytes >> 4)), b = b0 + (unsigned long long)(bundle * (bundle_bytes >> 4));
 #pragma unroll
-            for (int s = 0; s < GD_BUNDLE; ++s, a += GD_SLOT >> 4, b += GD_SLOT >> 4) {
+            for (int s = 0; s < 4; ++s, a += GD_SLOT >> 4, b += GD_SLOT >> 4) {
                 if (s >= n_slots) break;
                 if constexpr (GtType<T>::SPLIT) {
                     gt_mma<T>(leader, acc, a, b, wide, accumulate);
@@ -353,9 +404,11 @@ __global__ void __launch_bounds__(GD_THREADS, 1) oeq_grouped_tc_dw(const __grid_
     GtRange& range = *reinterpret_cast<GtRange*>(control + 512);
     constexpr int MMA_WARP = GD_PW + GD_EPI;
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < GD_BUNDLES; ++i) {
             mbar_init(bars.full + i, GD_PW / gd_sets(d));
             mbar_init(bars.empty + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
             mbar_init(bars.acc_full + i, 1);
             mbar_init(bars.acc_empty + i, GD_EPI);
         }

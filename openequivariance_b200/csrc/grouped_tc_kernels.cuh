@@ -126,6 +126,12 @@ __device__ __forceinline__ void gt_read(uint4 (&v)[D], const T* __restrict__ src
             w[i] = (2 * i / D < left ? (unsigned)__ldg(h + 2 * i) : 0u) | ((2 * i + 1) / D < left ? (unsigned)__ldg(h + 2 * i + 1) << 16 : 0u);
     }
 }
+// 16 bytes to shared memory without a register on the way; zeros where !in.
+__device__ __forceinline__ void gt_copy(void* dst, const void* src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void gt_copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void gt_copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // Byte offset of 16-byte piece c of row `row` of a K-major tile (128-byte rows, 128-byte swizzle).
 __device__ __forceinline__ int gt_place_k(int row, int c) { return row * 128 + (((row ^ c) & 7) << 4); }
 // The V channels of component k.
@@ -253,6 +259,13 @@ __device__ __forceinline__ void gt_fill_b(unsigned char* dst, const T* __restric
     constexpr int V = GtType<T>::V, AT_ONCE = 4;
     const int across = TRANS ? 8 : n / V, pieces = TRANS ? n * 8 : k_fill * across;     // K-major: (channel, piece of K); MN-major: (k, piece of channels)
     const unsigned magic = (65536 + across - 1) / across;       // i / across for i < 2048, across <= 32
+    if constexpr (FAST && !GtType<T>::SPLIT) {  // (16-bit weights are copied as they are)
+        for (int i = member; i < pieces; i += GT_SET * 32) {
+            const int row = TRANS ? i >> 3 : (int)((i * magic) >> 16), c = TRANS ? i & 7 : i - row * across;
+            const bool in = TRANS ? row < n_left && c * V < k_left : row < k_left && c * V < n_left;
+            gt_copy(dst + (TRANS ? gt_place_k(row, c) : gt_place_mn<T>(n, c * V, row)), in ? w + (long long)row * ld + c * V : w, in);
+        }
+    } else
 #pragma unroll 1
     for (int i0 = member; i0 < pieces; i0 += AT_ONCE * GT_SET * 32) {
         uint4 v[AT_ONCE][1];
@@ -290,6 +303,20 @@ __device__ __forceinline__ void gt_produce(const GtProblem& gt, const GtArgs& p,
     const bool resident = tile_of.chunks <= tile_of.slots, in_turn = tile_of.stages < GT_SETS;
     int it = 0, stage = 0, use = 0, slot = 0, have = -1;        // chunks so far; the group whose weights are in shared memory
     int turn = 0;                               // set that has the next chunk
+    // One component of a 16-bit type goes to its stage as it is: copies without registers, two chunks of a set on the way at once.
+    constexpr bool ASYNC = FAST && !GtType<T>::SPLIT && D == 1;
+    int held = -1;                              // the stage of the chunk before, whose copies are on their way
+    auto arrive = [&](int at) {
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars.full + at);
+    };
+    auto hand_over = [&]() {
+        if (held < 0) return;
+        gt_copies_wait<0>();
+        arrive(held);
+        held = -1;
+    };
     for (; walk.more(); walk.next(p.offsets, p.groups)) {
         walk.tile(TILE_ROWS);
         const T* w_group = static_cast<const T*>(p.W) + (long long)walk.g * gt.gp.w_numel;
@@ -307,47 +334,73 @@ __device__ __forceinline__ void gt_produce(const GtProblem& gt, const GtArgs& p,
             for (int u0 = 0; u0 < path.src_mul; u0 += KC) {
                 if (turn == set) {
                     const int left = path.src_mul - u0, k_fill = left >= KC ? KC : (left + KSTEP - 1) / KSTEP * KSTEP;
+                    const T* x = static_cast<const T*>(p.X) + path.src_off + (u0 + V * c) * D;
                     uint4 v[PIECES][D];
-const T* x = static_cast<const T*>(p.X) + path.src_off + (u0 + V * c) * D;
+                    if constexpr (!ASYNC) {
 #pragma unroll
-                    for (int i = 0; i < PIECES; ++i) gt_read<T, D, FAST>(v[i], x + (long long)row[i] * gt.gp.src_dim, left - V * c);
+                        for (int i = 0; i < PIECES; ++i) gt_read<T, D, FAST>(v[i], x + (long long)row[i] * gt.gp.src_dim, left - V * c);
+                    }
                     bool ok = true;
+                    const int last = load_b ? it - (resident ? tile_of.chunks : tile_of.slots) : -1;     // the chunk that used the slot before
+                    const bool wait_b = last >= 0 && last > it - tile_of.stages;
+                    if constexpr (ASYNC) {
+                        // a set that has to wait hands over first what it holds: the MMAs that it waits for may need it
+                        bool now = use == 0 || mbar_test(bars.empty + stage, (unsigned)(use - 1) & 1);
+                        if (!__all_sync(0xffffffffu, now && !wait_b && !in_turn)) hand_over();
+                    }
                     if (in_turn && it > 0) ok = warp_wait(ok, bars.turn + set, (unsigned)(it / GT_SETS - (set == 0)) & 1, &gt_status, ERR_GT_TURN);
                     if (use > 0) ok = warp_wait(ok, bars.empty + stage, (unsigned)(use - 1) & 1, &gt_status, ERR_GT_EMPTY);
-                    if (load_b) {
-                        const int last = it - (resident ? tile_of.chunks : tile_of.slots);      // the chunk that used the slot before
-                        if (last >= 0 && last > it - tile_of.stages)
-                            ok = warp_wait(ok, bars.empty + last % tile_of.stages, (unsigned)(last / tile_of.stages) & 1, &gt_status, ERR_GT_EMPTY);
+                    if (wait_b) ok = warp_wait(ok, bars.empty + last % tile_of.stages, (unsigned)(last / tile_of.stages) & 1, &gt_status, ERR_GT_EMPTY);
+                    if (!ok) {
+                        if constexpr (!GtType<T>::SPLIT) gt_copies_wait<0>();
+                        return;
                     }
-                    if (!ok) return;
                     if (in_turn && lane == 0) mbar_arrive(bars.turn + (set + 1) % GT_SETS);
                     unsigned char* a = a_base + stage * GtType<T>::A_BYTES;
+                    const T* w = w_group + path.w_off + (TRANS ? (long long)n0 * path.w_ld + u0 : (long long)u0 * path.w_ld + n0);
+                    unsigned char* b = b_base + slot * GtType<T>::b_bytes(n);
+                    if constexpr (ASYNC) {
+                        if (load_b) gt_fill_b<T, TRANS, FAST>(b, w, path.w_ld, n, to.mul - n0, left, k_fill, (float)to.scale, member);
 #pragma unroll
-                    for (int i = 0; i < PIECES; ++i) {
-                        const int r = r0 + i * (THREADS / 8);
-                        if (r < walk.rows) {
+                        for (int i = 0; i < PIECES; ++i) {
+                            const bool in = left > V * c;
+                            gt_copy(a + gt_place_k(r0 + i * (THREADS / 8), c), in ? x + (long long)row[i] * gt.gp.src_dim : static_cast<const T*>(p.X), in);
+                        }
+                        gt_copies_commit();
+                        if (held >= 0) {
+                            gt_copies_wait<1>();
+                            arrive(held);
+                        }
+                        held = stage;
+                    } else {
 #pragma unroll
-                            for (int k = 0; k < D; ++k) {
-                                const uint4 piece = gt_component<T, D>(v[i], k);
-                                unsigned char* at = a + gt_place_k(r * D + k, c);
-                                if constexpr (GtType<T>::SPLIT) {
-                                    float4 hi, lo;
-                                    gt_split(*reinterpret_cast<const float4*>(&piece), hi, lo);
-                                    *reinterpret_cast<float4*>(at) = hi;
-                                    *reinterpret_cast<float4*>(at + 16384) = lo;
-                                } else {
-                                    *reinterpret_cast<uint4*>(at) = piece;
+                        for (int i = 0; i < PIECES; ++i) {
+                            const int r = r0 + i * (THREADS / 8);
+                            if (r < walk.rows) {
+#pragma unroll
+                                for (int k = 0; k < D; ++k) {
+                                    const uint4 piece = gt_component<T, D>(v[i], k);
+                                    unsigned char* at = a + gt_place_k(r * D + k, c);
+                                    if constexpr (GtType<T>::SPLIT) {
+                                        float4 hi, lo;
+                                        gt_split(*reinterpret_cast<const float4*>(&piece), hi, lo);
+                                        *reinterpret_cast<float4*>(at) = hi;
+                                        *reinterpret_cast<float4*>(at + 16384) = lo;
+                                    } else {
+                                        *reinterpret_cast<uint4*>(at) = piece;
+                                    }
                                 }
                             }
                         }
+                        if (load_b) {
+                            gt_fill_b<T, TRANS, FAST>(b, w, path.w_ld, n, to.mul - n0, left, k_fill, (float)to.scale, member);
+                            if constexpr (!GtType<T>::SPLIT) {
+                                gt_copies_commit();
+                                gt_copies_wait<0>();
+                            }
+                        }
+                        arrive(stage);
                     }
-                    if (load_b) {
-                        const T* w = w_group + path.w_off + (TRANS ? (long long)n0 * path.w_ld + u0 : (long long)u0 * path.w_ld + n0);
-                        gt_fill_b<T, TRANS, FAST>(b_base + slot * GtType<T>::b_bytes(n), w, path.w_ld, n, to.mul - n0, left, k_fill, (float)to.scale, member);
-                    }
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bars.full + stage);
                 }
                 if (++turn == GT_SETS) turn = 0;
                 ++it;
@@ -359,6 +412,7 @@ const T* x = static_cast<const T*>(p.X) + path.src_off + (u0 + V * c) * D;
             }
         }
     }
+    if constexpr (ASYNC) hand_over();
 }
 
 // ---------------------------------------------------------------------------- MMA
