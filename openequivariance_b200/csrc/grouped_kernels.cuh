@@ -194,6 +194,8 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt(const __grid
 // one that began before it goes to slot 0 of the CTA's two partial tiles, the part of one that goes on behind it to slot 1.
 // oeq_grouped_join adds the parts in the order of the ranges: no atomics, the same sums in every run.
 constexpr int GP_PARTS = 1024;                  // most ranges of a path
+// First sorted position of a CTA's range, and its group.
+struct GpStart { int lo, group; };
 struct GpSplit {
     int parts[GP_PATHS];        // ranges of each path
     int first[GP_PATHS + 1];    // its first CTA
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __g
                                                                        const T* __restrict__ X, const T* __restrict__ dZ,
                                                                        const long long* __restrict__ order, const long long* __restrict__ offsets,
                                                                        long long rows, int groups, T* __restrict__ dW,
-                                                                       typename GpAcc<T>::type* __restrict__ partial, long long* __restrict__ lo_of) {
+                                                                       typename GpAcc<T>::type* __restrict__ partial, GpStart* __restrict__ starts) {
     typedef typename GpAcc<T>::type A;
     __shared__ __align__(16) A sa[GP_STEP][GpProduct<A>::PITCH], sb[GP_STEP][GpProduct<A>::PITCH];
     const int tid = threadIdx.x;
@@ -214,10 +216,10 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __g
     const int parts = split.parts[p], part = ((int)blockIdx.x - split.first[p]) % parts, tile_of = ((int)blockIdx.x - split.first[p]) / parts;
     const int w_tiles = (to.mul + GP_TILE - 1) / GP_TILE, u_tile = tile_of / w_tiles * GP_TILE, w_tile = tile_of % w_tiles * GP_TILE, d = to.d;
     const long long n = min(__ldg(offsets + groups), rows), lo = gp_cut(n, part, parts), hi = gp_cut(n, part + 1, parts);
-    if (tid == 0) lo_of[blockIdx.x] = lo;
+    int g = lo < n ? gp_group(offsets, groups, lo) : 0;
+    if (tid == 0) starts[blockIdx.x] = {(int)lo, g};
     if (lo >= hi) return;
     const int k_s = tid / 16, c_s = tid % 16;
-    int g = gp_group(offsets, groups, lo);
     for (long long at = lo; at < hi;) {
         long long begin = __ldg(offsets + g), end = __ldg(offsets + g + 1);
         if (end <= at) {                        // (a group without rows)
@@ -265,69 +267,74 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __g
     }
 }
 
-// Gradients of the groups that no single range has: the sum of their parts, and zeros where there are no rows.
-// lo_of: first positions of the CTAs' ranges, ascending over the parts of a tile.  CTA (x, y): one of `slices` parts of a tile of
-// TILE x TILE weights, and every gridDim.y-th group.  (A thread for each weight and group, 65 536 x 512x0e to 512x0e BF16, 64 groups: 200 us,
-// most of it to find that a group is complete; by tiles 10.)
+// Gradients of the groups that no single range has, which are those with the first row of some range behind their own: a CTA for each
+// range and four rows of its tile.  The CTA of the first such range adds up the group's parts, 256 / TILE threads to four weights, in a fixed
+// order.  Behind them `zero_ctas` CTAs write the zeros of the groups without rows.  (A CTA for every tile and group takes 25 us for 89 groups
+// and three paths of 128 x 128, most of it to find that a group is complete.)
 template <class T, int TILE>
 __global__ void __launch_bounds__(256) oeq_grouped_join(const __grid_constant__ GpProblem gp, const __grid_constant__ GpSplit split,
-                                                        const long long* __restrict__ offsets, long long rows, int groups, int slices,
-                                                        const typename GpAcc<T>::type* __restrict__ partial, const long long* __restrict__ lo_of, T* __restrict__ dW) {
+                                                        const long long* __restrict__ offsets, long long rows, int groups, int zero_ctas,
+                                                        const typename GpAcc<T>::type* __restrict__ partial, const GpStart* __restrict__ starts, T* __restrict__ dW) {
     typedef typename GpAcc<T>::type A;
-    __shared__ int list[GP_PARTS + 1];          // ranges whose parts are added, and their number
-    const int slice = TILE / slices;
-    int p = 0, tile = blockIdx.x / slices;
-    for (;; ++p) {
-        const int tiles = (split.first[p + 1] - split.first[p]) / split.parts[p];
-        if (tile < tiles) break;
-        tile -= tiles;
+    constexpr int SLICE = 4, SLICES = TILE / SLICE, SHARES = 256 / TILE;
+    struct alignas(4 * sizeof(A)) Four { A v[4]; };
+    __shared__ int list[GP_PARTS + 2];          // partial tiles that are added, and their number
+    __shared__ Four sums[256];
+    const long long n = min(__ldg(offsets + groups), rows);
+    const int ctas = split.first[gp.n_paths];
+    if ((int)blockIdx.x >= ctas * SLICES) {
+        for (int g = blockIdx.x - ctas * SLICES; g < groups; g += zero_ctas)
+            if (min(__ldg(offsets + g), n) >= min(__ldg(offsets + g + 1), n))
+                for (int i = threadIdx.x; i < gp.w_numel; i += 256) gp_store(dW + (long long)g * gp.w_numel + i, A(0));
+        return;
     }
+    const int c = blockIdx.x / SLICES, u_slice = blockIdx.x % SLICES * SLICE;
+    int p = 0;
+    while (c >= split.first[p + 1]) ++p;
+    const int parts = split.parts[p], j = (c - split.first[p]) % parts, tile = (c - split.first[p]) / parts;
+    if (j == 0 || starts[c].lo >= n) return;
+    const int lo = starts[c].lo, g = starts[c].group;
+    const GpStart* of = starts + (c - j);       // of the tile's ranges
+    const int begin = (int)__ldg(offsets + g), end = (int)min(__ldg(offsets + g + 1), n);
+    if (begin >= lo || of[j - 1].lo > begin) return;        // no group goes on here, or an earlier range has seen to it
     const GpPath& path = gp.path[p];
     const GpTarget& to = gp.target[path.dst];
-    const int parts = split.parts[p], cta = split.first[p] + tile * parts, w_tiles = (to.mul + TILE - 1) / TILE;
-    const int u0 = tile / w_tiles * TILE + blockIdx.x % slices * slice, w0 = tile % w_tiles * TILE, nu = min(slice, path.src_mul - u0), nw = min(TILE, to.mul - w0);
+    const int w_tiles = (to.mul + TILE - 1) / TILE, u0 = tile / w_tiles * TILE + u_slice, w0 = tile % w_tiles * TILE, nu = min(SLICE, path.src_mul - u0), nw = min(TILE, to.mul - w0);
     if (nu <= 0) return;
-    const A* at = partial + (long long)cta * 2 * (TILE * TILE) + blockIdx.x % slices * slice * TILE;
-    const long long n = min(__ldg(offsets + groups), rows);
-    const A scale = (A)to.scale;
-    for (int g = blockIdx.y; g < groups; g += gridDim.y) {
-        const long long begin = min(__ldg(offsets + g), n), end = min(__ldg(offsets + g + 1), n);
-        int j0 = -1, j1 = -1;                   // the last ranges that begin at or before the group's first and last row
-        if (begin < end) {
-            for (int j = 0; j < parts; j += 256) {
-                const long long lo = j + threadIdx.x < parts ? __ldg(lo_of + cta + j + threadIdx.x) : n;
-                j0 += __syncthreads_count(lo <= begin);
-                j1 += __syncthreads_count(lo <= end - 1);
-            }
-            if (j0 == j1) continue;
-            if (threadIdx.x < 32) {             // (a range without rows has no part)
-                int count = 0;
-                for (int j = j0 + 1; j <= j1; j += 32) {
-                    const int k = j + threadIdx.x;
-                    const bool in = k <= j1 && (k == j1 || __ldg(lo_of + cta + k) < __ldg(lo_of + cta + k + 1));
-                    const unsigned all = __ballot_sync(0xffffffffu, in);
-                    if (in) list[count + __popc(all & ((1u << threadIdx.x) - 1))] = k;
-                    count += __popc(all);
-                }
-                if (threadIdx.x == 0) list[GP_PARTS] = count;
-            }
-            __syncthreads();
+    if (threadIdx.x < 32) {                     // the first range's part, then those of the others that have rows of the group
+        int count = 1;
+        if (threadIdx.x == 0) list[0] = 2 * (j - 1) + 1;
+        for (int i = j;; i += 32) {
+            const int k = i + threadIdx.x;
+            const bool in = k < parts && of[k].lo < end, some = in && (k + 1 == parts || of[k + 1].lo > of[k].lo);
+            const unsigned all = __ballot_sync(0xffffffffu, some);
+            if (some) list[count + __popc(all & ((1u << threadIdx.x) - 1))] = 2 * k;
+            count += __popc(all);
+            if (!__all_sync(0xffffffffu, in)) break;
         }
-        T* out = dW + (long long)g * gp.w_numel + path.w_off + (long long)u0 * path.w_ld + w0;
-        for (int i = threadIdx.x; i < nu * TILE; i += 256) {
-            const int u = i / TILE, w = i % TILE;
-            if (w >= nw) continue;
-            A s = A(0);
-            if (begin < end) {
-                s = at[(long long)(j0 * 2 + 1) * (TILE * TILE) + i];
-                const int count = list[GP_PARTS];
+        if (threadIdx.x == 0) list[GP_PARTS + 1] = count;
+    }
+    __syncthreads();
+    const int count = list[GP_PARTS + 1], i = 4 * (threadIdx.x % TILE), share = threadIdx.x / TILE;
+    const A* at = partial + (long long)(c - j) * 2 * (TILE * TILE) + u_slice * TILE + i;
+    Four s = {};
 #pragma unroll 8
-                for (int k = 0; k < count; ++k) s += at[(long long)list[k] * 2 * (TILE * TILE) + i];
-                s *= scale;
-            }
-            gp_store(out + (long long)u * path.w_ld + w, s);
-        }
-        __syncthreads();                        // (the list is written again)
+    for (int k = share; k < count; k += SHARES) {
+        const Four v = *reinterpret_cast<const Four*>(at + (long long)list[k] * (TILE * TILE));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s.v[e] += v.v[e];
+    }
+    sums[threadIdx.x] = s;
+    __syncthreads();
+    const int u = i / TILE;
+    if (share > 0 || u >= nu) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int w = i % TILE + e;
+        if (w >= nw) break;
+        A all = s.v[e];
+        for (int k = 1; k < SHARES; ++k) all += sums[threadIdx.x + k * TILE].v[e];
+        gp_store(dW + (long long)g * gp.w_numel + path.w_off + (long long)(u0 + u) * path.w_ld + w0 + w, (A)(all * (A)to.scale));
     }
 }
 

@@ -47,7 +47,7 @@ struct GdArgs {
     const long long *order, *offsets;
     void* dW;
     float* partial;             // [CTAs][2][128][128]
-    long long* lo;              // [CTAs] first position of each CTA's range
+    GpStart* starts;            // [CTAs]
     long long rows;
     int groups;
     int w_vec;                  // weights of dW in 16-byte pieces
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(GD_THREADS, 1) oeq_grouped_tc_dw(const __grid_
     tc_fence_after();
     const unsigned tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile unsigned*>(bars.tmem), 0);
     const long long lo = range.lo, hi = range.hi;
-    if (tid == 0) p.lo[blockIdx.x] = lo;
+    if (tid == 0) p.starts[blockIdx.x] = {(int)lo, range.g};
     const GtWalk walk(p.offsets, range.g, (int)lo, (int)hi);
     if (warp > MMA_WARP) {
         gd_ahead<T>(p, gd.gp, path, to, d, gd_unit<T>(d), u0, w0, mu, mw, bars, walk, tid - (MMA_WARP + 1) * 32);

@@ -129,17 +129,13 @@ GpSplit simt_split(const GpProblem& gp, int64_t rows, int sms) {
 }
 
 // The workspace of a weight gradient: the CTAs' first positions, then their partial tiles.
-size_t positions_bytes(const GpProblem& gp, const GpSplit& split) { return ((size_t)split.first[gp.n_paths] * sizeof(int64_t) + 255) / 256 * 256; }
+size_t positions_bytes(const GpProblem& gp, const GpSplit& split) { return ((size_t)split.first[gp.n_paths] * sizeof(GpStart) + 255) / 256 * 256; }
 
 template <class T, int TILE>
 int join(const GpProblem& gp, const GpSplit& split, int64_t rows, int64_t groups, const int64_t* offsets, void* dW, const void* ws, cudaStream_t st) {
-    int tiles = 0;
-    for (int p = 0; p < gp.n_paths; ++p) tiles += (split.first[p + 1] - split.first[p]) / split.parts[p];
-    int slices = 1;                     // some dozen CTAs for every SM: most find a complete group and leave
-    while (slices < TILE / 4 && (int64_t)slices * tiles * groups < 4096) slices *= 2;
-    const dim3 grid((unsigned)(slices * tiles), (unsigned)std::min<int64_t>(groups, 1024));
-    oeq_grouped_join<T, TILE><<<grid, 256, 0, st>>>(gp, split, (const long long*)offsets, rows, (int)groups, slices,
-                                                    (const typename GpAcc<T>::type*)((const char*)ws + positions_bytes(gp, split)), (const long long*)ws, (T*)dW);
+    const int ctas = split.first[gp.n_paths], zero_ctas = (int)std::min<int64_t>(groups, 296);
+    oeq_grouped_join<T, TILE><<<TILE / 4 * ctas + zero_ctas, 256, 0, st>>>(gp, split, (const long long*)offsets, rows, (int)groups, zero_ctas,
+                                                                         (const typename GpAcc<T>::type*)((const char*)ws + positions_bytes(gp, split)), (const GpStart*)ws, (T*)dW);
     OEQ_CUDA(cudaGetLastError());
     return OEQ_OK;
 }
@@ -152,7 +148,7 @@ int simt_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* 
     const GpSplit split = simt_split(gp, rows, sms);
     oeq_grouped_simt_dw<T><<<split.first[gp.n_paths], GP_SIMT_THREADS, 0, st>>>(gp, split, (const T*)X, (const T*)dZ, (const long long*)order,
                                                                                 (const long long*)offsets, rows, (int)groups, (T*)dW,
-                                                                                (typename GpAcc<T>::type*)((char*)ws + positions_bytes(gp, split)), (long long*)ws);
+                                                                                (typename GpAcc<T>::type*)((char*)ws + positions_bytes(gp, split)), (GpStart*)ws);
     OEQ_CUDA(cudaGetLastError());
     return join<T, GP_TILE>(gp, split, rows, groups, offsets, dW, ws, st);
 }
@@ -282,7 +278,7 @@ int tc_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* X,
     if (int rc = sm_count(sms)) return rc;
     GdProblem gd{gp, tc_split(gp, rows, groups, sms), {}};
     for (int p = 0; p < gp.n_paths; ++p) gd.extra[p] = GROUP_PAIRS / gp.target[gp.path[p].dst].d;
-    const GdArgs args{X, dZ, (const long long*)order, (const long long*)offsets, dW, (float*)((char*)ws + positions_bytes(gp, gd.split)), (long long*)ws, rows, (int)groups,
+    const GdArgs args{X, dZ, (const long long*)order, (const long long*)offsets, dW, (float*)((char*)ws + positions_bytes(gp, gd.split)), (GpStart*)ws, rows, (int)groups,
                       aligned(dW, 16) && gp.w_numel * sizeof(T) % 16 == 0};
     constexpr int V = 16 / sizeof(T);
     bool fast = aligned(X, 16) && aligned(dZ, 16) && gp.src_dim % V == 0 && gp.dst_dim % V == 0;
