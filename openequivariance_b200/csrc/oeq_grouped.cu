@@ -128,7 +128,13 @@ GpSplit simt_split(const GpProblem& gp, int64_t rows, int sms) {
     return s;
 }
 
-// The workspace of a weight gradient: the CTAs' first positions, then their partial tiles.
+// The workspace of a weight gradient: the starts of the CTAs' ranges, then their partial tiles, of which a path in one range has none.
+size_t partial_ctas(const GpProblem& gp, const GpSplit& split) {
+    int n = 0;
+    for (int p = 0; p < gp.n_paths; ++p)
+        if (split.parts[p] > 1) n = split.first[p + 1];
+    return (size_t)n;
+}
 size_t positions_bytes(const GpProblem& gp, const GpSplit& split) { return ((size_t)split.first[gp.n_paths] * sizeof(GpStart) + 255) / 256 * 256; }
 
 template <class T, int TILE>
@@ -154,6 +160,7 @@ int simt_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* 
 }
 
 // ---- tensor cores
+constexpr int MOST_PARTS = GP_PARTS;    // ranges of rows
 // The time of a group's weights, in (row, component) pairs.
 constexpr int GROUP_PAIRS = 96;
 // The CTAs, one for each SM, are dealt to the tiles of channels by the time that they take: for every (row, component) pair, and for
@@ -193,10 +200,18 @@ int tc_plan(const GpProblem& gp, int64_t rows, int64_t groups, int sms, GtProble
         cost[t] = ((double)rows * to.d + (double)std::min(rows, groups) * GROUP_PAIRS) * (k + x.n + 32);
         ctas += x.n_tiles;
     }
+    double all = 0;
+    for (int t = 0; t < gp.n_targets; ++t) all += cost[t] * gt.target[t].n_tiles;
+    ctas = 0;
+    for (int t = 0; t < gp.n_targets; ++t) {            // (whole shares first: the rest takes a few steps)
+        GtTarget& x = gt.target[t];
+        if (x.parts) x.parts = (int)std::max(1.0, std::min((double)std::min<int64_t>(rows, MOST_PARTS), std::floor(sms * cost[t] / all)));
+        ctas += x.parts * x.n_tiles;
+    }
     for (;;) {                          // the tile whose ranges take longest gets another CTA
         int most = -1;
         for (int t = 0; t < gp.n_targets; ++t)
-            if (gt.target[t].parts && gt.target[t].parts < rows && (most < 0 || cost[t] / gt.target[t].parts > cost[most] / gt.target[most].parts)) most = t;
+            if (gt.target[t].parts && gt.target[t].parts < std::min<int64_t>(rows, MOST_PARTS) && (most < 0 || cost[t] / gt.target[t].parts > cost[most] / gt.target[most].parts)) most = t;
         if (most < 0 || ctas + gt.target[most].n_tiles > sms) break;
         ++gt.target[most].parts;
         ctas += gt.target[most].n_tiles;
@@ -259,10 +274,17 @@ GpSplit tc_split(const GpProblem& gp, int64_t rows, int64_t groups, int sms) {
         s.parts[p] = 1;
         ctas += tiles[p];
     }
+    double all = 0;
+    for (int p = 0; p < gp.n_paths; ++p) all += cost[p] * tiles[p];
+    ctas = 0;
+    for (int p = 0; p < gp.n_paths; ++p) {
+        s.parts[p] = (int)std::max(1.0, std::min((double)std::min<int64_t>(rows, MOST_PARTS), std::floor(sms * cost[p] / all)));
+        ctas += s.parts[p] * tiles[p];
+    }
     for (;;) {
         int most = -1;
         for (int p = 0; p < gp.n_paths; ++p)
-            if (s.parts[p] < std::min<int64_t>(rows, GP_PARTS) && (most < 0 || cost[p] / s.parts[p] > cost[most] / s.parts[most])) most = p;
+            if (s.parts[p] < std::min<int64_t>(rows, MOST_PARTS) && (most < 0 || cost[p] / s.parts[p] > cost[most] / s.parts[most])) most = p;
         if (most < 0 || ctas + tiles[most] > sms) break;
         ++s.parts[most];
         ctas += tiles[most];
@@ -478,7 +500,7 @@ size_t oeq_grouped_workspace_bytes(const oeq_grouped* h, int dtype, int64_t rows
     const bool tc = dtype != OEQ_F64 && h->d_max <= GT_D_MAX;
     const GpSplit s = tc ? tc_split(gp, rows, groups, sms) : simt_split(gp, rows, sms);
     const size_t tile = tc ? GD_TILE * GD_TILE * sizeof(float) : GP_TILE * GP_TILE * std::max<size_t>(4, elem_bytes(dtype));
-    return positions_bytes(gp, s) + (size_t)s.first[gp.n_paths] * 2 * tile;
+    return positions_bytes(gp, s) + partial_ctas(gp, s) * 2 * tile;
 }
 
 int oeq_grouped_backward_weights(oeq_grouped* h, int dtype, int64_t rows, int64_t groups, const void* X, const void* dZ, const int64_t* order,

@@ -156,6 +156,31 @@ def test_linear(irreps_in, irreps_out, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("irreps_in,irreps_out", [("1100x0e", "300x0e"), ("300x0e", "1100x0e"), ("520x0e+8x1o", "136x0e+272x1o"), ("600x1o", "40x1o")])
+def test_linear_of_many_channels(irreps_in, irreps_out, dtype):
+    """Weights of a group that do not fit shared memory, several tiles of channels."""
+    check_linear(irreps_in, irreps_out, dtype, 300, 3, seed=3)
+
+
+def test_blocks_without_a_path():
+    """Irreps that one side alone has, of any degree, and blocks of no channels: zeros, with and without gradients."""
+    for names in (("4x0e+2x6e", "3x9o+4x0e"), ("0x1o+4x0e+0x0e", "0x0e+8x0e+0x2e"), ("2x5e", "2x5o")):
+        for dtype in (F32, F64, BF16):
+            check_linear(*names, dtype, 70, 3, seed=1)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=TYPE_IDS)
+def test_expanded_gradients(dtype):
+    """The gradient that a sum sends back has one value for all."""
+    x, w, _, index = inputs("16x0e+8x1o", "8x0e+8x1o", dtype, 120, 4, 2)
+    lin, plan = oeq.GroupedLinear("16x0e+8x1o", "8x0e+8x1o"), groups_of(index, 4)
+    xg, wg = (t.to(dtype).cuda().requires_grad_(True) for t in (x, w))
+    z = lin(xg, wg, plan)
+    z.sum().backward()
+    compare("16x0e+8x1o", "8x0e+8x1o", dtype, x, w, torch.ones(z.shape, dtype=F64), index, z, xg.grad, wg.grad)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=TYPE_IDS)
 @pytest.mark.parametrize("rows", [1, 2, 63, 64, 65, 127, 128, 129, 700])
 def test_linear_rows(rows, dtype):
     check_linear("32x0e+20x1o", "24x0e+32x1o", dtype, rows, 3, seed=rows)
@@ -277,6 +302,17 @@ def test_second_derivatives(dtype):
     want_z = ref.linear(*names, ex, w, index) + ref.linear(*names, x, ew, index)
     for got, want in ((gx, want_x), (gw, want_w), (gdz, want_z)):
         assert float((got.cpu().double() - want).abs().max() / want.abs().max()) < (1e-5 if dtype == F32 else 1e-12)
+
+
+def test_weights_changed_in_place_are_noticed():
+    x, w, dz, index = inputs("8x0e", "8x0e", F32, 50, 3, 1)
+    plan, lin = groups_of(index, 3), oeq.GroupedLinear("8x0e", "8x0e")
+    wg = w.float().cuda().requires_grad_(True)
+    z = lin(x.float().cuda().requires_grad_(True), wg, plan)
+    with torch.no_grad():
+        wg.mul_(2.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        z.backward(dz.float().cuda())
 
 
 def test_only_the_gradients_that_are_asked_for():
