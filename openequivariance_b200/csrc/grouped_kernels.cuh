@@ -1,11 +1,13 @@
-// Linear maps of irreps with one set of weights for each group of rows, on the FMA units (FP64: the FP64 tensor
-// units): every type, every degree.
+// Linear maps of irreps with one set of weights for each group of rows, without tcgen05: FP64, and blocks of l = 4 and above of
+// every type.
 //
 //   Z[r,o,w,k] = c_o sum_{i,u} W_g[i,o][u,w] X[r,i,u,k],  g = group of row r          (product; dX with W transposed)
 //   dW_g[i,o][u,w] = c_o sum_{r in g, k} X[r,i,u,k] dZ[r,o,w,k]                        (weight gradient)
 //
-// Both kernels are 64 x 64 register-tiled products with 4 x 4 values
-// per thread; 16 steps of the sum are staged in shared memory while the next 16 are on their way in registers.
+// Both kernels are 64 x 64 products in registers, 16 values of a thread; 16 steps of the sum are staged in shared memory while the next 16
+// are on their way in registers.  FP64 goes through mma.m8n8k4 (there is no FP64 kind of tcgen05.mma): 10 007 rows of 64x(0e+1o+2e) 62 us, weight
+// gradient 80, 12 and 9 TFLOP/s; with FMAs 102 and 129.  Bound by latency with two or three CTAs an SM: issue 42 %, load and store unit 49 %, FP64 tensor
+// pipe 35 %.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -62,7 +64,7 @@ __device__ __forceinline__ long long gp_row(const long long* __restrict__ order,
 __device__ __forceinline__ long long gp_cut(long long n, int part, int parts) { return (long long)((unsigned long long)n * part / parts); }
 constexpr int GP_TILE = 64, GP_STEP = 16, GP_SIMT_THREADS = 256;
 // A 64 x 64 product by 256 threads, 16 values each, over GP_STEP staged steps.  PITCH of a staged step: 16 steps by two rows, which a warp
-// writes, and what it reads lie in different banks (a pitch of 64: 120 us instead of 102 for 10 007 rows of 64x(0e+1o+2e) FP64).
+// writes, and what it reads lie in different banks, or two at most to a bank (a pitch of 64 values: 120 us instead of 102 with FMAs).
 template <class A> struct GpProduct {           // FMA: 4 rows by 4 columns of a thread
     static constexpr int PITCH = GP_TILE + 2;
     A acc[16] = {};
