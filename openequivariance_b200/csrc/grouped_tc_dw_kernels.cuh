@@ -126,7 +126,11 @@ template <class T, int D, bool FAST>
 __device__ __forceinline__ bool gd_fill(const GdArgs& p, const GpProblem& gp, const GtWalk& walk, const GdLane& l, const T* x, const T* z, int n, unsigned char* ring,
                                         const GdBars& bars, int bundle, int use) {
     constexpr bool BOTH = gd_sets(D) == 2;      // a lane reads both operands
-    constexpr int ROWS = GdType<T>::ROWS, THREADS = 256, PASS = D == 1 ? 4 : (sizeof(T) == 4 ? 1 : 2), FIRST = gd_first(D), BUNDLE = gd_bundle<T>(D);
+    // Rows of a lane on the way together.  Two of 16 bits with components instead of one: 122 us instead of 126 for 300 000 rows of 128x1o and 132 instead of
+    // 136 for 100 000 rows in 256 groups, but 152 instead of 134 for 200 000 of 128x2e, 130 instead of 122 for 120 000 of 128x3o, and 259 instead of 249 for 512x0e:
+    // all widths share the kernel's 72 registers.
+    constexpr int PASS = D == 1 ? 4 : 1;
+    constexpr int ROWS = GdType<T>::ROWS, THREADS = 256, FIRST = gd_first(D), BUNDLE = gd_bundle<T>(D);
     const int rows = (walk.rows + ROWS - 1) / ROWS * ROWS, step = THREADS >> l.lp, blocks = (n + 63) / 64, lane = threadIdx.x & 31;
     const bool is_x = l.x_left > 0;
     auto free_again = [&](int b) { return use == 0 || warp_wait(true, bars.empty + b, (unsigned)(use - 1) & 1, &gt_status, ERR_GD_EMPTY); };

@@ -161,8 +161,11 @@ int simt_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* 
 
 // ---- tensor cores
 constexpr int MOST_PARTS = GP_PARTS;    // ranges of rows
-// The time of a group's weights, in (row, component) pairs.
-constexpr int GROUP_PAIRS = 96;
+// The time of a group's weights, in (row, component) pairs.  FP32, whose weights are split: 160 instead of 96 takes 4 999 rows of 128x(0e+1o+2e) in 89 groups
+// from 41.0 to 36.9 us (64: 50, 240: 42) and 50 000 rows in 10 groups from 219 to 221.  In 16 bits, where they are copied, 64 and 96 are equal (143 us, 100 000 rows
+// in 256 groups) and 160 takes 148.  The weight gradient of the first: 54 / 47 / 50 / 54 us with 64 / 96 / 160 / 240.
+template <class T> constexpr int group_pairs() { return GtType<T>::SPLIT ? 160 : 96; }
+constexpr int GROUP_PAIRS_DW = 96;
 // The CTAs, one for each SM, are dealt to the tiles of channels by the time that they take: for every (row, component) pair, and for
 // those that a group's weights count for, the channels read and written and a fixed part.  (By the rows alone 4 999 rows in 89
 // groups take 58 us: an output of scalars, with as many weights as the others, has a ninth of the CTAs.)
@@ -196,8 +199,8 @@ int tc_plan(const GpProblem& gp, int64_t rows, int64_t groups, int sms, GtProble
             }
         }
         x.n_tiles = (to.mul + x.n - 1) / x.n;
-        x.extra = GROUP_PAIRS / to.d;
-        cost[t] = ((double)rows * to.d + (double)std::min(rows, groups) * GROUP_PAIRS) * (k + x.n + 32);
+        x.extra = group_pairs<T>() / to.d;
+        cost[t] = ((double)rows * to.d + (double)std::min(rows, groups) * group_pairs<T>()) * (k + x.n + 32);
         ctas += x.n_tiles;
     }
     double all = 0;
@@ -270,7 +273,7 @@ GpSplit tc_split(const GpProblem& gp, int64_t rows, int64_t groups, int sms) {
     for (int p = 0; p < gp.n_paths; ++p) {
         const GpTarget& to = gp.target[gp.path[p].dst];
         tiles[p] = (gp.path[p].src_mul + GD_TILE - 1) / GD_TILE * ((to.mul + GD_TILE - 1) / GD_TILE);
-        cost[p] = ((double)rows * to.d + (double)std::min(rows, groups) * GROUP_PAIRS) * (std::min(GD_TILE, gp.path[p].src_mul) + std::min(GD_TILE, to.mul) + 64);
+        cost[p] = ((double)rows * to.d + (double)std::min(rows, groups) * GROUP_PAIRS_DW) * (std::min(GD_TILE, gp.path[p].src_mul) + std::min(GD_TILE, to.mul) + 64);
         s.parts[p] = 1;
         ctas += tiles[p];
     }
@@ -299,7 +302,7 @@ int tc_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* X,
     int sms = 0;
     if (int rc = sm_count(sms)) return rc;
     GdProblem gd{gp, tc_split(gp, rows, groups, sms), {}};
-    for (int p = 0; p < gp.n_paths; ++p) gd.extra[p] = GROUP_PAIRS / gp.target[gp.path[p].dst].d;
+    for (int p = 0; p < gp.n_paths; ++p) gd.extra[p] = GROUP_PAIRS_DW / gp.target[gp.path[p].dst].d;
     const GdArgs args{X, dZ, (const long long*)order, (const long long*)offsets, dW, (float*)((char*)ws + positions_bytes(gp, gd.split)), (GpStart*)ws, rows, (int)groups,
                       aligned(dW, 16) && gp.w_numel * sizeof(T) % 16 == 0};
     constexpr int V = 16 / sizeof(T);
