@@ -16,7 +16,7 @@
 //     rounded, and the error grows with the length of a chain (relative, one chain of 750 slots: 1e-5).  The two accumulators alternate.
 //   * 3 warps prefetch rows to L2, up to two units ahead of the MMAs.
 // Measured from a cold L2 with the sum over ranges, 50 000 rows in 10 groups of 128x(0e+1o+2e+3o) FP32: 234 us (3.5 TB/s); 100 000 rows of 128x(0e+1o+2e)
-// BF16 131 us; 65 536 rows of 512x0e with 1024x0e BF16 256 us (32 tiles of 128 x 128 read 1.1 GB through L2).  Loads on their way bound it (long
+// BF16 in 256 groups 133 us; 65 536 rows of 512x0e with 1024x0e BF16 246 us (32 tiles of 128 x 128 read 1.1 GB through L2).  Loads on their way bound it (long
 // scoreboard), with the load and store unit at 56 % and the tensor pipe at 32 %.
 // A CTA has one tile of one path and a range of the sorted rows (gt_range); groups that go beyond the range leave a partial tile for
 // oeq_grouped_join.  Every wait is bounded.
@@ -127,8 +127,8 @@ __device__ __forceinline__ bool gd_fill(const GdArgs& p, const GpProblem& gp, co
                                         const GdBars& bars, int bundle, int use) {
     constexpr bool BOTH = gd_sets(D) == 2;      // a lane reads both operands
     // Rows of a lane on the way together.  Two of 16 bits with components instead of one: 122 us instead of 126 for 300 000 rows of 128x1o and 132 instead of
-    // 136 for 100 000 rows in 256 groups, but 152 instead of 134 for 200 000 of 128x2e, 130 instead of 122 for 120 000 of 128x3o, and 259 instead of 249 for 512x0e:
-    // all widths share the kernel's 72 registers.
+    // 136 for 100 000 rows in 256 groups, but 152 instead of 134 for 200 000 of 128x2e, 130 instead of 122 for 120 000 of 128x3o, and 259 instead of 249 for 65 536 of 512x0e
+    // with 1024x0e: all widths share the kernel's registers, 72 at most, which spilled.
     constexpr int PASS = D == 1 ? 4 : 1;
     constexpr int ROWS = GdType<T>::ROWS, THREADS = 256, FIRST = gd_first(D), BUNDLE = gd_bundle<T>(D);
     const int rows = (walk.rows + ROWS - 1) / ROWS * ROWS, step = THREADS >> l.lp, blocks = (n + 63) / 64, lane = threadIdx.x & 31;
