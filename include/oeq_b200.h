@@ -253,14 +253,16 @@ int oeq_grouped_backward_weights(oeq_grouped* h, int dtype, int64_t rows, int64_
                                  const int64_t* order, const int64_t* offsets, void* dW, void* workspace,
                                  size_t workspace_bytes, void* stream);
 
-/* Status of these kernels on the current device (synchronises it): OEQ_OK, or OEQ_ERR_DEVICE_WAIT once a kernel has abandoned a
- * bounded wait. */
+/* Status of these kernels on the current device, after waiting for all of its streams (so not while one is captured): OEQ_OK, or
+ * OEQ_ERR_DEVICE_WAIT if a kernel has abandoned a bounded wait since the last check.  Reporting it clears it. */
 int oeq_grouped_check(void);
 
 /* Exercises the error path of the kernels' bounded waits without harming the device: one thread polls a barrier
  * that nothing completes `polls` times (at most 2^20), gives up, and the call reports what oeq_*_check would report,
  * OEQ_ERR_DEVICE_WAIT.  The context stays usable.  No counterpart in the reference (its kernels have no waits). */
 int oeq_selftest_bounded_wait(int polls, void* stream);
+/* The same for the status of the row group kernels: the wait is queued on the stream, and the next oeq_grouped_check reports it. */
+int oeq_selftest_grouped_wait(int polls, void* stream);
 
 /* Launch geometry of the most recent specialisation, for benchmarks and tests:
  * which = 0 forward, 1 backward.  Any output pointer may be NULL. */

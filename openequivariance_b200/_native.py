@@ -93,6 +93,7 @@ SYMBOLS = {
     "oeq_grouped_backward_weights": (_INT, [_P, _INT, _I64, _I64, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "oeq_grouped_check": (_INT, []),
     "oeq_selftest_bounded_wait": (_INT, [_INT, _P]),
+    "oeq_selftest_grouped_wait": (_INT, [_INT, _P]),
     "oeq_tp_launch_info": (_INT, [_P, _INT, _PI, _PI, _PI, _PI, _PI, _PI]),
     "oeq_conv_launch_info": (_INT, [_P, _INT, _PI, _PI, _PI, _PI, _PI, _PI]),
 }

@@ -322,6 +322,17 @@ int tc_weights(const GpProblem& gp, int64_t rows, int64_t groups, const void* X,
     return join<T, GD_TILE>(gp, gd.split, rows, groups, offsets, dW, ws, st);
 }
 
+// One thread polls a barrier that nothing completes, gives up and records the code, as a kernel whose wait runs out does.
+__global__ void oeq_grouped_wait_probe(unsigned polls) {
+    __shared__ unsigned long long bar;
+    if (threadIdx.x != 0) return;
+    mbar_init(&bar, 1);
+    fence_mbar_init();
+    for (unsigned i = 0; i < polls; ++i)
+        if (mbar_try_wait(&bar, 0u)) return;
+    atomicCAS(&gt_status, 0, ERR_GT_FULL);
+}
+
 int check_call(const oeq_grouped* h, int dtype, int64_t rows, int64_t groups) {
     if (!h) return oeq_fail(OEQ_ERR_INVALID, "null handle");
     if (!known_dtype(dtype)) return oeq_fail(OEQ_ERR_INVALID, "unknown dtype");
@@ -527,10 +538,21 @@ int oeq_grouped_backward_weights(oeq_grouped* h, int dtype, int64_t rows, int64_
     }
 }
 
+// (the copy alone is ordered behind the default stream and the streams that block with it: the device is waited for)
 int oeq_grouped_check(void) {
     int code = 0;
+    OEQ_CUDA(cudaDeviceSynchronize());
     OEQ_CUDA(cudaMemcpyFromSymbol(&code, gt_status, sizeof code));
-    if (code) return oeq_fail(OEQ_ERR_DEVICE_WAIT, "a kernel gave up on a bounded wait (code " + std::to_string(code) + ")");
+    if (code == 0) return OEQ_OK;
+    const int none = 0;
+    OEQ_CUDA(cudaMemcpyToSymbol(gt_status, &none, sizeof none));
+    return oeq_fail(OEQ_ERR_DEVICE_WAIT, "a kernel abandoned a bounded wait (code " + std::to_string(code) + ")");
+}
+
+int oeq_selftest_grouped_wait(int polls, void* stream) {
+    if (polls < 1 || polls > (1 << 20)) return oeq_fail(OEQ_ERR_INVALID, "polls must be in 1 .. 2^20");
+    oeq_grouped_wait_probe<<<1, 32, 0, (cudaStream_t)stream>>>((unsigned)polls);
+    OEQ_CUDA(cudaGetLastError());
     return OEQ_OK;
 }
 

@@ -151,5 +151,6 @@ class GroupedLinear:
 
     @staticmethod
     def check_device_status():
-        """Raises if a kernel on the current device has abandoned a bounded wait (waits for the device)."""
+        """Raises if a kernel on the current device has abandoned a bounded wait since the last check.  Waits for all streams of
+        the device."""
         _native.check(_native.lib().oeq_grouped_check())

@@ -515,3 +515,28 @@ def test_wrong_arguments_raise():
     with pytest.raises(NotImplementedError, match="forward-mode"):
         with torch.autograd.forward_ad.dual_level():
             lin(torch.autograd.forward_ad.make_dual(cuda(10, 8), cuda(10, 8)), cuda(3, 32), plan)
+
+
+# ------------------------------------------------------------------------------------------ status
+
+def test_the_check_waits_for_every_stream():
+    """Streams of torch's pool do not block with the default stream: a copy of the status alone does not wait for them."""
+    a, side, done = torch.randn(8192, 8192, device="cuda"), torch.cuda.Stream(), torch.cuda.Event()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):                     # some 30 ms
+            a @ a
+        done.record()
+    oeq.GroupedLinear.check_device_status()
+    assert done.query()
+
+
+def test_a_wait_that_runs_out_is_reported_once():
+    from openequivariance_b200 import _native
+    lib, side = _native.lib(), torch.cuda.Stream()
+    assert lib.oeq_selftest_grouped_wait(2000, side.cuda_stream) == _native.OEQ_OK
+    with pytest.raises(_native.OeqError, match="bounded wait"):
+        oeq.GroupedLinear.check_device_status()
+    oeq.GroupedLinear.check_device_status()
+    assert lib.oeq_selftest_grouped_wait(0, side.cuda_stream) == _native.OEQ_ERR_INVALID
+    check_linear("8x0e", "8x0e", F32, 70, 3)
