@@ -263,6 +263,9 @@ int oeq_grouped_check(void);
 int oeq_selftest_bounded_wait(int polls, void* stream);
 /* The same for the status of the row group kernels: the wait is queued on the stream, and the next oeq_grouped_check reports it. */
 int oeq_selftest_grouped_wait(int polls, void* stream);
+/* Exercises the warps that write the results of a product when the wait of one of the eight (`warp`; -1: of none) runs out and those of
+ * the others do not: the kernel ends, and oeq_grouped_check reports the wait. */
+int oeq_selftest_grouped_drain(int warp, void* stream);
 
 /* Launch geometry of the most recent specialisation, for benchmarks and tests:
  * which = 0 forward, 1 backward.  Any output pointer may be NULL. */

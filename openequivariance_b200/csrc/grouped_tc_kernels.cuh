@@ -580,9 +580,12 @@ __device__ __forceinline__ void gt_ahead(const GtProblem& gt, const GtArgs& p, c
 
 // ---------------------------------------------------------------------------- epilogue
 // The chunks of 32 channels of all tiles go to the two groups of four warps in turn.
-template <class T, bool TRANS, int D>
+// acc_wait(buffer, parity): the warp's wait for an accumulator.  A warp whose wait ran out reads and writes nothing more but comes to every
+// barrier of its group: each warp counts its own polls, so the other three may have seen the accumulator complete, and a hardware barrier
+// waits without limit.  (It keeps the rows' numbers up to date: the others write the rows that stand there.)
+template <class T, bool TRANS, int D, class Wait>
 __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, float* staging,
-                                         const GtBars& bars, GtWalk walk, unsigned tmem, int group, int warp, int lane) {
+                                         const GtBars& bars, GtWalk walk, unsigned tmem, int group, int warp, int lane, Wait&& acc_wait) {
     constexpr int TILE_ROWS = gt_tile_rows(D), PITCH = gt_pitch<D>();
     const int n = tile_of.n, mul = min(n, to.mul - n0), pair = warp * 32 + lane, r_of = pair / D, k_of = pair % D;
     const float scale = (float)to.scale;
@@ -590,33 +593,34 @@ __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, c
     int* rows_of = bars.rows + 128 * group;
     staging += group * (GT_STAGING / 4);
     int tiles = 0, turn = 0;
+    bool alive = true;
     for (; walk.more(); walk.next(p.offsets, p.groups), ++tiles) {
         walk.tile(TILE_ROWS);
         const int buf = tiles & 1;
         if (pair < walk.rows) rows_of[pair] = (int)gp_row(p.order, walk.pos + pair);         // (read behind the first barrier below)
-        if (!warp_wait(true, bars.acc_full + buf, (unsigned)(tiles / 2) & 1, &gt_status, ERR_GT_ACC_FULL)) return;
+        alive = alive && acc_wait(buf, (unsigned)(tiles / 2) & 1);
         tc_fence_after();
         bool mine = false;
         for (int w0 = 0; w0 < mul; w0 += 32, turn ^= 1) {
             if (turn != group) continue;
             mine = true;
-const bool last = w0 + 32 * GT_EPI_GROUPS >= mul;           // the group has read its part of the accumulator then
+            const bool last = w0 + 32 * GT_EPI_GROUPS >= mul;           // the group has read its part of the accumulator then
             float* to_smem = staging + r_of * PITCH + k_of;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 unsigned v[16], u[GtType<T>::SPLIT ? 16 : 1];
                 const unsigned at = quarter + (unsigned)(buf * 256 + w0 + 16 * h);
-                if (w0 + 16 * h < n) {
+                if (alive && w0 + 16 * h < n) {
                     tc_load16(at, v);
                     if constexpr (GtType<T>::SPLIT) tc_load16(at + n, u);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                 }
-                if (last && h == 1) {
+                if (alive && last && h == 1) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bars.acc_empty + buf);
                 }
-                if (w0 + 16 * h < n && r_of < walk.rows) {
+                if (alive && w0 + 16 * h < n && r_of < walk.rows) {
                     float s[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
@@ -636,13 +640,14 @@ const bool last = w0 + 32 * GT_EPI_GROUPS >= mul;           // the group has rea
             group_sync(1 + group, 128);
             const int values = min(32, mul - w0) * D;
             T* z = static_cast<T*>(p.Z) + to.off + (n0 + w0) * D;
-            if (p.z_vec && (to.off | values) % (16 / (int)sizeof(T)) == 0) gt_write<T, D, true>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
+            if (!alive) {}
+            else if (p.z_vec && (to.off | values) % (16 / (int)sizeof(T)) == 0) gt_write<T, D, true>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
             else gt_write<T, D, false>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
             group_sync(1 + group, 128);
         }
         if (!mine) {
             __syncwarp();
-            if (lane == 0) mbar_arrive(bars.acc_empty + buf);
+            if (alive && lane == 0) mbar_arrive(bars.acc_empty + buf);
             group_sync(1 + group, 128);         // (rows_of is written again by all four warps)
         }
     }
@@ -653,7 +658,41 @@ template <class T, bool TRANS, bool FAST, int D>
 __device__ __forceinline__ void gt_roles(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, unsigned char* a_base,
                                          unsigned char* b_base, float* staging, const GtBars& bars, const GtWalk& walk, unsigned tmem, int warp, int tid) {
     if (warp < GT_PW) gt_produce<T, TRANS, FAST, D>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid);
-    else gt_drain<T, TRANS, D>(gt, p, tile_of, to, n0, staging, bars, walk, tmem, (warp - GT_PW) >> 2, warp & 3, tid & 31);
+    else gt_drain<T, TRANS, D>(gt, p, tile_of, to, n0, staging, bars, walk, tmem, (warp - GT_PW) >> 2, warp & 3, tid & 31, [&](int buf, unsigned parity) {
+        return warp_wait(true, bars.acc_full + buf, parity, &gt_status, ERR_GT_ACC_FULL);
+    });
+}
+
+// Self-test: the drain of three tiles of one row, whose accumulators hold anything.  Warp `lost` has its waits run out, the others have
+// theirs complete; all come back.
+constexpr int GT_PROBE_ROWS = 3, GT_PROBE_COLUMNS = 80;
+__device__ const long long gt_probe_offsets[GT_PROBE_ROWS + 1] = {0, 1, 2, 3};
+__device__ float gt_probe_z[GT_PROBE_ROWS * GT_PROBE_COLUMNS];
+__global__ void __launch_bounds__(32 * GT_EPI) oeq_grouped_drain_probe(const __grid_constant__ GtProblem gt, int lost) {
+    __shared__ __align__(1024) unsigned char smem[GT_EPI_GROUPS * GT_STAGING + GT_CONTROL];
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const GtBars bars(smem + GT_EPI_GROUPS * GT_STAGING);
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) mbar_init(bars.acc_empty + i, GT_EPI);
+        fence_mbar_init();
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(bars.tmem)), "n"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile unsigned*>(bars.tmem), 0);
+    const GtArgs p{nullptr, nullptr, nullptr, gt_probe_offsets, gt_probe_z, GT_PROBE_ROWS, GT_PROBE_ROWS, 0};
+    gt_drain<float, false, 1>(gt, p, gt.target[0], gt.gp.target[0], 0, reinterpret_cast<float*>(smem), bars, GtWalk(gt_probe_offsets, 0, 0, GT_PROBE_ROWS), tmem, warp >> 2,
+                              warp & 3, lane, [&](int, unsigned) {
+                                  if (warp == lost && lane == 0) atomicCAS(&gt_status, 0, ERR_GT_ACC_FULL);
+                                  return warp != lost;
+                              });
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
 }
 
 // FAST: every block of rows and weights is made of whole, aligned 16-byte pieces.

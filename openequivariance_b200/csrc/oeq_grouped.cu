@@ -549,6 +549,20 @@ int oeq_grouped_check(void) {
     return oeq_fail(OEQ_ERR_DEVICE_WAIT, "a kernel abandoned a bounded wait (code " + std::to_string(code) + ")");
 }
 
+int oeq_selftest_grouped_drain(int warp, void* stream) {
+    if (warp < -1 || warp >= GT_EPI) return oeq_fail(OEQ_ERR_INVALID, "warp must be in -1 .. " + std::to_string(GT_EPI - 1));
+    for (const int channels : {16, GT_PROBE_COLUMNS}) {         // one chunk of a tile (a group has none in turn) and three
+        GtProblem gt{};
+        gt.gp.n_targets = gt.gp.n_paths = 1;
+        gt.gp.dst_dim = channels;
+        gt.gp.target[0] = {0, channels, 1, 0, 1, 1.0};
+        gt.target[0] = {1, channels, 1, 0, 1, 1, 1, 0};
+        oeq_grouped_drain_probe<<<1, 32 * GT_EPI, 0, (cudaStream_t)stream>>>(gt, warp);
+        OEQ_CUDA(cudaGetLastError());
+    }
+    return OEQ_OK;
+}
+
 int oeq_selftest_grouped_wait(int polls, void* stream) {
     if (polls < 1 || polls > (1 << 20)) return oeq_fail(OEQ_ERR_INVALID, "polls must be in 1 .. 2^20");
     oeq_grouped_wait_probe<<<1, 32, 0, (cudaStream_t)stream>>>((unsigned)polls);

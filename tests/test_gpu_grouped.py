@@ -540,3 +540,17 @@ def test_a_wait_that_runs_out_is_reported_once():
     oeq.GroupedLinear.check_device_status()
     assert lib.oeq_selftest_grouped_wait(0, side.cuda_stream) == _native.OEQ_ERR_INVALID
     check_linear("8x0e", "8x0e", F32, 70, 3)
+
+
+@pytest.mark.parametrize("warp", [-1, 0, 3, 4, 7])
+def test_a_warp_whose_wait_runs_out_comes_to_its_barriers(warp):
+    """Three of the four warps that share a barrier go on; the kernel ends all the same."""
+    from openequivariance_b200 import _native
+    lib = _native.lib()
+    assert lib.oeq_selftest_grouped_drain(warp, torch.cuda.current_stream().cuda_stream) == _native.OEQ_OK
+    if warp < 0:
+        oeq.GroupedLinear.check_device_status()
+    else:
+        with pytest.raises(_native.OeqError, match="bounded wait"):
+            oeq.GroupedLinear.check_device_status()
+    check_linear("8x0e", "8x0e", F32, 70, 3)

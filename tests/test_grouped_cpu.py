@@ -101,3 +101,11 @@ def test_reference_of_row_groups():
     assert offsets.tolist() == [0, 2, 2, 4] and blocks.tolist() == [[0, 0, 2], [2, 2, 2], [-1, 0, 0]]
     index, offsets, _ = ref.from_counts([2, -1, 9], 5)
     assert index.tolist() == [0, 0, 2, 2, 2] and offsets.tolist() == [0, 2, 2, 5]
+
+
+def test_selftests_refuse_bad_arguments():
+    lib = _native.lib()
+    for warp in (-2, 8):
+        assert lib.oeq_selftest_grouped_drain(warp, None) == _native.OEQ_ERR_INVALID
+    for polls in (0, 2 ** 20 + 1):
+        assert lib.oeq_selftest_grouped_wait(polls, None) == _native.OEQ_ERR_INVALID
