@@ -266,6 +266,9 @@ int oeq_selftest_grouped_wait(int polls, void* stream);
 /* Exercises the warps that write the results of a product when the wait of one of the eight (`warp`; -1: of none) runs out and those of
  * the others do not: the kernel ends, and oeq_grouped_check reports the wait. */
 int oeq_selftest_grouped_drain(int warp, void* stream);
+/* The same for the warp that issues the MMAs: those on their way are over before the kernel ends (oeq_grouped_check reports code 84, and 86
+ * if they are not). */
+int oeq_selftest_grouped_issue(void* stream);
 
 /* Launch geometry of the most recent specialisation, for benchmarks and tests:
  * which = 0 forward, 1 backward.  Any output pointer may be NULL. */

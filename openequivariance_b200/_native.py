@@ -95,6 +95,7 @@ SYMBOLS = {
     "oeq_selftest_bounded_wait": (_INT, [_INT, _P]),
     "oeq_selftest_grouped_wait": (_INT, [_INT, _P]),
     "oeq_selftest_grouped_drain": (_INT, [_INT, _P]),
+    "oeq_selftest_grouped_issue": (_INT, [_P]),
     "oeq_tp_launch_info": (_INT, [_P, _INT, _PI, _PI, _PI, _PI, _PI, _PI]),
     "oeq_conv_launch_info": (_INT, [_P, _INT, _PI, _PI, _PI, _PI, _PI, _PI]),
 }

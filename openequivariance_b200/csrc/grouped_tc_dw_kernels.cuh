@@ -70,7 +70,7 @@ __device__ __forceinline__ unsigned long long gd_desc(unsigned addr, int blocks)
 }
 
 struct GdBars {
-    unsigned long long *full, *empty, *acc_full, *acc_empty;
+    unsigned long long *full, *empty, *acc_full, *acc_empty, *done;
     unsigned* tmem;
     volatile int* progress;     // units whose MMAs are on their way
     __device__ explicit GdBars(unsigned char* control) {
@@ -78,7 +78,8 @@ struct GdBars {
         empty = full + GD_BUNDLES;
         acc_full = empty + GD_BUNDLES;
         acc_empty = acc_full + 2;
-        tmem = reinterpret_cast<unsigned*>(acc_empty + 2);
+        done = acc_empty + 2;
+        tmem = reinterpret_cast<unsigned*>(done + 1);
         progress = reinterpret_cast<volatile int*>(tmem + 1);
     }
 };
@@ -315,6 +316,7 @@ __device__ __forceinline__ void gd_multiply(const GdArgs& p, int d, int unit, in
             ++accs;
         }
     }
+    if (!ok) gt_settle(leader, bars.done);
 }
 
 // ---------------------------------------------------------------------------- prefetch
@@ -419,6 +421,7 @@ __global__ void __launch_bounds__(GD_THREADS, 1) oeq_grouped_tc_dw(const __grid_
             mbar_init(bars.acc_full + i, 1);
             mbar_init(bars.acc_empty + i, GD_EPI);
         }
+        mbar_init(bars.done, 1);
         *bars.progress = 0;
         fence_mbar_init();
     }

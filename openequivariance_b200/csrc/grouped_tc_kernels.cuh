@@ -34,7 +34,7 @@ constexpr int GT_SETS = 3, GT_SET = 4, GT_PW = GT_SETS * GT_SET, GT_EPI_GROUPS =
 constexpr int GT_STAGES = 6;                    // most stages of A
 constexpr int GT_STAGING = 42 * 100 * 4;        // 32 channels of a tile's pairs (three components take most), for each epilogue group
 constexpr int GT_CONTROL = 1536;                // barriers, rows of the tiles that drain, the CTA's range
-constexpr int ERR_GT_EMPTY = 81, ERR_GT_FULL = 82, ERR_GT_ACC_FULL = 83, ERR_GT_ACC_EMPTY = 84, ERR_GT_TURN = 85;
+constexpr int ERR_GT_EMPTY = 81, ERR_GT_FULL = 82, ERR_GT_ACC_FULL = 83, ERR_GT_ACC_EMPTY = 84, ERR_GT_TURN = 85, ERR_GT_DONE = 86;
 
 // Set by a kernel whose bounded wait ran out; read by oeq_grouped_check.
 __device__ int gt_status;
@@ -239,7 +239,7 @@ struct GtArgs {
     int z_vec;                  // rows of Z in 16-byte pieces
 };
 struct GtBars {
-    unsigned long long *full, *empty, *acc_full, *acc_empty, *turn;
+    unsigned long long *full, *empty, *acc_full, *acc_empty, *turn, *done;
     unsigned* tmem;
     volatile int* progress;     // tiles whose MMAs are on their way
     int* rows;                  // of the tile that drains, for each epilogue group
@@ -249,7 +249,8 @@ struct GtBars {
         acc_full = empty + GT_STAGES;
         acc_empty = acc_full + 2;
         turn = acc_empty + 2;
-        tmem = reinterpret_cast<unsigned*>(turn + GT_SETS);
+        done = turn + GT_SETS;
+        tmem = reinterpret_cast<unsigned*>(done + 1);
         progress = reinterpret_cast<volatile int*>(tmem + 1);
         rows = reinterpret_cast<int*>(control + 512);      // (behind the range)
     }
@@ -419,9 +420,14 @@ __device__ __forceinline__ void gt_produce(const GtProblem& gt, const GtArgs& p,
 }
 
 // ---------------------------------------------------------------------------- MMA
-template <class T, bool TRANS>
+// After a wait that ran out: MMAs that are on their way read shared memory and write tensor memory, which the CTA gives back when it ends.
+__device__ __forceinline__ void gt_settle(unsigned leader, unsigned long long* done) {
+    tc_commit_if(leader, done);
+    warp_wait(true, done, 0, &gt_status, ERR_GT_DONE);
+}
+template <class T, bool TRANS, class Wait>
 __device__ __forceinline__ void gt_multiply(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, unsigned char* a_base,
-                                            unsigned char* b_base, const GtBars& bars, GtWalk walk, int tile_rows, unsigned tmem, unsigned leader) {
+                                            unsigned char* b_base, const GtBars& bars, GtWalk walk, int tile_rows, unsigned tmem, unsigned leader, Wait&& acc_wait) {
     constexpr int KC = GtType<T>::KC, KSTEP = GtType<T>::KSTEP;
     constexpr bool B_MN = !TRANS;
     const int n = tile_of.n, acc = GtType<T>::acc(n), step_b = gt_step_b<T, B_MN>(n) >> 4;
@@ -433,7 +439,7 @@ __device__ __forceinline__ void gt_multiply(const GtProblem& gt, const GtArgs& p
         walk.tile(tile_rows);
         const int buf = tiles & 1;
         bool ok = true;
-        if (tiles >= 2) ok = warp_wait(ok, bars.acc_empty + buf, (unsigned)(tiles / 2 - 1) & 1, &gt_status, ERR_GT_ACC_EMPTY);
+        if (tiles >= 2) ok = acc_wait(buf, (unsigned)(tiles / 2 - 1) & 1);
         const unsigned d = tmem + (unsigned)(buf * 256);
         unsigned accumulate = 0;
         if (resident) slot = 0;
@@ -459,7 +465,7 @@ __device__ __forceinline__ void gt_multiply(const GtProblem& gt, const GtArgs& p
                 if (++slot == tile_of.slots) slot = 0;
             }
         }
-        if (!ok) return;
+        if (!ok) return gt_settle(leader, bars.done);
         tc_commit_if(leader, bars.acc_full + buf);
         if (leader) *bars.progress = tiles + 1;
     }
@@ -663,10 +669,46 @@ __device__ __forceinline__ void gt_roles(const GtProblem& gt, const GtArgs& p, c
     });
 }
 
+// Self-test: the MMAs of three tiles of one row, of zeros.  The third finds no accumulator free; the MMAs of the first two are over when the
+// warp comes back.
+constexpr int GT_PROBE_STAGES = 2, GT_PROBE_SMEM = GT_PROBE_STAGES * GtType<float>::A_BYTES + GtType<float>::b_bytes(16) + GT_CONTROL;
+__device__ const long long gt_probe_offsets[] = {0, 1, 2, 3};
+__global__ void __launch_bounds__(32) oeq_grouped_issue_probe(const __grid_constant__ GtProblem gt) {
+    extern __shared__ __align__(1024) unsigned char gt_smem[];
+    const int lane = threadIdx.x;
+    unsigned char *b = gt_smem + GT_PROBE_STAGES * GtType<float>::A_BYTES, *control = b + GtType<float>::b_bytes(16);
+    const GtBars bars(control);
+    for (int i = lane; i < (GT_PROBE_SMEM - GT_CONTROL) / 16; i += 32) reinterpret_cast<uint4*>(gt_smem)[i] = make_uint4(0, 0, 0, 0);
+    fence_async_smem();
+    if (lane == 0) {
+        for (int i = 0; i < GT_PROBE_STAGES; ++i) {
+            mbar_init(bars.full + i, 1);
+            mbar_init(bars.empty + i, 1);
+            mbar_init(bars.acc_full + i, 1);
+        }
+        mbar_init(bars.done, 1);
+        fence_mbar_init();
+        for (int i = 0; i < GT_PROBE_STAGES; ++i) mbar_arrive(bars.full + i);
+    }
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(bars.tmem)), "n"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tc_fence_before();
+    __syncwarp();
+    tc_fence_after();
+    const unsigned tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile unsigned*>(bars.tmem), 0);
+    const GtArgs p{nullptr, nullptr, nullptr, gt_probe_offsets, nullptr, 3, 3, 0};
+    gt_multiply<float, false>(gt, p, gt.target[0], gt.gp.target[0], gt_smem, b, bars, GtWalk(gt_probe_offsets, 0, 0, 3), 128, tmem, elect_lane(), [&](int, unsigned) { return false; });
+    const bool over = mbar_test(bars.done, 0);
+    if (lane == 0) atomicCAS(&gt_status, 0, over ? ERR_GT_ACC_EMPTY : ERR_GT_DONE);
+    tc_fence_before();
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+}
+
 // Self-test: the drain of three tiles of one row, whose accumulators hold anything.  Warp `lost` has its waits run out, the others have
 // theirs complete; all come back.
 constexpr int GT_PROBE_ROWS = 3, GT_PROBE_COLUMNS = 80;
-__device__ const long long gt_probe_offsets[GT_PROBE_ROWS + 1] = {0, 1, 2, 3};
 __device__ float gt_probe_z[GT_PROBE_ROWS * GT_PROBE_COLUMNS];
 __global__ void __launch_bounds__(32 * GT_EPI) oeq_grouped_drain_probe(const __grid_constant__ GtProblem gt, int lost) {
     __shared__ __align__(1024) unsigned char smem[GT_EPI_GROUPS * GT_STAGING + GT_CONTROL];
@@ -720,6 +762,7 @@ __global__ void __launch_bounds__(GT_THREADS, 1) oeq_grouped_tc(const __grid_con
             mbar_init(bars.acc_empty + i, GT_EPI);
         }
         for (int i = 0; i < GT_SETS; ++i) mbar_init(bars.turn + i, GT_SET);
+        mbar_init(bars.done, 1);
         *bars.progress = 0;
         fence_mbar_init();
     }
@@ -736,7 +779,9 @@ __global__ void __launch_bounds__(GT_THREADS, 1) oeq_grouped_tc(const __grid_con
     const unsigned tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile unsigned*>(bars.tmem), 0);
     const GtWalk walk(p.offsets, range.g, work ? (int)range.lo : 0, work ? (int)range.hi : 0);
     if (warp > MMA_WARP) gt_ahead<T, TRANS>(gt, p, tile_of, to, n0, bars, walk, gt_tile_rows(d), tid - (MMA_WARP + 1) * 32);
-    else if (warp == MMA_WARP) gt_multiply<T, TRANS>(gt, p, tile_of, to, a_base, b_base, bars, walk, gt_tile_rows(d), tmem, elect_lane());
+    else if (warp == MMA_WARP) gt_multiply<T, TRANS>(gt, p, tile_of, to, a_base, b_base, bars, walk, gt_tile_rows(d), tmem, elect_lane(), [&](int buf, unsigned parity) {
+        return warp_wait(true, bars.acc_empty + buf, parity, &gt_status, ERR_GT_ACC_EMPTY);
+    });
     else if (d == 1) gt_roles<T, TRANS, FAST, 1>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
     else if (d == 3) gt_roles<T, TRANS, FAST, 3>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
     else if (d == 5) gt_roles<T, TRANS, FAST, 5>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);

@@ -549,6 +549,18 @@ int oeq_grouped_check(void) {
     return oeq_fail(OEQ_ERR_DEVICE_WAIT, "a kernel abandoned a bounded wait (code " + std::to_string(code) + ")");
 }
 
+int oeq_selftest_grouped_issue(void* stream) {
+    if (int rc = allow_smem<oeq_grouped_issue_probe>(GT_PROBE_SMEM)) return rc;
+    GtProblem gt{};
+    gt.gp.n_targets = gt.gp.n_paths = 1;
+    gt.gp.target[0] = {0, 16, 1, 0, 1, 1.0};
+    gt.gp.path[0] = {0, 16, 0, 0, 16, 0};
+    gt.target[0] = {1, 16, 1, 0, GT_PROBE_STAGES, 1, 1, 0};
+    oeq_grouped_issue_probe<<<1, 32, GT_PROBE_SMEM, (cudaStream_t)stream>>>(gt);
+    OEQ_CUDA(cudaGetLastError());
+    return OEQ_OK;
+}
+
 int oeq_selftest_grouped_drain(int warp, void* stream) {
     if (warp < -1 || warp >= GT_EPI) return oeq_fail(OEQ_ERR_INVALID, "warp must be in -1 .. " + std::to_string(GT_EPI - 1));
     for (const int channels : {16, GT_PROBE_COLUMNS}) {         // one chunk of a tile (a group has none in turn) and three

@@ -554,3 +554,11 @@ def test_a_warp_whose_wait_runs_out_comes_to_its_barriers(warp):
         with pytest.raises(_native.OeqError, match="bounded wait"):
             oeq.GroupedLinear.check_device_status()
     check_linear("8x0e", "8x0e", F32, 70, 3)
+
+
+def test_products_on_their_way_are_over_before_a_kernel_gives_up():
+    from openequivariance_b200 import _native
+    assert _native.lib().oeq_selftest_grouped_issue(torch.cuda.current_stream().cuda_stream) == _native.OEQ_OK
+    with pytest.raises(_native.OeqError, match="code 84"):
+        oeq.GroupedLinear.check_device_status()
+    check_linear("8x0e", "8x0e", F32, 70, 3)
