@@ -247,7 +247,7 @@ int oeq_grouped_forward(oeq_grouped* h, int dtype, int64_t rows, int64_t groups,
 int oeq_grouped_backward_input(oeq_grouped* h, int dtype, int64_t rows, int64_t groups, const void* dZ, const void* W,
                                const int64_t* order, const int64_t* offsets, const int32_t* blocks, void* dX, void* stream);
 /* dW from X and dZ, every weight of every group (zeros for groups without rows), summed in a fixed order.  The workspace
- * (oeq_grouped_workspace_bytes, of the current device) is free again after the call's launches. */
+ * (oeq_grouped_workspace_bytes, of the current device; aligned to 32 bytes) is free again after the call's launches. */
 size_t oeq_grouped_workspace_bytes(const oeq_grouped* h, int dtype, int64_t rows, int64_t groups);
 int oeq_grouped_backward_weights(oeq_grouped* h, int dtype, int64_t rows, int64_t groups, const void* X, const void* dZ,
                                  const int64_t* order, const int64_t* offsets, void* dW, void* workspace,

@@ -29,7 +29,7 @@ namespace {
     } while (0)
 
 constexpr int64_t MOST_ROWS = (int64_t(1) << 31) - 1;
-constexpr size_t SMEM_MOST = 227 * 1024;
+constexpr size_t SMEM_MOST = 227 * 1024, WORKSPACE_ALIGN = 32;
 
 size_t elem_bytes(int dtype) { return dtype == OEQ_F64 ? 8 : (dtype == OEQ_F32 ? 4 : 2); }
 bool known_dtype(int dtype) { return dtype == OEQ_F32 || dtype == OEQ_F64 || dtype == OEQ_BF16 || dtype == OEQ_F16; }
@@ -523,6 +523,8 @@ int oeq_grouped_backward_weights(oeq_grouped* h, int dtype, int64_t rows, int64_
     const GpProblem& gp = h->weights;
     if (gp.w_numel == 0) return OEQ_OK;
     if (!offsets || !dW || (rows > 0 && (!X || !dZ))) return oeq_fail(OEQ_ERR_INVALID, "null pointer");
+    // (partial sums are written and joined in pieces of 16 bytes, four FP64 sums at a time)
+    if (!aligned(workspace, WORKSPACE_ALIGN)) return oeq_fail(OEQ_ERR_INVALID, "workspace must be aligned to " + std::to_string(WORKSPACE_ALIGN) + " bytes");
     const size_t want = oeq_grouped_workspace_bytes(h, dtype, rows, groups);
     if (want == 0 || workspace_bytes < want || !workspace) return oeq_fail(OEQ_ERR_INVALID, "workspace too small");
     const cudaStream_t st = (cudaStream_t)stream;

@@ -109,3 +109,15 @@ def test_selftests_refuse_bad_arguments():
         assert lib.oeq_selftest_grouped_drain(warp, None) == _native.OEQ_ERR_INVALID
     for polls in (0, 2 ** 20 + 1):
         assert lib.oeq_selftest_grouped_wait(polls, None) == _native.OEQ_ERR_INVALID
+
+
+@pytest.mark.parametrize("offset", [4, 8, 16])
+def test_abi_refuses_a_workspace_that_is_not_aligned(offset):
+    """Partial sums are read 32 bytes at a time: an address between faults on the device, so the call ends before a launch."""
+    lib, handle = _native.lib(), C.c_void_p()
+    irrep = (_native._Irrep * 1)(_native._Irrep(4, 1, 1))
+    assert lib.oeq_grouped_create(irrep, 1, irrep, 1, C.byref(handle)) == _native.OEQ_OK
+    some = C.c_void_p(1 << 20)
+    assert lib.oeq_grouped_backward_weights(handle, 1, 5, 2, some, some, None, some, some, C.c_void_p((1 << 20) + offset), 1 << 30, None) == _native.OEQ_ERR_INVALID
+    assert b"aligned to 32 bytes" in lib.oeq_last_error()
+    assert lib.oeq_grouped_destroy(handle) == _native.OEQ_OK
