@@ -140,7 +140,7 @@ def torch_lib():
             t.oeq_torch_call_second.argtypes = [C.c_char_p, _INT]
             t.oeq_torch_conv_gradients.argtypes = [C.c_char_p] + [_I64] * 2 + [_P] * 14 + [C.POINTER(_I64), C.POINTER(_P)]
             t.oeq_torch_grouped_error.restype = C.c_char_p
-            t.oeq_torch_grouped_register.restype, t.oeq_torch_grouped_register.argtypes = _I64, [_P, _I64, _I64]
+            t.oeq_torch_grouped_register.argtypes = [C.c_char_p]
             _torch_lib = t
     return _torch_lib
 

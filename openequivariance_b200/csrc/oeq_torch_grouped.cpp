@@ -10,10 +10,13 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
-#include <deque>
+#include <map>
 #include <mutex>
 #include <optional>
+#include <string>
+#include <string_view>
 #include <tuple>
+#include <vector>
 
 #include "oeq_torch_common.h"
 
@@ -26,23 +29,66 @@ using oeq_torch::index_ptr;
 
 enum Kind { PRODUCT = 0, INPUT = 1, WEIGHTS = 2 };      // F(x, w), T(dz, w), G(x, dz)
 
-// Maps live as long as the process: an autograd graph may hold one after its front end has gone.
+// A map is named by its irreps, "8x0e+4x1o->6x0e+4x1o": a traced graph that is saved holds the name, and another process makes the map when
+// it first meets it.  Maps live as long as the process: an autograd graph may hold one after its front end has gone.
 struct Linear {
+    std::string name;
     oeq_grouped* handle;
     int64_t in, out, numel;
     int64_t width(int64_t kind) const { return kind == PRODUCT ? out : (kind == INPUT ? in : numel); }     // of a result
     int64_t width_a(int64_t kind) const { return kind == INPUT ? out : in; }
     int64_t width_b(int64_t kind) const { return kind == WEIGHTS ? out : numel; }
 };
-std::mutex linear_mutex;
-std::deque<Linear>& linears() {
-    static auto* d = new std::deque<Linear>();
-    return *d;
+// "8x0e+4x1o" -> its blocks and their width; false if it is anything else.
+bool read_irreps(std::string_view s, std::vector<oeq_irrep>& blocks, int64_t& dim) {
+    dim = 0;
+    auto number = [&](int32_t& v) {
+        size_t n = 0;
+        for (v = 0; n < s.size() && n < 9 && s[n] >= '0' && s[n] <= '9'; ++n) v = 10 * v + (s[n] - '0');
+        s.remove_prefix(n);
+        return n > 0;
+    };
+    auto one_of = [&](std::string_view chars) {
+        const char c = !s.empty() && chars.find(s[0]) != chars.npos ? s[0] : '\0';
+        if (c) s.remove_prefix(1);
+        return c;
+    };
+    while (!s.empty()) {
+        oeq_irrep b{};
+        if (!number(b.mul) || !one_of("x") || !number(b.l)) return false;
+        const char parity = one_of("eo");
+        if (!parity) return false;
+        b.parity = parity == 'e' ? 1 : -1;
+        blocks.push_back(b);
+        dim += (int64_t)b.mul * (2 * b.l + 1);
+        if (!s.empty() && (!one_of("+") || s.empty())) return false;
+    }
+    return true;
 }
-const Linear& linear_of(int64_t id, int64_t kind) {
+std::mutex linear_mutex;
+// Makes the map if it is not known yet: an OEQ code (oeq_last_error has the reason).
+int find_linear(std::string_view name, const Linear*& found) {
+    static auto* known = new std::map<std::string, Linear, std::less<>>();      // (elements of a map stay where they are)
     std::lock_guard<std::mutex> lock(linear_mutex);
-    TORCH_CHECK_VALUE(id >= 0 && id < (int64_t)linears().size() && kind >= PRODUCT && kind <= WEIGHTS, "no such linear map");
-    return linears()[id];       // (a deque's elements stay where they are)
+    auto at = known->find(name);
+    if (at == known->end()) {
+        const size_t arrow = name.find("->");
+        std::vector<oeq_irrep> in, out;
+        Linear lin{std::string(name), nullptr, 0, 0, 0};
+        TORCH_CHECK_VALUE(arrow != name.npos && read_irreps(name.substr(0, arrow), in, lin.in) && read_irreps(name.substr(arrow + 2), out, lin.out),
+                          "a linear map is named by its irreps, as in 8x0e+4x1o->6x0e, got ", name);
+        if (int rc = oeq_grouped_create(in.data(), (int)in.size(), out.data(), (int)out.size(), &lin.handle)) return rc;
+        lin.numel = oeq_grouped_weight_numel(lin.handle);
+        at = known->emplace(lin.name, lin).first;
+    }
+    found = &at->second;
+    return OEQ_OK;
+}
+const Linear& linear_of(std::string_view name, int64_t kind) {
+    TORCH_CHECK_VALUE(kind >= PRODUCT && kind <= WEIGHTS, "no such product of a linear map: ", kind);
+    const Linear* lin = nullptr;
+    check(find_linear(name, lin));
+    return *lin;
 }
 
 int dtype_of(at::ScalarType t) {
@@ -93,9 +139,8 @@ std::tuple<Tensor, Tensor, Tensor> row_groups_from_counts_cuda(const Tensor& cou
 }
 
 // ---------------------------------------------------------------- the product and its gradients
-Tensor linear_cuda(const Tensor& a_in, const Tensor& b_in, const std::optional<Tensor>& order_in, const Tensor& offsets_in, const Tensor& blocks_in,
-                   int64_t id, int64_t kind) {
-    const Linear& lin = linear_of(id, kind);
+Tensor run_linear(const Linear& lin, const Tensor& a_in, const Tensor& b_in, const std::optional<Tensor>& order_in, const Tensor& offsets_in,
+                  const Tensor& blocks_in, int64_t kind) {
     const int dtype = dtype_of(a_in.scalar_type());
     const char* names[3][2] = {{"rows", "weights"}, {"output gradient", "weights"}, {"rows", "output gradient"}};
     TORCH_CHECK_VALUE(offsets_in.dim() == 1 && offsets_in.size(0) >= 2 && offsets_in.scalar_type() == at::kLong, "offsets must be a 1-D int64 tensor");
@@ -132,17 +177,23 @@ Tensor linear_cuda(const Tensor& a_in, const Tensor& b_in, const std::optional<T
     return out;
 }
 
-using Signature = Tensor(const Tensor&, const Tensor&, const std::optional<Tensor>&, const Tensor&, const Tensor&, int64_t, int64_t);
-
-Tensor call_linear(const Tensor& a, const Tensor& b, const std::optional<Tensor>& order, const Tensor& offsets, const Tensor& blocks, int64_t id,
+Tensor linear_cuda(const Tensor& a, const Tensor& b, const std::optional<Tensor>& order, const Tensor& offsets, const Tensor& blocks, std::string_view name,
                    int64_t kind) {
-    if (direct({a, b, offsets, blocks})) return linear_cuda(a, b, order, offsets, blocks, id, kind);
+    return run_linear(linear_of(name, kind), a, b, order, offsets, blocks, kind);
+}
+
+using Signature = Tensor(const Tensor&, const Tensor&, const std::optional<Tensor>&, const Tensor&, const Tensor&, std::string_view, int64_t);
+
+Tensor call_linear(const Linear& lin, const Tensor& a, const Tensor& b, const std::optional<Tensor>& order, const Tensor& offsets, const Tensor& blocks,
+                   int64_t kind) {
+    if (direct({a, b, offsets, blocks})) return run_linear(lin, a, b, order, offsets, blocks, kind);
     static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("openequivariance_b200::grouped_linear", "").typed<Signature>();
-    return op.call(a, b, order, offsets, blocks, id, kind);
+    return op.call(a, b, order, offsets, blocks, lin.name, kind);
 }
 
 struct LinearNode final : torch::autograd::Node {
-    int64_t id, kind;
+    const Linear* lin;
+    int64_t kind;
     bool has_order;
     torch::autograd::SavedVariable a, b, order, offsets, blocks;
     std::string name() const override { return "OeqGroupedLinearBackward"; }
@@ -160,7 +211,7 @@ struct LinearNode final : torch::autograd::Node {
             blk = blocks.unpack();
             if (has_order) ord = order.unpack();
         }
-        auto call = [&](int64_t k, const Tensor& p, const Tensor& q) { return call_linear(p, q, ord, off, blk, id, k); };
+        auto call = [&](int64_t k, const Tensor& p, const Tensor& q) { return call_linear(*lin, p, q, ord, off, blk, k); };
         Tensor ga, gb;
         if (task_should_compute_output(0)) ga = kind == PRODUCT ? call(INPUT, e, y) : (kind == INPUT ? call(PRODUCT, e, y) : call(INPUT, y, e));
         if (task_should_compute_output(1)) gb = kind == PRODUCT ? call(WEIGHTS, x, e) : (kind == INPUT ? call(WEIGHTS, e, x) : call(PRODUCT, x, e));
@@ -168,15 +219,15 @@ struct LinearNode final : torch::autograd::Node {
     }
 };
 
-Tensor linear_autograd(const Tensor& a, const Tensor& b, const std::optional<Tensor>& order, const Tensor& offsets, const Tensor& blocks, int64_t id,
-                       int64_t kind) {
+Tensor linear_autograd(const Tensor& a, const Tensor& b, const std::optional<Tensor>& order, const Tensor& offsets, const Tensor& blocks,
+                       std::string_view name, int64_t kind) {
     TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(a) && !torch::autograd::isFwGradDefined(b),
                                 "openequivariance_b200: the operators have no forward-mode derivative");
     static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("openequivariance_b200::grouped_linear", "").typed<Signature>();
     std::shared_ptr<LinearNode> node;
     if (at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad())) {
         node = std::shared_ptr<LinearNode>(new LinearNode(), torch::autograd::deleteNode);
-        node->id = id;
+        node->lin = &linear_of(name, kind);
         node->kind = kind;
         node->has_order = order.has_value();
         node->a = torch::autograd::SavedVariable(a, false);
@@ -188,7 +239,7 @@ Tensor linear_autograd(const Tensor& a, const Tensor& b, const std::optional<Ten
     }
     Tensor out = [&] {
         at::AutoDispatchBelowADInplaceOrView guard;
-        return op.call(a, b, order, offsets, blocks, id, kind);
+        return op.call(a, b, order, offsets, blocks, name, kind);
     }();
     if (node) torch::autograd::set_history(out, node);
     return out;
@@ -202,7 +253,7 @@ TORCH_LIBRARY_FRAGMENT(openequivariance_b200, m) {
     const std::vector<at::Tag> tags{at::Tag::pt2_compliant_tag};
     m.def("row_groups(Tensor index, int groups) -> (Tensor, Tensor, Tensor, Tensor)", tags);
     m.def("row_groups_from_counts(Tensor counts, int rows) -> (Tensor, Tensor, Tensor)", tags);
-    m.def("grouped_linear(Tensor a, Tensor b, Tensor? order, Tensor offsets, Tensor blocks, int linear, int kind) -> Tensor", tags);
+    m.def("grouped_linear(Tensor a, Tensor b, Tensor? order, Tensor offsets, Tensor blocks, str map, int kind) -> Tensor", tags);
 }
 TORCH_LIBRARY_IMPL(openequivariance_b200, CUDA, m) {
     m.impl("row_groups", TORCH_FN(row_groups_cuda));
@@ -215,12 +266,11 @@ extern "C" {
 
 const char* oeq_torch_grouped_error() { return grouped_error.c_str(); }
 
-// Makes a map known to the ops: its number, or -1.
-int64_t oeq_torch_grouped_register(oeq_grouped* handle, int64_t in, int64_t out) {
+// Makes a map known to the ops, so that what cannot be made is refused before a call: an OEQ code, or -1 (oeq_torch_grouped_error).
+int oeq_torch_grouped_register(const char* name) {
     try {
-        std::lock_guard<std::mutex> lock(linear_mutex);
-        linears().push_back({handle, in, out, oeq_grouped_weight_numel(handle)});
-        return (int64_t)linears().size() - 1;
+        const Linear* lin = nullptr;
+        return find_linear(name, lin);
     } catch (const std::exception& e) {
         grouped_error = e.what();
         return -1;

@@ -13,8 +13,7 @@ The reference has no counterpart; its users index the weights by row (``w[specie
 
 from __future__ import annotations
 
-import ctypes as C
-import threading
+import functools
 
 import torch
 
@@ -23,8 +22,22 @@ from .irreps import Irreps
 from .tensor_product import _require_cuda
 
 
-_widths = []        # of each map: results of the product, its input gradient and its weight gradient
-_numbers, _register_lock = {}, threading.Lock()
+def _paths(irreps_in, irreps_out):
+    """(input block, output block, slice of the weights, shape) of every pair of blocks with the same irrep."""
+    paths, at = [], 0
+    for i, (mul_in, ir_in) in enumerate(irreps_in):
+        for o, (mul_out, ir_out) in enumerate(irreps_out):
+            if ir_in == ir_out and mul_in * mul_out > 0:
+                paths.append((i, o, slice(at, at + mul_in * mul_out), (mul_in, mul_out)))
+                at += mul_in * mul_out
+    return paths, at
+
+
+@functools.lru_cache(maxsize=None)
+def _widths(name):
+    """Of the results of a map's product, its input gradient and its weight gradient."""
+    irreps_in, irreps_out = (Irreps(part) for part in name.split("->"))
+    return irreps_out.dim, irreps_in.dim, _paths(irreps_in, irreps_out)[1]
 
 
 def _ops():
@@ -45,8 +58,8 @@ def _ops():
                 counts.new_empty((blocks_of(rows, groups), 3), dtype=torch.int32))
 
     @torch.library.register_fake("openequivariance_b200::grouped_linear")
-    def _(a, b, order, offsets, blocks, linear, kind):
-        return a.new_empty(offsets.shape[0] - 1 if kind == 2 else a.shape[0], _widths[linear][kind])
+    def _(a, b, order, offsets, blocks, map, kind):
+        return a.new_empty(offsets.shape[0] - 1 if kind == 2 else a.shape[0], _widths(map)[kind])
 
     return ns.row_groups.default, ns.row_groups_from_counts.default, ns.grouped_linear.default
 
@@ -89,26 +102,13 @@ class RowGroups:
         return self
 
 
-def _register(irreps_in: Irreps, irreps_out: Irreps) -> int:
-    """The map's number.  Maps are kept for the life of the process, as a compiled or an autograd graph may hold one."""
-    with _register_lock:
-        if (irreps_in, irreps_out) not in _numbers:
-            _numbers[irreps_in, irreps_out] = _new_map(irreps_in, irreps_out)
-        return _numbers[irreps_in, irreps_out]
-
-
-def _new_map(irreps_in, irreps_out):
-    def array(irreps):
-        return (_native._Irrep * max(1, len(irreps)))(*[_native._Irrep(mul, ir.l, ir.p) for mul, ir in irreps])
-
-    handle, library = C.c_void_p(), _native.lib()
-    _native.check(library.oeq_grouped_create(array(irreps_in), len(irreps_in), array(irreps_out), len(irreps_out), C.byref(handle)))
-    number = _native.torch_lib().oeq_torch_grouped_register(handle, irreps_in.dim, irreps_out.dim)
-    if number < 0:
-        raise RuntimeError(_native.torch_lib().oeq_torch_grouped_error().decode(errors="replace"))
-    assert number == len(_widths)
-    _widths.append((irreps_out.dim, irreps_in.dim, library.oeq_grouped_weight_numel(handle)))
-    return number
+def _register(name):
+    """Makes the map known, which refuses what cannot be made.  Maps are kept for the life of the process."""
+    library = _native.torch_lib()
+    code = library.oeq_torch_grouped_register(name.encode())
+    if code < 0:
+        raise RuntimeError(library.oeq_torch_grouped_error().decode(errors="replace"))
+    _native.check(code)
 
 
 class GroupedLinear:
@@ -127,25 +127,26 @@ class GroupedLinear:
     rounded once) and float64; the type is that of the tensors.  Derivatives of any order; gradients of weights are summed
     in a fixed order, so every result is the same in every run.  In float32 an infinity, a NaN or a number within 2^-12 of
     the largest one gives NaN in the results that it has a part in.
+
+    An exported or pickled call holds the map's irreps and means the same map in every process that has imported this module.
     """
 
     def __init__(self, irreps_in, irreps_out):
         self.irreps_in, self.irreps_out = Irreps(irreps_in), Irreps(irreps_out)
-        self.paths, at = [], 0
-        for i, (mul_in, ir_in) in enumerate(self.irreps_in):
-            for o, (mul_out, ir_out) in enumerate(self.irreps_out):
-                if ir_in == ir_out and mul_in * mul_out > 0:
-                    self.paths.append((i, o, slice(at, at + mul_in * mul_out), (mul_in, mul_out)))
-                    at += mul_in * mul_out
-        self.weight_numel = at
-        self._number = _register(self.irreps_in, self.irreps_out)
+        self.paths, self.weight_numel = _paths(self.irreps_in, self.irreps_out)
+        self._map = f"{self.irreps_in}->{self.irreps_out}"      # the map as the op takes it: the same in every process
+        _register(self._map)
+
+    @property
+    def _number(self):
+        return self._map
 
     def forward(self, x: torch.Tensor, weights: torch.Tensor, groups: RowGroups) -> torch.Tensor:
         if not x.is_cuda or not weights.is_cuda:
             _require_cuda(x, weights)
         if x.dim() != 2 or x.shape[0] != groups.rows:
             raise ValueError(f"rows must be [{groups.rows}, {self.irreps_in.dim}], got {tuple(x.shape)}")
-        return _grouped_linear(x, weights, groups.order, groups.offsets, groups.blocks, self._number, 0)
+        return _grouped_linear(x, weights, groups.order, groups.offsets, groups.blocks, self._map, 0)
 
     __call__ = forward
 

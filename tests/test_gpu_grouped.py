@@ -8,6 +8,7 @@ import torch
 import openequivariance_b200 as oeq
 from openequivariance_b200 import Irreps
 import grouped_reference as ref
+from conftest import ROOT
 
 pytestmark = pytest.mark.gpu
 
@@ -515,6 +516,53 @@ def test_wrong_arguments_raise():
     with pytest.raises(NotImplementedError, match="forward-mode"):
         with torch.autograd.forward_ad.dual_level():
             lin(torch.autograd.forward_ad.make_dual(cuda(10, 8), cuda(10, 8)), cuda(3, 32), plan)
+
+
+def test_an_op_makes_the_map_that_it_names():
+    """A map that no GroupedLinear of this process has, and names that are none."""
+    names = "13x0e+3x1o", "11x0e+3x1o"
+    x, w, dz, index = (t.cuda() for t in map_inputs(*names, 60, 4))
+    plan = oeq.RowGroups(index, 4)
+    op = torch.ops.openequivariance_b200.grouped_linear
+    z = op(x, w, plan.order, plan.offsets, plan.blocks, "->".join(names), 0)
+    assert torch.equal(z, oeq.GroupedLinear(*names)(x, w, plan))
+    for bad, kind, match in (("13x0e", 0, "named by its irreps"), ("13x0e+3x1o->11x0e+3x1o", 3, "no such product"), ("12x0e->11x0e", 0, "rows must be")):
+        with pytest.raises(ValueError, match=match):
+            op(x, w, plan.order, plan.offsets, plan.blocks, bad, kind)
+    with pytest.raises(RuntimeError, match="32 blocks"):
+        op(x, w, plan.order, plan.offsets, plan.blocks, "+".join(["1x0e"] * 33) + "->1x0e", 0)
+
+
+def map_inputs(irreps_in, irreps_out, rows, groups):
+    gen = torch.Generator().manual_seed(7)
+    a, b = Irreps(irreps_in), Irreps(irreps_out)
+    numel = sum(m * n for m, p in a for n, q in b if p == q)
+    return (torch.randn(rows, a.dim, generator=gen), torch.randn(groups, numel, generator=gen), torch.randn(rows, b.dim, generator=gen),
+            torch.randint(0, groups, (rows,), generator=gen))
+
+
+def test_an_exported_program_in_another_process(tmp_path):
+    """The other process has made another map of the same widths before, with other weights in each place."""
+    import subprocess
+    import sys
+    names, other = ("8x0e+8x0e", "4x0e+4x0e"), ("16x0e", "8x0e")
+    x, w, _, index = (t.cuda() for t in map_inputs(*names, 50, 3))
+    lin = oeq.GroupedLinear(*names)
+
+    class Call(torch.nn.Module):
+        def forward(self, x, w, index):
+            return lin(x, w, oeq.RowGroups(index, 3))
+
+    torch.export.save(torch.export.export(Call(), (x, w, index)), tmp_path / "call.pt2")
+    torch.save((x.cpu(), w.cpu(), index.cpu()), tmp_path / "in.pt")
+    code = f"""
+import torch, openequivariance_b200 as oeq
+oeq.GroupedLinear({other[0]!r}, {other[1]!r})
+x, w, index = (t.cuda() for t in torch.load({str(tmp_path / 'in.pt')!r}))
+torch.save(torch.export.load({str(tmp_path / 'call.pt2')!r}).module()(x, w, index).cpu(), {str(tmp_path / 'out.pt')!r})
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=ROOT)
+    assert torch.equal(torch.load(tmp_path / "out.pt"), lin(x, w, oeq.RowGroups(index, 3)).cpu())
 
 
 # ------------------------------------------------------------------------------------------ status

@@ -9,6 +9,7 @@ import torch
 import openequivariance_b200 as oeq
 from openequivariance_b200 import _native
 import grouped_reference as ref
+from conftest import ROOT
 
 
 def test_paths_and_weights():
@@ -121,3 +122,41 @@ def test_abi_refuses_a_workspace_that_is_not_aligned(offset):
     assert lib.oeq_grouped_backward_weights(handle, 1, 5, 2, some, some, None, some, some, C.c_void_p((1 << 20) + offset), 1 << 30, None) == _native.OEQ_ERR_INVALID
     assert b"aligned to 32 bytes" in lib.oeq_last_error()
     assert lib.oeq_grouped_destroy(handle) == _native.OEQ_OK
+
+
+def test_a_map_is_the_same_in_every_process():
+    """What a traced graph holds names the map, whichever maps a process has made before.  The two maps agree in all widths and lay their
+    weights out differently."""
+    import subprocess
+    import sys
+    code = "import sys, openequivariance_b200 as oeq; print([oeq.GroupedLinear(*m.split('/'))._number for m in sys.argv[1:]])"
+    maps = ["8x0e+8x0e/4x0e+4x0e", "16x0e/8x0e"]
+    run = lambda names: eval(subprocess.run([sys.executable, "-c", code, *names], capture_output=True, text=True, check=True, cwd=ROOT).stdout)
+    first, second = run(maps), run(maps[::-1])
+    assert first == second[::-1] and first[0] != first[1]
+
+
+def test_a_traced_call_holds_the_irreps():
+    from torch._subclasses import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    lin = oeq.GroupedLinear("8x0e+4x1o", "6x0e+4x1o")
+    with FakeTensorMode():
+        x, w, index = torch.empty(10, 20, device="cuda"), torch.empty(3, 64, device="cuda"), torch.zeros(10, dtype=torch.int64, device="cuda")
+        graph = make_fx(lambda x, w, index: lin(x, w, oeq.RowGroups(index, 3)))(x, w, index).graph
+    calls = [n for n in graph.nodes if "grouped_linear" in str(n.target)]
+    assert len(calls) == 1 and "8x0e+4x1o->6x0e+4x1o" in calls[0].args
+
+
+def test_pickled():
+    import pickle
+    lin = pickle.loads(pickle.dumps(oeq.GroupedLinear("3x0e", "5x0e+1x1o")))
+    assert lin._map == "3x0e->5x0e+1x1o" and lin.weight_numel == 15
+
+
+def test_maps_that_are_no_maps_are_refused():
+    from openequivariance_b200 import grouped
+    for name in ("3x0e", "3x0e->3", "3x0e->3x", "3x0e->3x0", "3x0e->3x0x", "3x0e+->3x0e", "-1x0e->1x0e", "1x0e->1x0e ", "9999999999x0e->1x0e", "a->b"):
+        with pytest.raises(RuntimeError, match="named by its irreps"):
+            grouped._register(name)
+    grouped._register("->")
+    grouped._register("12x0e->")
