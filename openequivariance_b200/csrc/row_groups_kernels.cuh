@@ -21,6 +21,11 @@ namespace oeq {
 constexpr int RG_BLOCK = 64;                    // rows of an entry of the block table
 constexpr int RG_SMALL_WARPS = 32, RG_WARPS = 4, RG_RUNS = 1184;           // most runs: eight warps an SM
 
+// Blocks of a group of n rows (up to 2^31 - 1 of them: n + 63 would leave the range of an int).
+__host__ __device__ constexpr int rg_group_blocks(int n) { return n / RG_BLOCK + (n % RG_BLOCK != 0); }
+static_assert(rg_group_blocks(0) == 0 && rg_group_blocks(1) == 1 && rg_group_blocks(64) == 1 && rg_group_blocks(65) == 2, "blocks of a group");
+static_assert(rg_group_blocks(0x7fffffff) == 1 << 25 && rg_group_blocks(0x7fffffff - 63) == (1 << 25) - 1, "blocks of a group");
+
 __device__ __forceinline__ int rg_key(const long long* __restrict__ index, long long r, int groups) {
     const long long g = index[r];
     return g >= 0 && g < groups ? (int)g : groups;
@@ -74,7 +79,7 @@ __device__ __forceinline__ int rg_find(const int* a, int n, int v) {
 // overwritten with the number of blocks before each group's.
 __device__ __forceinline__ void rg_tables(const int* offsets, int* first, int* part, int groups, int blocks, long long* __restrict__ offsets_out,
                                           int* __restrict__ table, long long thread, long long threads) {
-    for (int g = threadIdx.x; g < groups; g += blockDim.x) first[g] = (offsets[g + 1] - offsets[g] + RG_BLOCK - 1) / RG_BLOCK;
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) first[g] = rg_group_blocks(offsets[g + 1] - offsets[g]);
     __syncthreads();
     rg_scan(first, groups, part);
     for (long long g = thread; g <= groups; g += threads) offsets_out[g] = offsets[g];

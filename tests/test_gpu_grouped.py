@@ -470,6 +470,29 @@ def test_more_than_2_to_the_31_values():
     assert bool(((z[at.cuda()].cpu().double() - want).abs() <= ref.allowed(BF16, want, size, 128)).all())
 
 
+def test_one_group_of_all_the_rows_there_can_be():
+    """2^31 - 1 rows: the group's number of blocks, and a product that goes by the table of blocks (float64) and one that does not."""
+    rows = 2 ** 31 - 1
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("needs 100 GB")
+    plan = oeq.RowGroups.from_counts(torch.tensor([rows, 0], device="cuda"), rows)
+    used = 2 ** 25
+    assert plan.blocks.shape == (used + 1, 3) and plan.offsets.tolist() == [0, rows, rows]
+    assert plan.blocks[-2:].tolist() == [[0, rows - 63, 63], [-1, 0, 0]]
+    assert not plan.blocks[:used, 0].any() and bool((plan.blocks[:used - 1, 2] == 64).all())
+    assert torch.equal(plan.blocks[:used, 1], torch.arange(0, rows, 64, dtype=torch.int32, device="cuda"))
+    lin = oeq.GroupedLinear("1x0e", "1x0e")
+    for dtype in (F64, BF16):
+        x = torch.empty(rows, 1, dtype=dtype, device="cuda")
+        for part in x.split(1 << 28):
+            part.copy_((torch.arange(len(part), device="cuda") % 200)[:, None])
+        z = lin(x, torch.tensor([[-2.0], [5.0]], dtype=dtype, device="cuda"), plan)
+        assert all(torch.equal(p, q * -2) for p, q in zip(z.split(1 << 28), x.split(1 << 28)))
+        del x, z, part
+    del plan
+    torch.cuda.empty_cache()
+
+
 # ------------------------------------------------------------------------------------------ the ops
 
 def test_ops():
