@@ -18,7 +18,7 @@
 //   * 8 epilogue warps, in two groups, add those, scale, and write rows through shared memory, so that a row's values leave in order.
 //   * 3 warps prefetch rows and weights to L2, up to two tiles ahead of the MMAs: a producer's loads are half of its time, and registers for
 //     more of them on the way there are none.
-// Two accumulators: a tile drains while the next is computed.  Every wait is bounded; on expiry a role records a code and all
+// Two accumulators: a tile (FP32: up to 256 channels of its sum) drains while the next is computed.  Every wait is bounded; on expiry a role records a code and all
 // leave.
 // Measured from a cold L2, 50 000 rows in 10 groups, 128x(0e+1o+2e+3o) FP32: 219 us (3.7 TB/s of rows in and out, 120 TFLOP/s); 100 000 rows in 256
 // groups, 128x(0e+1o+2e) BF16: 143 us (3.4 TB/s).  The load and store unit bounds it (71 % of its wavefronts: rows of several components are read
@@ -32,6 +32,10 @@ namespace oeq {
 constexpr int GT_D_MAX = 7;
 constexpr int GT_SETS = 3, GT_SET = 4, GT_PW = GT_SETS * GT_SET, GT_EPI_GROUPS = 2, GT_EPI = 4 * GT_EPI_GROUPS, GT_AHEAD = 3, GT_THREADS = (GT_PW + GT_EPI + 1 + GT_AHEAD) * 32;
 constexpr int GT_STAGES = 6;                    // most stages of A
+// FP32: chunks of the sum in one accumulator, 32 additions of eight channels each.  The additions are cut off, not rounded, and all of them
+// one way: relative error (norm) 6.4e-7 at 256 channels, in one chain 4.9e-6 at 2 048 and 9.6e-6 at 4 096.  (16-bit results are rounded to
+// 2^-9 and coarser; their sums are one chain.)
+constexpr int GT_CHAIN = 8;
 constexpr int GT_STAGING = 42 * 100 * 4;        // 32 channels of a tile's pairs (three components take most), for each epilogue group
 constexpr int GT_CONTROL = 1536;                // barriers, rows of the tiles that drain, the CTA's range
 constexpr int ERR_GT_EMPTY = 81, ERR_GT_FULL = 82, ERR_GT_ACC_FULL = 83, ERR_GT_ACC_EMPTY = 84, ERR_GT_TURN = 85, ERR_GT_DONE = 86;
@@ -434,18 +438,28 @@ __device__ __forceinline__ void gt_multiply(const GtProblem& gt, const GtArgs& p
     const bool resident = tile_of.chunks <= tile_of.slots;
     const unsigned wide = gt_idesc<T, B_MN>(acc), narrow = gt_idesc<T, B_MN>(n);
     const unsigned long long a0 = tc_smem_desc(smem_u32(a_base)), b0 = gt_desc_b<T, B_MN>(smem_u32(b_base), n);
-    int stage = 0, use = 0, slot = 0, tiles = 0;
+    int stage = 0, use = 0, slot = 0, tiles = 0, accs = 0;
     for (; walk.more(); walk.next(p.offsets, p.groups), ++tiles) {
         walk.tile(tile_rows);
-        const int buf = tiles & 1;
         bool ok = true;
-        if (tiles >= 2) ok = acc_wait(buf, (unsigned)(tiles / 2 - 1) & 1);
-        const unsigned d = tmem + (unsigned)(buf * 256);
+        if (accs >= 2) ok = acc_wait(accs & 1, (unsigned)(accs / 2 - 1) & 1);
         unsigned accumulate = 0;
+        int in_chain = 0;
         if (resident) slot = 0;
         for (int path_no = to.path_begin; path_no < to.path_end && ok; ++path_no) {
             const int mul = gt.gp.path[path_no].src_mul;
             for (int u0 = 0; u0 < mul && ok; u0 += KC) {
+                if (GtType<T>::SPLIT && in_chain++ == GT_CHAIN) {       // the next accumulator
+                    tc_commit_if(leader, bars.acc_full + (accs & 1));
+                    ++accs;
+                    if (accs >= 2 && !acc_wait(accs & 1, (unsigned)(accs / 2 - 1) & 1)) {
+                        ok = false;
+                        break;
+                    }
+                    accumulate = 0;
+                    in_chain = 1;
+                }
+                const unsigned d = tmem + (unsigned)((accs & 1) * 256);
                 ok = warp_wait(ok, bars.full + stage, (unsigned)use & 1, &gt_status, ERR_GT_FULL);
                 if (!ok) break;
                 tc_fence_after();
@@ -466,7 +480,8 @@ __device__ __forceinline__ void gt_multiply(const GtProblem& gt, const GtArgs& p
             }
         }
         if (!ok) return gt_settle(leader, bars.done);
-        tc_commit_if(leader, bars.acc_full + buf);
+        tc_commit_if(leader, bars.acc_full + (accs & 1));
+        ++accs;
         if (leader) *bars.progress = tiles + 1;
     }
 }
@@ -490,6 +505,27 @@ template <> struct GtPair<__half> {
 // component: a lane writes whole pieces), else rows with 16 bytes of padding (a lane writes single values; two lanes meet in a bank).
 template <int D> __host__ __device__ constexpr int gt_pitch() { return D == 1 ? 32 : 32 * D + 4; }
 template <int D> __device__ __forceinline__ int gt_staged(int r, int i) { return D == 1 ? r * 32 + ((i ^ (4 * (r & 7)))) : r * gt_pitch<D>() + i; }
+
+// Rows of a tile, added to what stands there: each value by the thread that wrote it (gt_write; the same group of warps), so that no other
+// thread has to see it and the additions have one order.
+template <int D, bool VEC>
+__device__ __forceinline__ void gt_add(const float* staging, const int* rows_of, int rows, float* z_col, int dim, int values, int thread) {
+    constexpr int V = VEC ? 4 : 1, ROW = 32 * D / V;
+#pragma unroll 2
+    for (int i = thread; i < rows * ROW; i += 128) {
+        const int r = i / ROW, c = (i - r * ROW) * V;
+        if (c >= values) continue;
+        float* z = z_col + (long long)rows_of[r] * dim + c;
+        if constexpr (VEC) {
+            const float4 v = *reinterpret_cast<const float4*>(staging + gt_staged<D>(r, c));
+            float4 s = *reinterpret_cast<const float4*>(z);
+            s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+            *reinterpret_cast<float4*>(z) = s;
+        } else {
+            *z += staging[gt_staged<D>(r, c)];
+        }
+    }
+}
 
 // Rows of a tile from shared memory by the 128 threads of a group.  VEC: 16 bytes a thread; U of them are on the way together, past the
 // last one the last one again (the same values to the same place).
@@ -585,7 +621,8 @@ __device__ __forceinline__ void gt_ahead(const GtProblem& gt, const GtArgs& p, c
 }
 
 // ---------------------------------------------------------------------------- epilogue
-// The chunks of 32 channels of all tiles go to the two groups of four warps in turn.
+// The chunks of 32 channels of all tiles go to the two groups of four warps in turn.  FP32: a tile whose sum has several chains comes as
+// as many accumulators; the results of the first are written and the others added to them, a chunk of channels by the same group each time.
 // acc_wait(buffer, parity): the warp's wait for an accumulator.  A warp whose wait ran out reads and writes nothing more but comes to every
 // barrier of its group: each warp counts its own polls, so the other three may have seen the accumulator complete, and a hardware barrier
 // waits without limit.  (It keeps the rows' numbers up to date: the others write the rows that stand there.)
@@ -598,64 +635,77 @@ __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, c
     const unsigned quarter = tmem + ((unsigned)(warp * 32) << 16);
     int* rows_of = bars.rows + 128 * group;
     staging += group * (GT_STAGING / 4);
-    int tiles = 0, turn = 0;
+    const int chains = GtType<T>::SPLIT ? max(1, (tile_of.chunks + GT_CHAIN - 1) / GT_CHAIN) : 1;
+    int accs = 0, first_turn = 0;
     bool alive = true;
-    for (; walk.more(); walk.next(p.offsets, p.groups), ++tiles) {
+    for (; walk.more(); walk.next(p.offsets, p.groups)) {
         walk.tile(TILE_ROWS);
-        const int buf = tiles & 1;
         if (pair < walk.rows) rows_of[pair] = (int)gp_row(p.order, walk.pos + pair);         // (read behind the first barrier below)
-        alive = alive && acc_wait(buf, (unsigned)(tiles / 2) & 1);
-        tc_fence_after();
-        bool mine = false;
-        for (int w0 = 0; w0 < mul; w0 += 32, turn ^= 1) {
-            if (turn != group) continue;
-            mine = true;
-            const bool last = w0 + 32 * GT_EPI_GROUPS >= mul;           // the group has read its part of the accumulator then
-            float* to_smem = staging + r_of * PITCH + k_of;
+        int turn = first_turn;
+        for (int chain = 0; chain < chains; ++chain, ++accs) {
+            const int buf = accs & 1;
+            alive = alive && acc_wait(buf, (unsigned)(accs / 2) & 1);
+            tc_fence_after();
+            bool mine = false;
+            turn = first_turn;
+            for (int w0 = 0; w0 < mul; w0 += 32, turn ^= 1) {
+                if (turn != group) continue;
+                mine = true;
+                const bool last = w0 + 32 * GT_EPI_GROUPS >= mul;       // the group has read its part of the accumulator then
+                float* to_smem = staging + r_of * PITCH + k_of;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                unsigned v[16], u[GtType<T>::SPLIT ? 16 : 1];
-                const unsigned at = quarter + (unsigned)(buf * 256 + w0 + 16 * h);
-                if (alive && w0 + 16 * h < n) {
-                    tc_load16(at, v);
-                    if constexpr (GtType<T>::SPLIT) tc_load16(at + n, u);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                }
-                if (alive && last && h == 1) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bars.acc_empty + buf);
-                }
-                if (alive && w0 + 16 * h < n && r_of < walk.rows) {
-                    float s[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        if constexpr (GtType<T>::SPLIT) s[j] = __uint_as_float(v[j]) + __uint_as_float(u[j]);
-                        else s[j] = __uint_as_float(v[j]) * scale;
+                for (int h = 0; h < 2; ++h) {
+                    unsigned v[16], u[GtType<T>::SPLIT ? 16 : 1];
+                    const unsigned at = quarter + (unsigned)(buf * 256 + w0 + 16 * h);
+                    if (alive && w0 + 16 * h < n) {
+                        tc_load16(at, v);
+                        if constexpr (GtType<T>::SPLIT) tc_load16(at + n, u);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     }
+                    if (alive && last && h == 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bars.acc_empty + buf);
+                    }
+                    if (alive && w0 + 16 * h < n && r_of < walk.rows) {
+                        float s[16];
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        if constexpr (D == 1) *reinterpret_cast<float4*>(staging + gt_staged<1>(r_of, 16 * h + j)) = make_float4(s[j], s[j + 1], s[j + 2], s[j + 3]);
-                        else {
+                        for (int j = 0; j < 16; ++j) {
+                            if constexpr (GtType<T>::SPLIT) s[j] = __uint_as_float(v[j]) + __uint_as_float(u[j]);
+                            else s[j] = __uint_as_float(v[j]) * scale;
+                        }
 #pragma unroll
-                            for (int i = j; i < j + 4; ++i) to_smem[(16 * h + i) * D] = s[i];
+                        for (int j = 0; j < 16; j += 4) {
+                            if constexpr (D == 1) *reinterpret_cast<float4*>(staging + gt_staged<1>(r_of, 16 * h + j)) = make_float4(s[j], s[j + 1], s[j + 2], s[j + 3]);
+                            else {
+#pragma unroll
+                                for (int i = j; i < j + 4; ++i) to_smem[(16 * h + i) * D] = s[i];
+                            }
                         }
                     }
                 }
+                group_sync(1 + group, 128);
+                const int values = min(32, mul - w0) * D;
+                T* z = static_cast<T*>(p.Z) + to.off + (n0 + w0) * D;
+                const bool vec = p.z_vec && (to.off | values) % (16 / (int)sizeof(T)) == 0;
+                if (alive && chain == 0) {
+                    if (vec) gt_write<T, D, true>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
+                    else gt_write<T, D, false>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
+                } else if (alive) {
+                    if constexpr (GtType<T>::SPLIT) {
+                        if (vec) gt_add<D, true>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
+                        else gt_add<D, false>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
+                    }
+                }
+                group_sync(1 + group, 128);
             }
-            group_sync(1 + group, 128);
-            const int values = min(32, mul - w0) * D;
-            T* z = static_cast<T*>(p.Z) + to.off + (n0 + w0) * D;
-            if (!alive) {}
-            else if (p.z_vec && (to.off | values) % (16 / (int)sizeof(T)) == 0) gt_write<T, D, true>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
-            else gt_write<T, D, false>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
-            group_sync(1 + group, 128);
+            if (!mine) {
+                __syncwarp();
+                if (alive && lane == 0) mbar_arrive(bars.acc_empty + buf);
+                group_sync(1 + group, 128);     // (rows_of is written again by all four warps)
+            }
         }
-        if (!mine) {
-            __syncwarp();
-            if (alive && lane == 0) mbar_arrive(bars.acc_empty + buf);
-            group_sync(1 + group, 128);         // (rows_of is written again by all four warps)
-        }
+        first_turn = turn;
     }
 }
 

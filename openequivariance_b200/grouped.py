@@ -123,7 +123,7 @@ class GroupedLinear:
     normalisation as ``FullyConnectedTPProblem(irreps_in, "1x0e", irreps_out)``.  Rows without a group give zeros, and so
     do output blocks without a path.
 
-    float32 (three TF32 products on the tensor cores, relative error below 1e-6), bfloat16 and float16 (float32 sums,
+    float32 (three TF32 products on the tensor cores; relative error below 1e-6, whatever the number of terms), bfloat16 and float16 (float32 sums,
     rounded once) and float64; the type is that of the tensors.  Derivatives of any order; gradients of weights are summed
     in a fixed order, so every result is the same in every run.  In float32 an infinity, a NaN or a number within 2^-12 of
     the largest one gives NaN in the results that it has a part in.

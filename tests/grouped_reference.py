@@ -79,3 +79,15 @@ def allowed(dtype, want, size, terms):
     split = 2.0 ** -22 + 2 * 2.0 ** -21 if dtype == torch.float32 else 0.0
     least = 2.0 ** -25 if dtype == torch.float16 else 0.0
     return half * want.abs() + ((terms + 4) * step + split) * size + least
+
+
+def allowed_norm(chain, chains):
+    """Largest |result - exact| / |exact| (Frobenius norms) of float32 sums on the tensor cores of random values, sums being ended after
+    `chain` additions and `chains` of them added up.
+
+    An addition to an accumulator cuts off up to a step of the sum, 2^-23, towards zero: half of it on average, and as all of them go one
+    way a chain is short by chain / 2 steps at most (its running sums are no larger on average than its end).  The sum of the chains is short by
+    the same share.  Additions of chains round to nearest, half a step each in no direction: the root of their number.  Products: without
+    lo.lo (2^-22), lo cut to 11 bits in either factor (2^-21 each), the scale on a factor and its two parts' sum half a step each.
+    """
+    return chain / 2 * 2.0 ** -23 + 2.0 ** -22 + 2 * 2.0 ** -21 + chains ** 0.5 * 2.0 ** -24 + 2 * 2.0 ** -24

@@ -163,6 +163,43 @@ def test_linear_of_many_channels(irreps_in, irreps_out, dtype):
     check_linear(irreps_in, irreps_out, dtype, 300, 3, seed=3)
 
 
+CHAIN = 32          # additions to an accumulator: 256 channels, eight an addition
+
+
+@pytest.mark.parametrize("irreps,other", [("256x0e", "80x0e"), ("264x0e", "16x0e"), ("2048x0e", "48x0e"), ("4096x0e", "80x0e"), ("4096x0e", "33x0e"), ("2047x0e", "160x0e"),
+                                          ("1024x0e+512x0e+2048x0e+7x0e", "40x0e"), ("1500x1o", "24x1o"), ("1100x2e+1024x3o", "72x2e+8x3o")])
+def test_float32_sums_over_many_channels(irreps, other):
+    """The error of a sum does not grow with the number of its terms, in the product (many channels in) and in dX (many channels out)."""
+    rows, groups = 150, 2
+    for names in ((irreps, other), (other, irreps)):
+        x, w, dz, index = inputs(*names, F32, rows, groups, 21)
+        lin = oeq.GroupedLinear(*names)
+        xg, wg, dzg = (t.float().cuda().requires_grad_(True) for t in (x, w, dz))
+        z = lin(xg, wg, groups_of(index, groups))
+        dx, = torch.autograd.grad(z, xg, dzg)
+        want_z, want_dx, _ = ref.linear(*names, x, w, index, dz)
+        got, want, a = (z, want_z, names[0]) if names[0] == irreps else (dx, want_dx, names[1])
+        for (_, ir), block in zip(Irreps(other), Irreps(other).slices()):           # (they have different numbers of terms)
+            terms = sum(m for m, of in Irreps(a) if of == ir)
+            e = got.detach().cpu().double()[:, block] - want[:, block]
+            short = float(e.norm() / want[:, block].norm())
+            assert short <= ref.allowed_norm(CHAIN, -(-terms // (8 * CHAIN))), (names, short)
+            assert float(e.abs().max() / want[:, block].abs().max()) < 1e-5
+
+
+def test_float32_sums_over_many_channels_of_many_rows():
+    """Several tiles of rows in each range, an odd number of chunks of results; every run the same."""
+    names, rows, groups = ("700x0e+300x1o", "136x0e+40x1o"), 20_000, 3
+    x, w, dz, index = inputs(*names, F32, rows, groups, 22)
+    lin, plan = oeq.GroupedLinear(*names), groups_of(index, groups)
+    xg, wg, dzg = (t.float().cuda().requires_grad_(True) for t in (x, w, dz))
+    z = lin(xg, wg, plan)
+    dx, dw = torch.autograd.grad(z, (xg, wg), dzg)
+    compare(*names, F32, x, w, dz, index, z, dx, dw)
+    for _ in range(2):
+        assert torch.equal(lin(xg, wg, plan), z)
+
+
 def test_blocks_without_a_path():
     """Irreps that one side alone has, of any degree, and blocks of no channels: zeros, with and without gradients."""
     for names in (("4x0e+2x6e", "3x9o+4x0e"), ("0x1o+4x0e+0x0e", "0x0e+8x0e+0x2e"), ("2x5e", "2x5o")):
