@@ -65,9 +65,22 @@ __device__ __forceinline__ long long gp_cut(long long n, int part, int parts) { 
 constexpr int GP_TILE = 64, GP_STEP = 16, GP_SIMT_THREADS = 256;
 // A 64 x 64 product by 256 threads, 16 values each, over GP_STEP staged steps.  PITCH of a staged step: 16 steps by two rows, which a warp
 // writes, and what it reads lie in different banks, or two at most to a bank (a pitch of 64 values: 120 us instead of 102 with FMAs).
-template <class A> struct GpProduct {           // FMA: 4 rows by 4 columns of a thread
+// LONG: a sum of many terms is added up in chains of 512: the error of one chain grows with its length (FP32, relative, norm: 36 000 terms 3.4e-6, in
+// chains 4.3e-7).  The chains' sum is in shared memory, where it costs no registers (in registers: three CTAs an SM instead of four, 10 000 rows
+// of 256x4e FP32 571 us instead of 526, product).  For FP32 results; 16-bit ones are rounded to 2^-9 and coarser.
+constexpr int GP_CHAIN = 512 / GP_STEP;         // steps
+template <class A, bool LONG> struct GpProduct {            // FMA: 4 rows by 4 columns of a thread
     static constexpr int PITCH = GP_TILE + 2;
     A acc[16] = {};
+    int steps = 0;
+    static __device__ A* chains() {             // of the thread, GP_SIMT_THREADS apart
+        __shared__ A sum[16 * GP_SIMT_THREADS];
+        return sum + threadIdx.x;
+    }
+    __device__ A result(int i) const {
+        if (LONG && steps >= GP_CHAIN) return chains()[i * GP_SIMT_THREADS] + acc[i];
+        return acc[i];
+    }
     static __device__ int row(int i) { return threadIdx.x / 16 * 4 + (i >> 2); }
     static __device__ int col(int i) { return threadIdx.x % 16 * 4 + (i & 3); }
     __device__ void multiply(const A (*a)[PITCH], const A (*b)[PITCH]) {
@@ -82,13 +95,21 @@ template <class A> struct GpProduct {           // FMA: 4 rows by 4 columns of a
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[i] += x[i >> 2] * y[i & 3];
         }
+        if (!LONG || ++steps % GP_CHAIN) return;
+        A* sum = chains();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            sum[i * GP_SIMT_THREADS] = steps == GP_CHAIN ? acc[i] : sum[i * GP_SIMT_THREADS] + acc[i];
+            acc[i] = A(0);
+        }
     }
 };
 // FP64: mma.m8n8k4, rounded as FMAs are; a warp has 16 rows by 32 columns, six values to read for eight products of 8 x 8 x 4 where the FMAs
 // of a thread read eight for sixteen.
-template <> struct GpProduct<double> {
+template <bool LONG> struct GpProduct<double, LONG> {
     static constexpr int PITCH = GP_TILE + 10;
     double acc[16] = {};
+    __device__ double result(int i) const { return acc[i]; }
     static __device__ int row(int i) { return (threadIdx.x >> 6) * 16 + (i >> 3) * 8 + (threadIdx.x & 31) / 4; }
     static __device__ int col(int i) { return (threadIdx.x >> 5 & 1) * 32 + (i >> 1 & 3) * 8 + 2 * (threadIdx.x & 3) + (i & 1); }
     __device__ void multiply(const double (*a)[PITCH], const double (*b)[PITCH]) {
@@ -115,12 +136,13 @@ template <> struct GpProduct<double> {
 // CTA (x, y): entry x of the block table and column y; a column is a target block, 64 of its channels and 64 of the block's up
 // to 64 d (row, component) pairs.  Row y of the grid behind the table writes the zeros of the rows without a group.
 template <class T>
-__global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt(const __grid_constant__ GpProblem gp, const T* __restrict__ X, const T* __restrict__ W,
+__global__ void __launch_bounds__(GP_SIMT_THREADS, sizeof(T) == 4 ? 4 : 0) oeq_grouped_simt(const __grid_constant__ GpProblem gp, const T* __restrict__ X, const T* __restrict__ W,
                                                                     const long long* __restrict__ order, const long long* __restrict__ offsets,
                                                                     const int* __restrict__ table, int blocks, long long rows, int groups,
                                                                     T* __restrict__ Z) {
     typedef typename GpAcc<T>::type A;
-    __shared__ __align__(16) A sa[GP_STEP][GpProduct<A>::PITCH], sb[GP_STEP][GpProduct<A>::PITCH];
+    typedef GpProduct<A, sizeof(T) == 4> Product;
+    __shared__ __align__(16) A sa[GP_STEP][Product::PITCH], sb[GP_STEP][Product::PITCH];
     const int tid = threadIdx.x;
     if ((int)blockIdx.x >= blocks) {            // rows without a group: zeros
         const long long n = min(__ldg(offsets + groups), rows), part = (long long)(blockIdx.x - blocks) * gridDim.y + blockIdx.y;
@@ -151,7 +173,7 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt(const __grid
     }
     const T* w_group = W + (long long)g * gp.w_numel;
     const int kb = gp.transposed ? tid % GP_STEP : tid / 16 % GP_STEP, cb = gp.transposed ? tid / GP_STEP : tid % 16;
-    GpProduct<A> product;
+    Product product;
     A a[4], b[4];
     int p = to.path_begin, u0 = 0;
     auto fetch = [&]() {
@@ -187,7 +209,7 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt(const __grid
     for (int i = 0; i < 16; ++i) {
         const int pair = pair0 + product.row(i), c = c_tile + product.col(i);
         if (pair >= pairs || c >= to.mul) continue;
-        gp_store(Z + gp_row(order, first + pair / d) * gp.dst_dim + to.off + pair % d + c * d, (A)(product.acc[i] * (A)to.scale));
+        gp_store(Z + gp_row(order, first + pair / d) * gp.dst_dim + to.off + pair % d + c * d, (A)(product.result(i) * (A)to.scale));
     }
 }
 
@@ -203,13 +225,14 @@ struct GpSplit {
     int first[GP_PATHS + 1];    // its first CTA
 };
 template <class T>
-__global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __grid_constant__ GpProblem gp, const __grid_constant__ GpSplit split,
+__global__ void __launch_bounds__(GP_SIMT_THREADS, sizeof(T) == 4 ? 4 : 0) oeq_grouped_simt_dw(const __grid_constant__ GpProblem gp, const __grid_constant__ GpSplit split,
                                                                        const T* __restrict__ X, const T* __restrict__ dZ,
                                                                        const long long* __restrict__ order, const long long* __restrict__ offsets,
                                                                        long long rows, int groups, T* __restrict__ dW,
                                                                        typename GpAcc<T>::type* __restrict__ partial, GpStart* __restrict__ starts) {
     typedef typename GpAcc<T>::type A;
-    __shared__ __align__(16) A sa[GP_STEP][GpProduct<A>::PITCH], sb[GP_STEP][GpProduct<A>::PITCH];
+    typedef GpProduct<A, sizeof(T) == 4> Product;
+    __shared__ __align__(16) A sa[GP_STEP][Product::PITCH], sb[GP_STEP][Product::PITCH];
     const int tid = threadIdx.x;
     int p = 0;
     while ((int)blockIdx.x >= split.first[p + 1]) ++p;
@@ -230,7 +253,7 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __g
         }
         const long long stop = min(end, hi);
         const long long pairs = (stop - at) * d;
-        GpProduct<A> product;
+        Product product;
         A a[4], b[4];
         auto fetch = [&](long long k0) {
             const long long k = k0 + k_s;
@@ -261,8 +284,8 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS) oeq_grouped_simt_dw(const __g
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int r = product.row(i), c = product.col(i), u = u_tile + r, w = w_tile + c;
-            if (!whole) tile[r * GP_TILE + c] = product.acc[i];
-            else if (u < path.src_mul && w < to.mul) gp_store(dW + (long long)g * gp.w_numel + path.w_off + (long long)u * path.w_ld + w, (A)(product.acc[i] * (A)to.scale));
+            if (!whole) tile[r * GP_TILE + c] = product.result(i);
+            else if (u < path.src_mul && w < to.mul) gp_store(dW + (long long)g * gp.w_numel + path.w_off + (long long)u * path.w_ld + w, (A)(product.result(i) * (A)to.scale));
         }
         at = stop;
         ++g;

@@ -91,3 +91,9 @@ def allowed_norm(chain, chains):
     lo.lo (2^-22), lo cut to 11 bits in either factor (2^-21 each), the scale on a factor and its two parts' sum half a step each.
     """
     return chain / 2 * 2.0 ** -23 + 2.0 ** -22 + 2 * 2.0 ** -21 + chains ** 0.5 * 2.0 ** -24 + 2 * 2.0 ** -24
+
+
+def allowed_norm_rounded(chain, chains):
+    """The same of sums that round to nearest: half a step of the running sum for each addition, in no direction, the running sums' squares
+    being half of the end's on average; then the sum of the chains in the same way, and the scale and the result."""
+    return ((chain / 2) ** 0.5 + (chains / 2) ** 0.5 + 2) * 2.0 ** -24

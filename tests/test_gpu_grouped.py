@@ -200,6 +200,21 @@ def test_float32_sums_over_many_channels_of_many_rows():
         assert torch.equal(lin(xg, wg, plan), z)
 
 
+@pytest.mark.parametrize("irreps_in,irreps_out,rows", [("1600x4e", "1600x4e", 4000), ("64x4e", "48x4e", 50_000), ("9000x4e", "40x4e", 64)])
+def test_float32_sums_of_high_degrees(irreps_in, irreps_out, rows):
+    """The FMA kernels: long sums of a weight gradient in one range of rows and in many, and of a product."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    lin, a, b = oeq.GroupedLinear(irreps_in, irreps_out), Irreps(irreps_in)[0].mul, Irreps(irreps_out)[0].mul
+    x, dz = (torch.randn(rows, m * 9, device="cuda", generator=gen) for m in (a, b))
+    w = torch.randn(1, a * b, device="cuda", generator=gen).requires_grad_(True)
+    z = lin(x, w, oeq.RowGroups(torch.zeros(rows, dtype=torch.int64, device="cuda"), 1))
+    dw, = torch.autograd.grad(z, w, dz)
+    left, right = (t.double().view(rows, -1, 9).transpose(1, 2).reshape(rows * 9, -1) for t in (x, dz))
+    for got, want, terms in ((z.double().view(rows, b, 9).transpose(1, 2).reshape(rows * 9, b), left @ w.double().view(a, b) / a ** 0.5, a),
+                             (dw.double().view(a, b), left.T @ right / a ** 0.5, rows * 9)):
+        assert float((got - want).norm() / want.norm()) <= ref.allowed_norm_rounded(min(terms, 512), -(-terms // 512))
+
+
 def test_blocks_without_a_path():
     """Irreps that one side alone has, of any degree, and blocks of no channels: zeros, with and without gradients."""
     for names in (("4x0e+2x6e", "3x9o+4x0e"), ("0x1o+4x0e+0x0e", "0x0e+8x0e+0x2e"), ("2x5e", "2x5o")):
