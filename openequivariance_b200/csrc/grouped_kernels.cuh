@@ -133,13 +133,13 @@ template <bool LONG> struct GpProduct<double, LONG> {
 };
 
 // ---------------------------------------------------------------------------- product
-// CTA (x, y): entry x of the block table and column y; a column is a target block, 64 of its channels and 64 of the block's up
+// CTA (x, y): entry x of the block table and column first_column + y; a column is a target block, 64 of its channels and 64 of the block's up
 // to 64 d (row, component) pairs.  Row y of the grid behind the table writes the zeros of the rows without a group.
 template <class T>
 __global__ void __launch_bounds__(GP_SIMT_THREADS, sizeof(T) == 4 ? 4 : 0) oeq_grouped_simt(const __grid_constant__ GpProblem gp, const T* __restrict__ X, const T* __restrict__ W,
                                                                     const long long* __restrict__ order, const long long* __restrict__ offsets,
                                                                     const int* __restrict__ table, int blocks, long long rows, int groups,
-                                                                    T* __restrict__ Z) {
+                                                                    int first_column, T* __restrict__ Z) {
     typedef typename GpAcc<T>::type A;
     typedef GpProduct<A, sizeof(T) == 4> Product;
     __shared__ __align__(16) A sa[GP_STEP][Product::PITCH], sb[GP_STEP][Product::PITCH];
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(GP_SIMT_THREADS, sizeof(T) == 4 ? 4 : 0) oeq_g
     const int g = table[3 * blockIdx.x], n_rows = table[3 * blockIdx.x + 2];
     const long long first = table[3 * blockIdx.x + 1];
     if (g < 0) return;
-    int t = 0, column = blockIdx.y;
+    int t = 0, column = first_column + (int)blockIdx.y;
     for (; t < gp.n_targets; ++t) {
         const int n = (gp.target[t].mul + GP_TILE - 1) / GP_TILE * gp.target[t].d;
         if (column < n) break;

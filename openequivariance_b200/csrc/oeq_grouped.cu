@@ -29,6 +29,7 @@ namespace {
     } while (0)
 
 constexpr int64_t MOST_ROWS = (int64_t(1) << 31) - 1;
+constexpr int MOST_GRID_Y = 65535;
 constexpr size_t SMEM_MOST = 227 * 1024, WORKSPACE_ALIGN = 32;
 
 size_t elem_bytes(int dtype) { return dtype == OEQ_F64 ? 8 : (dtype == OEQ_F32 ? 4 : 2); }
@@ -107,10 +108,12 @@ int simt_product(const GpProblem& gp, int64_t rows, int64_t groups, const void* 
     if (columns == 0) return OEQ_OK;
     int sms = 0;
     if (int rc = sm_count(sms)) return rc;
-    const dim3 grid((unsigned)(n + (sms + columns - 1) / columns), (unsigned)columns);
-    oeq_grouped_simt<T><<<grid, GP_SIMT_THREADS, 0, st>>>(gp, (const T*)X, (const T*)W, (const long long*)order, (const long long*)offsets, blocks, n, rows,
-                                                          (int)groups, (T*)Z);
-    OEQ_CUDA(cudaGetLastError());
+    for (int first = 0; first < columns; first += MOST_GRID_Y) {       // (the zeros with the first columns)
+        const dim3 grid((unsigned)(n + (first ? 0 : (sms + columns - 1) / columns)), (unsigned)std::min(columns - first, MOST_GRID_Y));
+        oeq_grouped_simt<T><<<grid, GP_SIMT_THREADS, 0, st>>>(gp, (const T*)X, (const T*)W, (const long long*)order, (const long long*)offsets, blocks, n, rows,
+                                                              (int)groups, first, (T*)Z);
+        OEQ_CUDA(cudaGetLastError());
+    }
     return OEQ_OK;
 }
 

@@ -215,6 +215,13 @@ def test_float32_sums_of_high_degrees(irreps_in, irreps_out, rows):
         assert float((got - want).norm() / want.norm()) <= ref.allowed_norm_rounded(min(terms, 512), -(-terms // 512))
 
 
+@pytest.mark.parametrize("irreps,dtype", [("4200000x0e", F64), ("40000x64e", F32)])
+def test_more_columns_of_results_than_a_grid_has(irreps, dtype):
+    """Over 65 535 pieces of 64 channels and one component, with rows that have no group."""
+    one = "1x" + irreps.split("x")[1]
+    check_linear(one, irreps, dtype, 5, 2, seed=5, without=0.4)
+
+
 def test_blocks_without_a_path():
     """Irreps that one side alone has, of any degree, and blocks of no channels: zeros, with and without gradients."""
     for names in (("4x0e+2x6e", "3x9o+4x0e"), ("0x1o+4x0e+0x0e", "0x0e+8x0e+0x2e"), ("2x5e", "2x5o")):
