@@ -35,16 +35,15 @@ constexpr size_t SMEM_MOST = 227 * 1024, WORKSPACE_ALIGN = 32;
 size_t elem_bytes(int dtype) { return dtype == OEQ_F64 ? 8 : (dtype == OEQ_F32 ? 4 : 2); }
 bool known_dtype(int dtype) { return dtype == OEQ_F32 || dtype == OEQ_F64 || dtype == OEQ_BF16 || dtype == OEQ_F16; }
 
+constexpr int KNOWN_DEVICES = 64;       // what is kept of a device; of others it is asked for at every call
 int sm_count(int& n) {
-    static int counts[64] = {};         // of the devices; a race writes the same value twice
+    static std::atomic<int> counts[KNOWN_DEVICES];
     int dev = 0;
     OEQ_CUDA(cudaGetDevice(&dev));
-    if (dev < 64 && counts[dev]) {
-        n = counts[dev];
-        return OEQ_OK;
-    }
+    n = dev < KNOWN_DEVICES ? counts[dev].load(std::memory_order_relaxed) : 0;
+    if (n) return OEQ_OK;
     OEQ_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-    if (dev < 64) counts[dev] = n;
+    if (dev < KNOWN_DEVICES) counts[dev].store(n, std::memory_order_relaxed);
     return OEQ_OK;
 }
 
@@ -55,8 +54,8 @@ int allow_smem(size_t most) {
     static std::atomic<uint64_t> done{0};       // a bit for each device
     int dev = 0;
     OEQ_CUDA(cudaGetDevice(&dev));
-    const uint64_t bit = uint64_t(1) << (dev & 63);
-    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return OEQ_OK;
+    const uint64_t bit = dev < KNOWN_DEVICES ? uint64_t(1) << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return OEQ_OK;
     OEQ_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
     done.fetch_or(bit, std::memory_order_release);
     return OEQ_OK;
@@ -84,9 +83,9 @@ Runs runs_of(int64_t rows) {
     return {run, (int)std::max<int64_t>(1, (rows + run - 1) / run)};
 }
 
-// ---------------------------------------------------------------------------- linear maps
-
 }  // namespace
+
+// ---------------------------------------------------------------------------- linear maps
 
 struct oeq_grouped {
     GpProblem forward, backward, weights;       // X -> Z, dZ -> dX, and X -> Z with the paths in the order of their weights

@@ -512,6 +512,37 @@ def test_two_streams():
             assert all(torch.equal(p, q) for p, q in zip(run, want[k]))
 
 
+def test_calls_from_several_threads_at_once():
+    import threading
+    names = "32x0e+16x1o+3x4e", "24x0e+16x1o+5x4e"
+    data = []
+    for seed, dtype in enumerate(TYPES * 2):
+        x, w, dz, index = inputs(*names, dtype, 301, 5, seed)
+        data.append([t.to(dtype).cuda() for t in (x, w, dz)] + [index.cuda()])
+
+    def step(x, w, dz, index):
+        x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        z = oeq.GroupedLinear(*names)(x, w, oeq.RowGroups(index, 5))
+        return (z.detach(), *torch.autograd.grad(z, (x, w), dz))
+
+    want, got = [step(*d) for d in data], [None] * len(data)
+    torch.cuda.synchronize()
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[k] = step(*data[k])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(data))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for run, expected in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(run, expected))
+
+
 def test_more_than_2_to_the_31_values():
     """1.1 million rows of 2 048 values: offsets within the arrays pass 32 bits."""
     names, rows, groups = "128x0e+128x1o+128x2e+128x3o", 1_100_000, 3
