@@ -325,6 +325,47 @@ def test_values_that_are_not_numbers_stay_in_their_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("names", [("64x0e+8x1o+6x2e", "48x0e+8x1o+6x2e"), ("64x0e+16x1o+8x3o", "32x0e+64x1o+8x3o"), ("5x0e+2x4e", "7x0e+2x4e")], ids=["odd", "aligned", "high"])
+def test_gradients_of_values_that_are_not_numbers_stay_in_their_rows_and_groups(names, dtype):
+    """Rows of a product and of dX have their own; a row's numbers reach the weight gradient of its group alone, and a row without a
+    group reaches none."""
+    x, w, dz, index = inputs(*names, dtype, 400, 6, 19, without=0.2)
+    index[index == 4] = 1                                           # a group without rows
+    bad = torch.zeros(400, dtype=torch.bool)
+    bad[[0, 17, 18, 399]] = True
+    index[bad] = torch.tensor([2, -1, 5, 2])
+    value = torch.tensor([float("nan"), float("inf"), -float("inf"), float("nan")], dtype=F64)[:, None]
+    xb, dzb = x.clone(), dz.clone()
+    xb[bad], dzb[bad] = value, value
+    lin, plan = oeq.GroupedLinear(*names), groups_of(index, 6)
+
+    def gradients(x, dz):
+        a, b = (t.to(dtype).cuda().requires_grad_(True) for t in (x, w))
+        return [t.cpu() for t in torch.autograd.grad(lin(a, b, plan), (a, b), dz.to(dtype).cuda())]
+
+    clean_dx, clean_dw = gradients(x, dz)
+    touched, kept = bad & (index >= 0), [0, 1, 3, 4]
+    for dx, dw in (gradients(xb, dz), gradients(x, dzb)):
+        assert torch.equal(dw[kept], clean_dw[kept]) and not dw[4].any()
+        assert not torch.isfinite(dw[[2, 5]]).any()
+    assert torch.equal(gradients(xb, dz)[0], clean_dx)
+    dx = gradients(x, dzb)[0]
+    assert torch.equal(dx[~touched], clean_dx[~touched]) and not torch.isfinite(dx[touched]).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("names", [("128x0e+128x1o+64x2e+1x4e", "128x0e+64x1o+128x2e+1x4e"), ("64x0e+5x2e+64x1o", "64x0e+5x2e+64x1o")], ids=["high", "odd"])
+def test_wide_blocks_beside_one_that_takes_another_way(names, dtype):
+    check_linear(*names, dtype, 700, 5, seed=6)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=TYPE_IDS)
+def test_linear_of_many_channels_and_rows(dtype):
+    """Weights that do not stay in shared memory, many tiles of rows in a CTA's range, many groups in it."""
+    check_linear("520x0e+136x1o", "600x0e+136x1o", dtype, 6001, 40, seed=9)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=TYPE_IDS)
 def test_the_same_result_in_every_run(dtype):
     x, w, dz, index = inputs("64x0e+32x1o", "64x0e+32x1o", dtype, 6001, 5, 3)
     plan, lin = groups_of(index, 5), oeq.GroupedLinear("64x0e+32x1o", "64x0e+32x1o")
@@ -362,6 +403,39 @@ def test_second_derivatives(dtype):
     want_z = ref.linear(*names, ex, w, index) + ref.linear(*names, x, ew, index)
     for got, want in ((gx, want_x), (gw, want_w), (gdz, want_z)):
         assert float((got.cpu().double() - want).abs().max() / want.abs().max()) < (1e-5 if dtype == F32 else 1e-12)
+
+
+@pytest.mark.filterwarnings("ignore:There is a performance drop")
+def test_function_transforms():
+    """torch.func and batched gradients over the op: the same as calls one by one."""
+    names = "8x0e+4x1o", "6x0e+4x1o"
+    x, w, _, index = inputs(*names, F64, 40, 3, 1)
+    x, w, plan = x.cuda(), w.cuda(), groups_of(index, 3)
+    lin, gen = oeq.GroupedLinear(*names), torch.Generator(device="cuda").manual_seed(2)
+    loss = lambda p, q: lin(p, q, plan).square().sum()
+    many = lambda t: torch.randn(5, *t.shape, device="cuda", generator=gen, dtype=F64)
+    xs, ws = many(x), many(w)
+
+    def one_by_one(p, q):
+        p, q = p.clone().requires_grad_(True), q.clone().requires_grad_(True)
+        return torch.autograd.grad(loss(p, q), (p, q))
+
+    for got, want in zip(torch.func.grad(loss, (0, 1))(x, w), one_by_one(x, w)):
+        assert torch.equal(got, want)
+    assert torch.equal(torch.vmap(lambda p: lin(p, w, plan))(xs), torch.stack([lin(p, w, plan) for p in xs]))
+    assert torch.equal(torch.vmap(lambda q: lin(x, q, plan))(ws), torch.stack([lin(x, q, plan) for q in ws]))
+    want = [torch.stack(t) for t in zip(*[one_by_one(p, q) for p, q in zip(xs, ws)])]
+    for got, t in zip(torch.vmap(torch.func.grad(loss, (0, 1)))(xs, ws), want):
+        assert torch.equal(got, t)
+    xg = xs.clone().requires_grad_(True)
+    got, = torch.autograd.grad(torch.vmap(lambda p: lin(p, w, plan))(xg).square().sum(), xg)
+    assert torch.equal(got, torch.stack([one_by_one(p, w)[0] for p in xs]))
+    xg = x.clone().requires_grad_(True)
+    z = lin(xg, w, plan)
+    seeds = many(z)
+    got, = torch.autograd.grad(z, xg, seeds, is_grads_batched=True, retain_graph=True)
+    assert torch.equal(got, torch.stack([torch.autograd.grad(z, xg, e, retain_graph=True)[0] for e in seeds]))
+    assert torch.func.jacrev(torch.func.grad(loss))(x, w).shape == (40, 20, 40, 20)
 
 
 def test_weights_changed_in_place_are_noticed():
