@@ -67,7 +67,7 @@ constexpr int GP_TILE = 64, GP_STEP = 16, GP_SIMT_THREADS = 256;
 // writes, and what it reads lie in different banks, or two at most to a bank (a pitch of 64 values: 120 us instead of 102 with FMAs).
 // LONG: a sum of many terms is added up in chains of 512: the error of one chain grows with its length (FP32, relative, norm: 36 000 terms 3.4e-6, in
 // chains 4.3e-7).  The chains' sum is in shared memory, where it costs no registers (in registers: three CTAs an SM instead of four, 10 000 rows
-// of 256x4e FP32 571 us instead of 526, product).  For FP32 results; 16-bit ones are rounded to 2^-9 and coarser.
+// of 256x4e FP32 571 us instead of 526, product).  For FP32 results; 16-bit ones are rounded by up to 2^-8 and 2^-11.
 constexpr int GP_CHAIN = 512 / GP_STEP;         // steps
 template <class A, bool LONG> struct GpProduct {            // FMA: 4 rows by 4 columns of a thread
     static constexpr int PITCH = GP_TILE + 2;

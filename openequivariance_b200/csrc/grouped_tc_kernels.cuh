@@ -33,8 +33,11 @@ constexpr int GT_D_MAX = 7;
 constexpr int GT_SETS = 3, GT_SET = 4, GT_PW = GT_SETS * GT_SET, GT_EPI_GROUPS = 2, GT_EPI = 4 * GT_EPI_GROUPS, GT_AHEAD = 3, GT_THREADS = (GT_PW + GT_EPI + 1 + GT_AHEAD) * 32;
 constexpr int GT_STAGES = 6;                    // most stages of A
 // FP32: chunks of the sum in one accumulator, 32 additions of eight channels each.  The additions are cut off, not rounded, and all of them
-// one way: relative error (norm) 6.4e-7 at 256 channels, in one chain 4.9e-6 at 2 048 and 9.6e-6 at 4 096.  (16-bit results are rounded to
-// 2^-9 and coarser; their sums are one chain.)
+// one way: relative error (norm) 6.4e-7 at 256 channels, in one chain 4.9e-6 at 2 048 and 9.6e-6 at 4 096, in chains 6.6e-7 at most.  What the
+// drains of more than one chain cost, product: 65 536 rows of 512x0e 277 us instead of 260, 20 000 of 1024x0e 328 instead of 293, 30 000 of 300x1o 225
+// instead of 178 (chains of five and five chunks instead of eight and two: 226).  Kernels of their own (LONG): with the loop in all of them dX of
+// 50 000 rows of 128x(0e+1o+2e+3o) took 225 us instead of 219.  16-bit results are rounded by up to 2^-8 and 2^-11, and an
+// addition takes 16 channels: one chain, short by 5e-6 at 4 096 channels.
 constexpr int GT_CHAIN = 8;
 constexpr int GT_STAGING = 42 * 100 * 4;        // 32 channels of a tile's pairs (three components take most), for each epilogue group
 constexpr int GT_CONTROL = 1536;                // barriers, rows of the tiles that drain, the CTA's range
@@ -429,7 +432,7 @@ __device__ __forceinline__ void gt_settle(unsigned leader, unsigned long long* d
     tc_commit_if(leader, done);
     warp_wait(true, done, 0, &gt_status, ERR_GT_DONE);
 }
-template <class T, bool TRANS, class Wait>
+template <class T, bool TRANS, bool LONG, class Wait>
 __device__ __forceinline__ void gt_multiply(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, unsigned char* a_base,
                                             unsigned char* b_base, const GtBars& bars, GtWalk walk, int tile_rows, unsigned tmem, unsigned leader, Wait&& acc_wait) {
     constexpr int KC = GtType<T>::KC, KSTEP = GtType<T>::KSTEP;
@@ -449,7 +452,7 @@ __device__ __forceinline__ void gt_multiply(const GtProblem& gt, const GtArgs& p
         for (int path_no = to.path_begin; path_no < to.path_end && ok; ++path_no) {
             const int mul = gt.gp.path[path_no].src_mul;
             for (int u0 = 0; u0 < mul && ok; u0 += KC) {
-                if (GtType<T>::SPLIT && in_chain++ == GT_CHAIN) {       // the next accumulator
+                if (LONG && in_chain++ == GT_CHAIN) {       // the next accumulator
                     tc_commit_if(leader, bars.acc_full + (accs & 1));
                     ++accs;
                     if (accs >= 2 && !acc_wait(accs & 1, (unsigned)(accs / 2 - 1) & 1)) {
@@ -486,7 +489,7 @@ __device__ __forceinline__ void gt_multiply(const GtProblem& gt, const GtArgs& p
     }
 }
 
-// ---------------------------------------------------------------------------- epilogue
+// ---------------------------------------------------------------------------- rows of results
 template <class T> struct GtPair { static __device__ unsigned of(float, float) { return 0; } };
 template <> struct GtPair<__nv_bfloat16> {
     static __device__ unsigned of(float a, float b) {
@@ -620,13 +623,13 @@ __device__ __forceinline__ void gt_ahead(const GtProblem& gt, const GtArgs& p, c
     }
 }
 
-// ---------------------------------------------------------------------------- epilogue
+// ---------------------------------------------------------------------------- drain
 // The chunks of 32 channels of all tiles go to the two groups of four warps in turn.  FP32: a tile whose sum has several chains comes as
 // as many accumulators; the results of the first are written and the others added to them, a chunk of channels by the same group each time.
 // acc_wait(buffer, parity): the warp's wait for an accumulator.  A warp whose wait ran out reads and writes nothing more but comes to every
 // barrier of its group: each warp counts its own polls, so the other three may have seen the accumulator complete, and a hardware barrier
 // waits without limit.  (It keeps the rows' numbers up to date: the others write the rows that stand there.)
-template <class T, bool TRANS, int D, class Wait>
+template <class T, bool TRANS, bool LONG, int D, class Wait>
 __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, float* staging,
                                          const GtBars& bars, GtWalk walk, unsigned tmem, int group, int warp, int lane, Wait&& acc_wait) {
     constexpr int TILE_ROWS = gt_tile_rows(D), PITCH = gt_pitch<D>();
@@ -635,7 +638,7 @@ __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, c
     const unsigned quarter = tmem + ((unsigned)(warp * 32) << 16);
     int* rows_of = bars.rows + 128 * group;
     staging += group * (GT_STAGING / 4);
-    const int chains = GtType<T>::SPLIT ? max(1, (tile_of.chunks + GT_CHAIN - 1) / GT_CHAIN) : 1;
+    const int chains = LONG ? (tile_of.chunks + GT_CHAIN - 1) / GT_CHAIN : 1;
     int accs = 0, first_turn = 0;
     bool alive = true;
     for (; walk.more(); walk.next(p.offsets, p.groups)) {
@@ -692,7 +695,7 @@ __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, c
                     if (vec) gt_write<T, D, true>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
                     else gt_write<T, D, false>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
                 } else if (alive) {
-                    if constexpr (GtType<T>::SPLIT) {
+                    if constexpr (LONG) {
                         if (vec) gt_add<D, true>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
                         else gt_add<D, false>(staging, rows_of, walk.rows, z, gt.gp.dst_dim, values, pair);
                     }
@@ -710,11 +713,11 @@ __device__ __forceinline__ void gt_drain(const GtProblem& gt, const GtArgs& p, c
 }
 
 // What a role does for blocks of D components.
-template <class T, bool TRANS, bool FAST, int D>
+template <class T, bool TRANS, bool FAST, bool LONG, int D>
 __device__ __forceinline__ void gt_roles(const GtProblem& gt, const GtArgs& p, const GtTarget& tile_of, const GpTarget& to, int n0, unsigned char* a_base,
                                          unsigned char* b_base, float* staging, const GtBars& bars, const GtWalk& walk, unsigned tmem, int warp, int tid) {
     if (warp < GT_PW) gt_produce<T, TRANS, FAST, D>(gt, p, tile_of, to, n0, a_base, b_base, bars, walk, tid);
-    else gt_drain<T, TRANS, D>(gt, p, tile_of, to, n0, staging, bars, walk, tmem, (warp - GT_PW) >> 2, warp & 3, tid & 31, [&](int buf, unsigned parity) {
+    else gt_drain<T, TRANS, LONG, D>(gt, p, tile_of, to, n0, staging, bars, walk, tmem, (warp - GT_PW) >> 2, warp & 3, tid & 31, [&](int buf, unsigned parity) {
         return warp_wait(true, bars.acc_full + buf, parity, &gt_status, ERR_GT_ACC_FULL);
     });
 }
@@ -748,7 +751,7 @@ __global__ void __launch_bounds__(32) oeq_grouped_issue_probe(const __grid_const
     tc_fence_after();
     const unsigned tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile unsigned*>(bars.tmem), 0);
     const GtArgs p{nullptr, nullptr, nullptr, gt_probe_offsets, nullptr, 3, 3, 0};
-    gt_multiply<float, false>(gt, p, gt.target[0], gt.gp.target[0], gt_smem, b, bars, GtWalk(gt_probe_offsets, 0, 0, 3), 128, tmem, elect_lane(), [&](int, unsigned) { return false; });
+    gt_multiply<float, false, false>(gt, p, gt.target[0], gt.gp.target[0], gt_smem, b, bars, GtWalk(gt_probe_offsets, 0, 0, 3), 128, tmem, elect_lane(), [&](int, unsigned) { return false; });
     const bool over = mbar_test(bars.done, 0);
     if (lane == 0) atomicCAS(&gt_status, 0, over ? ERR_GT_ACC_EMPTY : ERR_GT_DONE);
     tc_fence_before();
@@ -777,7 +780,7 @@ __global__ void __launch_bounds__(32 * GT_EPI) oeq_grouped_drain_probe(const __g
     tc_fence_after();
     const unsigned tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile unsigned*>(bars.tmem), 0);
     const GtArgs p{nullptr, nullptr, nullptr, gt_probe_offsets, gt_probe_z, GT_PROBE_ROWS, GT_PROBE_ROWS, 0};
-    gt_drain<float, false, 1>(gt, p, gt.target[0], gt.gp.target[0], 0, reinterpret_cast<float*>(smem), bars, GtWalk(gt_probe_offsets, 0, 0, GT_PROBE_ROWS), tmem, warp >> 2,
+    gt_drain<float, false, false, 1>(gt, p, gt.target[0], gt.gp.target[0], 0, reinterpret_cast<float*>(smem), bars, GtWalk(gt_probe_offsets, 0, 0, GT_PROBE_ROWS), tmem, warp >> 2,
                               warp & 3, lane, [&](int, unsigned) {
                                   if (warp == lost && lane == 0) atomicCAS(&gt_status, 0, ERR_GT_ACC_FULL);
                                   return warp != lost;
@@ -787,8 +790,8 @@ __global__ void __launch_bounds__(32 * GT_EPI) oeq_grouped_drain_probe(const __g
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
 }
 
-// FAST: every block of rows and weights is made of whole, aligned 16-byte pieces.
-template <class T, bool TRANS, bool FAST>
+// FAST: every block of rows and weights is made of whole, aligned 16-byte pieces.  LONG (FP32): some sum has more than one chain.
+template <class T, bool TRANS, bool FAST, bool LONG>
 __global__ void __launch_bounds__(GT_THREADS, 1) oeq_grouped_tc(const __grid_constant__ GtProblem gt, const GtArgs p) {
     extern __shared__ __align__(1024) unsigned char gt_smem[];
     unsigned char* smem = gt_smem;
@@ -829,13 +832,13 @@ __global__ void __launch_bounds__(GT_THREADS, 1) oeq_grouped_tc(const __grid_con
     const unsigned tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile unsigned*>(bars.tmem), 0);
     const GtWalk walk(p.offsets, range.g, work ? (int)range.lo : 0, work ? (int)range.hi : 0);
     if (warp > MMA_WARP) gt_ahead<T, TRANS>(gt, p, tile_of, to, n0, bars, walk, gt_tile_rows(d), tid - (MMA_WARP + 1) * 32);
-    else if (warp == MMA_WARP) gt_multiply<T, TRANS>(gt, p, tile_of, to, a_base, b_base, bars, walk, gt_tile_rows(d), tmem, elect_lane(), [&](int buf, unsigned parity) {
+    else if (warp == MMA_WARP) gt_multiply<T, TRANS, LONG>(gt, p, tile_of, to, a_base, b_base, bars, walk, gt_tile_rows(d), tmem, elect_lane(), [&](int buf, unsigned parity) {
         return warp_wait(true, bars.acc_empty + buf, parity, &gt_status, ERR_GT_ACC_EMPTY);
     });
-    else if (d == 1) gt_roles<T, TRANS, FAST, 1>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
-    else if (d == 3) gt_roles<T, TRANS, FAST, 3>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
-    else if (d == 5) gt_roles<T, TRANS, FAST, 5>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
-    else gt_roles<T, TRANS, FAST, 7>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
+    else if (d == 1) gt_roles<T, TRANS, FAST, LONG, 1>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
+    else if (d == 3) gt_roles<T, TRANS, FAST, LONG, 3>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
+    else if (d == 5) gt_roles<T, TRANS, FAST, LONG, 5>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
+    else gt_roles<T, TRANS, FAST, LONG, 7>(gt, p, tile_of, to, n0, a_base, b_base, staging, bars, walk, tmem, warp, tid);
     // zeros: the rows without a group, every row where the block has no path
     {
         const long long from = work ? min(__ldg(p.offsets + p.groups), p.rows) : 0, count = p.rows - from;

@@ -243,6 +243,14 @@ int tc_plan(const GpProblem& gp, int64_t rows, int64_t groups, int sms, GtProble
 
 bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
+template <class T, bool TRANS, bool FAST, bool LONG>
+int tc_launch(const GtProblem& gt, const GtArgs& args, int ctas, size_t smem, cudaStream_t st) {
+    if (int rc = allow_smem<oeq_grouped_tc<T, TRANS, FAST, LONG>>(SMEM_MOST)) return rc;
+    oeq_grouped_tc<T, TRANS, FAST, LONG><<<ctas, GT_THREADS, smem, st>>>(gt, args);
+    OEQ_CUDA(cudaGetLastError());
+    return OEQ_OK;
+}
+
 template <class T, bool TRANS>
 int tc_product(const GpProblem& gp, int64_t rows, int64_t groups, const void* X, const void* W, const int64_t* order, const int64_t* offsets, void* Z,
                cudaStream_t st) {
@@ -256,15 +264,12 @@ int tc_product(const GpProblem& gp, int64_t rows, int64_t groups, const void* X,
     constexpr int V = 16 / sizeof(T);
     bool fast = aligned(X, 16) && aligned(W, 16) && gp.src_dim % V == 0 && gp.w_numel % V == 0;
     for (int p = 0; p < gp.n_paths; ++p) fast &= gp.path[p].src_off % V == 0 && gp.path[p].src_mul % V == 0 && gp.path[p].w_off % V == 0 && gp.path[p].w_ld % V == 0;
-    if (fast) {
-        if (int rc = allow_smem<oeq_grouped_tc<T, TRANS, true>>(SMEM_MOST)) return rc;
-        oeq_grouped_tc<T, TRANS, true><<<ctas, GT_THREADS, smem, st>>>(gt, args);
-    } else {
-        if (int rc = allow_smem<oeq_grouped_tc<T, TRANS, false>>(SMEM_MOST)) return rc;
-        oeq_grouped_tc<T, TRANS, false><<<ctas, GT_THREADS, smem, st>>>(gt, args);
+    if constexpr (GtType<T>::SPLIT) {
+        bool is_long = false;
+        for (int t = 0; t < gp.n_targets; ++t) is_long |= gt.target[t].chunks > GT_CHAIN;
+        if (is_long) return fast ? tc_launch<T, TRANS, true, true>(gt, args, ctas, smem, st) : tc_launch<T, TRANS, false, true>(gt, args, ctas, smem, st);
     }
-    OEQ_CUDA(cudaGetLastError());
-    return OEQ_OK;
+    return fast ? tc_launch<T, TRANS, true, false>(gt, args, ctas, smem, st) : tc_launch<T, TRANS, false, false>(gt, args, ctas, smem, st);
 }
 
 // CTAs of the tiles of the weight gradient, one for each SM, dealt by the time that a range of rows takes.

@@ -210,7 +210,7 @@ def test_float32_sums_of_high_degrees(irreps_in, irreps_out, rows):
     z = lin(x, w, oeq.RowGroups(torch.zeros(rows, dtype=torch.int64, device="cuda"), 1))
     dw, = torch.autograd.grad(z, w, dz)
     left, right = (t.double().view(rows, -1, 9).transpose(1, 2).reshape(rows * 9, -1) for t in (x, dz))
-    for got, want, terms in ((z.double().view(rows, b, 9).transpose(1, 2).reshape(rows * 9, b), left @ w.double().view(a, b) / a ** 0.5, a),
+    for got, want, terms in ((z.detach().double().view(rows, b, 9).transpose(1, 2).reshape(rows * 9, b), left @ w.detach().double().view(a, b) / a ** 0.5, a),
                              (dw.double().view(a, b), left.T @ right / a ** 0.5, rows * 9)):
         assert float((got - want).norm() / want.norm()) <= ref.allowed_norm_rounded(min(terms, 512), -(-terms // 512))
 
