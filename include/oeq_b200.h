@@ -235,7 +235,8 @@ int oeq_row_groups_from_counts(int64_t rows, int64_t groups, const int64_t* coun
  * Z[r,o,w,k] = c sum over input blocks i with the irrep of o and channels u of W[group of r][i,o][u,w] X[r,i,u,k], where
  * 1 / c^2 is the number of channels summed.  W is [groups][weight_numel]: the paths (i, o) with i outermost, each
  * [channels of i][channels of o].  Rows without a group get zeros.  dtype: OEQ_F32 (three TF32
- * products on the tensor cores), OEQ_BF16, OEQ_F16 (FP32 sums, rounded once), OEQ_F64.  `order` may be NULL when the rows lie in the order of their groups.
+ * products on the tensor cores), OEQ_BF16, OEQ_F16 (FP32 sums, rounded once), OEQ_F64; a map with a path of l >= 4 runs on FMA kernels in
+ * every type.  `order` may be NULL when the rows lie in the order of their groups.
  * A handle holds no device memory: calls on one may run on any streams and threads at once. */
 typedef struct oeq_grouped oeq_grouped;
 int oeq_grouped_create(const oeq_irrep* in, int n_in, const oeq_irrep* out, int n_out, oeq_grouped** handle);

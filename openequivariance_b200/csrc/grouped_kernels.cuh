@@ -1,12 +1,12 @@
-// Linear maps of irreps with one set of weights for each group of rows, without tcgen05: FP64, and blocks of l = 4 and above of
-// every type.
+// Linear maps of irreps with one set of weights for each group of rows, without tcgen05: FP64, and in every
+// type the maps that have a path of l = 4 or above, all of their paths.
 //
 //   Z[r,o,w,k] = c_o sum_{i,u} W_g[i,o][u,w] X[r,i,u,k],  g = group of row r          (product; dX with W transposed)
 //   dW_g[i,o][u,w] = c_o sum_{r in g, k} X[r,i,u,k] dZ[r,o,w,k]                        (weight gradient)
 //
 // Both kernels are 64 x 64 products in registers, 16 values of a thread; 16 steps of the sum are staged in shared memory while the next 16
-// are on their way in registers.  FP64 goes through mma.m8n8k4 (there is no FP64 kind of tcgen05.mma): 10 007 rows of 64x(0e+1o+2e) 62 us, weight
-// gradient 80, 12 and 9 TFLOP/s; with FMAs 102 and 129.  Bound by latency with two or three CTAs an SM: issue 42 %, load and store unit 49 %, FP64 tensor
+// are on their way in registers.  FP64 goes through mma.m8n8k4 (there is no FP64 kind of tcgen05.mma): 10 007 rows of 64x(0e+1o+2e) 61 us, weight
+// gradient 60 and 20 for the join, 12 and 9 TFLOP/s; with FMAs 102 and 129.  Bound by latency with two or three CTAs an SM: issue 42 %, load and store unit 49 %, FP64 tensor
 // pipe 35 %.
 #pragma once
 #include <cuda_bf16.h>

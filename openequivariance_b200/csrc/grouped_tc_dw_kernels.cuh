@@ -15,8 +15,8 @@
 //   * 8 warps add the accumulators to sums in shared memory at the end of a group and after CHAIN slots: an MMA's additions are cut off, not
 //     rounded, and the error grows with the length of a chain (relative, one chain of 750 slots: 1e-5).  The two accumulators alternate.
 //   * 3 warps prefetch rows to L2, up to two units ahead of the MMAs.
-// Measured from a cold L2 with the sum over ranges, 50 000 rows in 10 groups of 128x(0e+1o+2e+3o) FP32: 234 us (3.5 TB/s); 100 000 rows of 128x(0e+1o+2e)
-// BF16 in 256 groups 133 us; 65 536 rows of 512x0e with 1024x0e BF16 246 us (32 tiles of 128 x 128 read 1.1 GB through L2).  Loads on their way bound it (long
+// Measured from a cold L2 with the sum over ranges, 50 000 rows in 10 groups of 128x(0e+1o+2e+3o) FP32: 235 us (3.5 TB/s); 100 000 rows of 128x(0e+1o+2e)
+// BF16 in 256 groups 133 us; 65 536 rows of 512x0e with 1024x0e BF16 248 us (32 tiles of 128 x 128 read 1.1 GB through L2).  Loads on their way bound it (long
 // scoreboard), with the load and store unit at 56 % and the tensor pipe at 32 %.
 // A CTA has one tile of one path and a range of the sorted rows (gt_range); groups that go beyond the range leave a partial tile for
 // oeq_grouped_join.  Every wait is bounded.

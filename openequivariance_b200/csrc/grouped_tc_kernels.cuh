@@ -19,9 +19,9 @@
 //   * 3 warps prefetch rows and weights to L2, up to two tiles ahead of the MMAs: a producer's loads are half of its time, and registers for
 //     more of them on the way there are none.
 // Two accumulators: a tile (FP32: up to 256 channels of its sum) drains while the next is computed.  Every wait is bounded; on expiry a role records a code and all
-// leave.
-// Measured from a cold L2, 50 000 rows in 10 groups, 128x(0e+1o+2e+3o) FP32: 219 us (3.7 TB/s of rows in and out, 120 TFLOP/s); 100 000 rows in 256
-// groups, 128x(0e+1o+2e) BF16: 143 us (3.4 TB/s).  The load and store unit bounds it (71 % of its wavefronts: rows of several components are read
+// leave, the drain by way of its barriers and the MMA warp once its MMAs are over.
+// Measured from a cold L2, 50 000 rows in 10 groups, 128x(0e+1o+2e+3o) FP32: 227 us (3.6 TB/s of rows in and out, 115 TFLOP/s); 100 000 rows in 256
+// groups, 128x(0e+1o+2e) BF16: 145 us (3.3 TB/s).  The load and store unit bounds it (71 % of its wavefronts: rows of several components are read
 // with a stride of 16 d bytes, results staged with two lanes to a bank), then issue (42 %); the tensor pipe is at 34 % (BF16 9 %).
 #pragma once
 #include "grouped_kernels.cuh"
@@ -790,7 +790,8 @@ __global__ void __launch_bounds__(32 * GT_EPI) oeq_grouped_drain_probe(const __g
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
 }
 
-// FAST: every block of rows and weights is made of whole, aligned 16-byte pieces.  LONG (FP32): some sum has more than one chain.
+// FAST: every block of rows and weights, of all paths, is made of whole, aligned 16-byte pieces; else values are read one by one (16-bit types
+// with spills then: 68 bytes for the product, 12 for dX).  LONG (FP32): some sum has more than one chain.
 template <class T, bool TRANS, bool FAST, bool LONG>
 __global__ void __launch_bounds__(GT_THREADS, 1) oeq_grouped_tc(const __grid_constant__ GtProblem gt, const GtArgs p) {
     extern __shared__ __align__(1024) unsigned char gt_smem[];

@@ -128,6 +128,9 @@ class GroupedLinear:
     in a fixed order, so every result is the same in every run.  In float32 an infinity, a NaN or a number within 2^-12 of
     the largest one gives NaN in the results that it has a part in.
 
+    The kernel is chosen for the map as a whole: with a path of l = 4 or above all of its paths run on FMA kernels in float32, bfloat16
+    and float16 too, and with a multiplicity that is no multiple of 4 (16-bit types: 8) values are read one by one.
+
     An exported or pickled call holds the map's irreps and means the same map in every process that has imported this module.
     """
 

@@ -200,6 +200,20 @@ def test_float32_sums_over_many_channels_of_many_rows():
         assert torch.equal(lin(xg, wg, plan), z)
 
 
+@pytest.mark.parametrize("irreps,rows", [("64x0e", 400_000), ("32x3o", 60_000), ("1400x0e", 30_000)])
+def test_float32_weight_gradients_of_many_rows(irreps, rows):
+    """A sum over all rows, in many ranges and in one (a tile for each CTA)."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    lin, (mul, ir) = oeq.GroupedLinear(irreps, irreps), Irreps(irreps)[0]
+    x, dz = (torch.randn(rows, mul * ir.dim, device="cuda", generator=gen) for _ in range(2))
+    w = torch.zeros(1, mul * mul, device="cuda", requires_grad=True)
+    dw, = torch.autograd.grad(lin(x, w, oeq.RowGroups(torch.zeros(rows, dtype=torch.int64, device="cuda"), 1)), w, dz)
+    left, right = (t.view(rows, mul, ir.dim).transpose(1, 2).reshape(rows * ir.dim, mul).double() for t in (x, dz))
+    want = left.T @ right / mul ** 0.5
+    # (a chain ends with a unit of rows of all components: 35 additions of eight rows at most)
+    assert float((dw.double().view(mul, mul) - want).norm() / want.norm()) <= ref.allowed_norm(35, -(-rows * ir.dim // 256))
+
+
 @pytest.mark.parametrize("irreps_in,irreps_out,rows", [("1600x4e", "1600x4e", 4000), ("64x4e", "48x4e", 50_000), ("9000x4e", "40x4e", 64)])
 def test_float32_sums_of_high_degrees(irreps_in, irreps_out, rows):
     """The FMA kernels: long sums of a weight gradient in one range of rows and in many, and of a product."""
